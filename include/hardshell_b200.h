@@ -404,6 +404,141 @@ int hs_batch_profile(hs_batch* batch, hs_op_profile* out, int cap);
 /* The number of kernel launches of this library in this process (for the benchmark). */
 uint64_t hs_launch_count(void);
 
+/* ---- device-resident operators: drafts that branch ----
+ *
+ * The kernels of the draft trees and beams of a batch (hs_batch_run_tree, hs_batch_beam_step), for
+ * callers whose caches, activations and logits are already on the GPU. No counterpart in the
+ * reference. Every pointer of an argument struct is device memory of the handle's GPU (checked on
+ * the host: HS_BAD_ARGUMENT), and `stream` is a cudaStream_t of that GPU (NULL: the legacy default
+ * stream). A call checks its arguments, launches and returns: it does not wait, allocates nothing,
+ * keeps no state between calls, leaves the caller's current device as it was, and may be captured
+ * into a CUDA graph. Calls on different streams may overlap, except on the same outputs or on a
+ * cache that one of them writes.
+ *
+ * What only the device knows (sequence records, parents, paths) is checked by the kernels: an
+ * entry that is not valid is left out, its outputs as they were, and sets an error word that
+ * hs_dev_check reports. All results are whole numbers, the same for every split of the work. */
+
+/* Waits for `stream` and reports the first error that the device-resident operators of this handle
+ * met on the device since the last check (HS_BAD_ARGUMENT for an entry that is not valid, HS_CUDA
+ * for a failed launch), and clears it. */
+int hs_dev_check(hs_dev* dev, void* stream);
+
+/* A KV cache as a batch keeps it: k [slots][planes][n_ctx][head_dim] and v, transposed,
+ * [slots][planes][head_dim][n_ctx], int8; a plane is one layer and head. slot_stride: the bytes
+ * from a slot to the next in both (0: planes * n_ctx * head_dim). The vector kernels need 16-byte
+ * aligned k, v and slot_stride and n_ctx and head_dim multiples of 16; other caches take byte
+ * kernels. n_ctx at most 8192, head_dim at most 1024, planes at most 65535, slots * planes below
+ * 2^31. */
+typedef struct hs_kv_cache {
+    int8_t* k;
+    int8_t* v;
+    uint64_t slot_stride;
+    uint32_t slots, planes, n_ctx, head_dim;
+} hs_kv_cache;
+
+/* The integer rules of one layer's attention (crates/hardshell/src/gpt2/reference.rs:252-284): the
+ * score and output multipliers and shifts, the softmax precision P <= 30 and the exponent table
+ * (1 to 8192 entries, none negative; copied). Shifts at most 127. */
+typedef struct hs_attn_rule hs_attn_rule;
+int hs_attn_rule_new(hs_dev* dev, int32_t score_m, uint32_t score_s, int32_t out_m, uint32_t out_s, uint32_t softmax_p,
+                     const int32_t* exp_table, uint32_t table_len, hs_attn_rule** out);
+void hs_attn_rule_free(hs_attn_rule* rule);
+
+/* One draft tree: its nodes are rows first_row .. first_row + count - 1 of q and out, and cache
+ * rows prefix .. prefix + count - 1 of `slot` hold their keys and values; the slot's context is
+ * cache rows 0 .. prefix - 1. */
+#define HS_MAX_TREE 128
+typedef struct hs_tree_seq {
+    uint32_t first_row, count, slot, prefix;
+} hs_tree_seq;
+
+/* Attention of trees of drafted tokens over the cache: row r of a tree sees the whole context of
+ * its slot and the nodes whose bits are set in its mask (bit j % 32 of word j / 32 of
+ * mask[r * mask_words ..]: node j; a node sees itself only if its own bit is set). out row r, head
+ * h = clamp(rescale(sum p v, out_m, out_s)) over those keys, p the integer softmax
+ * (crates/hardshell/src/softmax.rs:78-104); a row that sees nothing gets 0. Query head h reads
+ * plane plane0 + h / (n_head / n_kv_head). q and out are int8 rows of n_head * head_dim, q_stride
+ * and out_stride bytes apart (0: dense); rows of no tree stay as they were. count <= max_count <=
+ * HS_MAX_TREE and prefix + count <= max_keys <= n_ctx for every tree, 32 * mask_words >= max_count.
+ * Trees must not share rows. */
+typedef struct hs_tree_attention {
+    hs_kv_cache cache;
+    const int8_t* q;
+    int8_t* out;
+    uint64_t q_stride, out_stride;
+    const hs_tree_seq* seqs;
+    const uint32_t* mask;
+    uint32_t plane0, n_head, n_kv_head, n_rows, n_seq, max_count, max_keys, mask_words;
+} hs_tree_attention;
+int hs_op_tree_attention(hs_attn_rule* rule, const hs_tree_attention* args, void* stream);
+
+/* The logits-to-weights table of a model (crates/hardshell/src/logits.rs:62-72): 1 to 16384 weights
+ * by distance from the row's largest logit, not increasing, the first not 0; copied. */
+typedef struct hs_weight_rule hs_weight_rule;
+int hs_weight_rule_new(hs_dev* dev, const uint64_t* table, uint32_t table_len, hs_weight_rule** out);
+void hs_weight_rule_free(hs_weight_rule* rule);
+
+#define HS_NO_TOKEN 0xFFFFFFFFu
+#define HS_MAX_BEAMS 32
+#define HS_MAX_KEEP 64
+
+/* The selection of a beam search over beams and vocabulary. Group g has the logits rows
+ * g * beams .. g * beams + beams - 1 in the form the LM head leaves them: tops[r * tops_stride + t]
+ * is the largest logit of tile t (2^tile_shift symbols, 6 or 7), dist[r * dist_stride + s] the
+ * distance of symbol s from its tile's largest logit, cut at the table's last entry or beyond. With
+ * D(s) = min(row max - tile max + dist, table_len - 1), w(s) = table[D(s)], W = the sum of w over
+ * the row and N = the number of entries table[j] with table[j] * W > table[0]^2 (the negative log
+ * of 1 / W in units of the table), the candidate (beam, s) costs base[row] + N + D(s); symbols of
+ * weight 0 are no candidates. The `keep` cheapest of a group come back in order, the lower beam and
+ * then the lower symbol first among equal costs: parent (the beam), token and cost of
+ * [groups][keep]. finished (may be NULL): a beam whose byte is not 0 keeps its place as one
+ * candidate of cost base and token HS_NO_TOKEN, and its logits are not read. A beam whose base is
+ * negative or at least 2^62 has no candidates. With fewer than `keep` candidates the rest of
+ * parent and token is HS_NO_TOKEN, of cost -1. The strides count elements (0: dense rows of vocab
+ * symbols and of its tiles); dist must be 16-byte aligned and dist_stride a multiple of 8 for the
+ * vector loads, else it is read by symbols. vocab * table[0] < 2^64, vocab 2 to 65536, beams at
+ * most HS_MAX_BEAMS, keep at most HS_MAX_KEEP. */
+typedef struct hs_beam_select {
+    const uint16_t* dist;
+    const int64_t* tops;
+    uint64_t dist_stride, tops_stride;
+    const int64_t* base;
+    const uint8_t* finished;
+    uint32_t* parent;
+    uint32_t* token;
+    int64_t* cost;
+    uint32_t tile_shift, vocab, groups, beams, keep, reserved;
+} hs_beam_select;
+int hs_op_beam_select(hs_weight_rule* rule, const hs_beam_select* args, void* stream);
+
+/* The reordering of the beams' states after a selection, in place: beam j of group g has the cache
+ * slot slots[g * beams + j] (NULL: slot g * beams + j; the slots of a call must be distinct) and
+ * takes the first rows[g * beams + parent] cache rows (all planes, keys and values) of the beam
+ * parent = parents[g * beams + j] of its group as it was before the call; parent = j or HS_NO_TOKEN
+ * leaves the slot as it is. Rows from rows[..] on stay as they were. */
+typedef struct hs_cache_reorder {
+    hs_kv_cache cache;
+    const uint32_t* slots;
+    const uint32_t* parents;
+    const uint32_t* rows;
+    uint32_t groups, beams;
+} hs_cache_reorder;
+int hs_op_cache_reorder(hs_dev* dev, const hs_cache_reorder* args, void* stream);
+
+/* The commit of an accepted path, in place: with the nodes path[i * path_stride + 0 ..
+ * lengths[i] - 1] of tree seqs[i], strictly increasing and below its count, cache row prefix +
+ * path[j] of its slot moves to row prefix + j, in all planes, keys and values. The other rows stay
+ * as they were. Trees must not share a slot. */
+typedef struct hs_cache_commit {
+    hs_kv_cache cache;
+    const hs_tree_seq* seqs;
+    const uint32_t* path;
+    const uint32_t* lengths;
+    uint32_t n_seq, path_stride;
+} hs_cache_commit;
+int hs_op_cache_commit(hs_dev* dev, const hs_cache_commit* args, void* stream);
+
 /* ---- op-level entry points: the kernels alone, for tests and measurements ----
  * (the reference's op-level path, crates/hardshell-cuda/src/batch/record.rs, and its GEMM tests,
  * crates/hardshell-cuda/tests/ops.rs). Host buffers in and out. */

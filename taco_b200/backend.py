@@ -75,6 +75,41 @@ class FoldStats(ctypes.Structure):
                 ("prep_ms", ctypes.c_double), ("gpu_ms", ctypes.c_double), ("finish_ms", ctypes.c_double)]
 
 
+class KvCacheArgs(ctypes.Structure):
+    """hs_kv_cache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("slot_stride", ctypes.c_uint64)] + \
+               [(n, ctypes.c_uint32) for n in ("slots", "planes", "n_ctx", "head_dim")]
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    """hs_tree_attention."""
+    _fields_ = [("cache", KvCacheArgs), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("q_stride", ctypes.c_uint64), ("out_stride", ctypes.c_uint64), ("seqs", ctypes.c_void_p),
+                ("mask", ctypes.c_void_p)] + \
+               [(n, ctypes.c_uint32) for n in ("plane0", "n_head", "n_kv_head", "n_rows", "n_seq", "max_count",
+                                               "max_keys", "mask_words")]
+
+
+class BeamSelectArgs(ctypes.Structure):
+    """hs_beam_select."""
+    _fields_ = [("dist", ctypes.c_void_p), ("tops", ctypes.c_void_p), ("dist_stride", ctypes.c_uint64),
+                ("tops_stride", ctypes.c_uint64)] + \
+               [(n, ctypes.c_void_p) for n in ("base", "finished", "parent", "token", "cost")] + \
+               [(n, ctypes.c_uint32) for n in ("tile_shift", "vocab", "groups", "beams", "keep", "reserved")]
+
+
+class CacheReorderArgs(ctypes.Structure):
+    """hs_cache_reorder."""
+    _fields_ = [("cache", KvCacheArgs), ("slots", ctypes.c_void_p), ("parents", ctypes.c_void_p),
+                ("rows", ctypes.c_void_p), ("groups", ctypes.c_uint32), ("beams", ctypes.c_uint32)]
+
+
+class CacheCommitArgs(ctypes.Structure):
+    """hs_cache_commit."""
+    _fields_ = [("cache", KvCacheArgs), ("seqs", ctypes.c_void_p), ("path", ctypes.c_void_p),
+                ("lengths", ctypes.c_void_p), ("n_seq", ctypes.c_uint32), ("path_stride", ctypes.c_uint32)]
+
+
 SOURCE_FN = ctypes.CFUNCTYPE(ctypes.c_int64, ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint8), ctypes.c_size_t)
 SINK_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_uint64, ctypes.POINTER(ctypes.c_uint8),
                            ctypes.c_size_t)
@@ -168,6 +203,17 @@ def lib() -> ctypes.CDLL:
     L.hs_op_linear_act.argtypes = [vp, i32, vp, vp, vp, vp, u32, u32, u32, u32, vp, vp]
     L.hs_op_linear_act_noalloc.argtypes = [vp, i32, vp, vp, vp, vp, u32, u32, u32, u32, vp, vp]
     L.hs_op_linear_bench.argtypes = [vp, i32, u32, u32, u32, u64, i32, i32, ctypes.POINTER(ctypes.c_double)]
+    L.hs_dev_check.argtypes = [vp, vp]
+    L.hs_attn_rule_new.argtypes = [vp, ctypes.c_int32, u32, ctypes.c_int32, u32, u32, vp, u32, ctypes.POINTER(vp)]
+    L.hs_attn_rule_free.argtypes = [vp]
+    L.hs_attn_rule_free.restype = None
+    L.hs_weight_rule_new.argtypes = [vp, vp, u32, ctypes.POINTER(vp)]
+    L.hs_weight_rule_free.argtypes = [vp]
+    L.hs_weight_rule_free.restype = None
+    L.hs_op_tree_attention.argtypes = [vp, ctypes.POINTER(TreeAttentionArgs), vp]
+    L.hs_op_beam_select.argtypes = [vp, ctypes.POINTER(BeamSelectArgs), vp]
+    L.hs_op_cache_reorder.argtypes = [vp, ctypes.POINTER(CacheReorderArgs), vp]
+    L.hs_op_cache_commit.argtypes = [vp, ctypes.POINTER(CacheCommitArgs), vp]
     L.hs_batch_set_profiling.argtypes = [vp, i32]
     L.hs_batch_profile.argtypes = [vp, vp, i32]
     L.hs_launch_count.argtypes = []
@@ -185,6 +231,13 @@ def _check(rc: int):
 
 def _p(a: np.ndarray) -> ctypes.c_void_p:
     return ctypes.c_void_p(a.ctypes.data)
+
+
+def _ptr(x) -> int | None:
+    """The device address of a tensor (an object with data_ptr()), an address, or None."""
+    if x is None:
+        return None
+    return x.data_ptr() if hasattr(x, "data_ptr") else int(x)
 
 
 def launch_count() -> int:
@@ -493,6 +546,10 @@ class CudaDevice:
         _check(lib().hs_mem_info(self.h, ctypes.byref(f), ctypes.byref(t)))
         return f.value, t.value
 
+    def check(self, stream: int = 0):
+        """hs_dev_check: waits for the stream and raises what the device-resident operators met."""
+        _check(lib().hs_dev_check(self.h, stream))
+
     def linear_act(self, A: np.ndarray, W: np.ndarray, bias: np.ndarray, mult: np.ndarray, shift: int,
                    path: str = "tc") -> np.ndarray:
         """The linear op alone: clamp(rescale(A . W^T + b, m, s), -127, 127) (tests)."""
@@ -775,3 +832,122 @@ class CudaBatch:
                                             freq_bits, _p(out), total, _p(toff), _p(status)))
         toks = [out[int(toff[i]):int(toff[i]) + int(cnt[i])].copy() for i in range(n)]
         return toks, status[:n].copy()
+
+
+# ---- device-resident operators: drafts that branch ----
+#
+# Arguments are device addresses or tensors of the device (anything with data_ptr()); an operator
+# object holds them, and run(stream) launches it on a CUDA stream (its address; 0 is the legacy
+# default stream). The objects keep their tensors alive. CudaDevice.check(stream) waits and raises the
+# errors that the kernels met.
+
+NO_TOKEN = 0xFFFFFFFF
+MAX_TREE, MAX_BEAMS, MAX_KEEP = 128, 32, 64
+
+
+class _Rule:
+    """A device copy of a model's table and rules, freed with its device."""
+    _free = ""
+
+    def __init__(self, device: CudaDevice):
+        if not device.h:
+            raise HardShellError(HS_BAD_ARGUMENT, "the device is closed")
+        self.device = device
+        self.h = ctypes.c_void_p()
+
+    def close(self):
+        if getattr(self, "h", None):
+            getattr(lib(), self._free)(self.h)
+            self.h = None
+
+    def __del__(self):
+        self.close()
+
+
+class AttnRule(_Rule):
+    """hs_attn_rule: the integer rules of one layer's attention."""
+    _free = "hs_attn_rule_free"
+
+    def __init__(self, device: CudaDevice, score_m: int, score_s: int, out_m: int, out_s: int, softmax_p: int,
+                 exp_table):
+        super().__init__(device)
+        t = np.ascontiguousarray(exp_table, dtype=np.int32)
+        _check(lib().hs_attn_rule_new(device.h, score_m, score_s, out_m, out_s, softmax_p, _p(t), t.size,
+                                      ctypes.byref(self.h)))
+        device._children.add(self)
+
+
+class WeightRule(_Rule):
+    """hs_weight_rule: the logits-to-weights table of a model."""
+    _free = "hs_weight_rule_free"
+
+    def __init__(self, device: CudaDevice, table):
+        super().__init__(device)
+        t = np.ascontiguousarray(table, dtype=np.uint64)
+        _check(lib().hs_weight_rule_new(device.h, _p(t), t.size, ctypes.byref(self.h)))
+        device._children.add(self)
+
+
+class KvCache:
+    """hs_kv_cache: keys [slots, planes, n_ctx, head_dim] and values [slots, planes, head_dim, n_ctx]."""
+
+    def __init__(self, k, v, slots: int, planes: int, n_ctx: int, head_dim: int, slot_stride: int = 0):
+        self.keep = (k, v)
+        self.args = KvCacheArgs(_ptr(k), _ptr(v), slot_stride, slots, planes, n_ctx, head_dim)
+
+
+class _DeviceOp:
+    """One bound call of a device-resident operator."""
+
+    def __init__(self, name: str, handle, args, keep):
+        self._fn, self._handle, self._args, self._keep = getattr(lib(), name), handle, args, keep
+        self._ref = ctypes.byref(args)
+
+    def run(self, stream: int = 0):
+        if not self._handle.h:
+            raise HardShellError(HS_BAD_ARGUMENT, "the handle is closed")
+        rc = self._fn(self._handle.h, self._ref, stream)
+        if rc:
+            _check(rc)
+
+
+class TreeAttention(_DeviceOp):
+    """hs_op_tree_attention."""
+
+    def __init__(self, rule: AttnRule, cache: KvCache, heads: int, kv_heads: int, q, out, rows: int, seqs, n_seq: int,
+                 max_count: int, max_keys: int, mask, mask_words: int, plane0: int = 0, q_stride: int = 0,
+                 out_stride: int = 0):
+        args = TreeAttentionArgs(cache.args, _ptr(q), _ptr(out), q_stride, out_stride, _ptr(seqs), _ptr(mask), plane0,
+                                 heads, kv_heads, rows, n_seq, max_count, max_keys, mask_words)
+        super().__init__("hs_op_tree_attention", rule, args, (cache, q, out, seqs, mask))
+
+
+class BeamSelect(_DeviceOp):
+    """hs_op_beam_select."""
+
+    def __init__(self, rule: WeightRule, dist, tops, vocab: int, groups: int, beams: int, keep: int, base, parent,
+                 token, cost, finished=None, dist_stride: int | None = None, tops_stride: int | None = None,
+                 tile_shift: int = 7):
+        if dist_stride is None:
+            dist_stride = dist.stride(0) if hasattr(dist, "stride") else 0
+        if tops_stride is None:
+            tops_stride = tops.stride(0) if hasattr(tops, "stride") else 0
+        args = BeamSelectArgs(_ptr(dist), _ptr(tops), dist_stride, tops_stride, _ptr(base), _ptr(finished),
+                              _ptr(parent), _ptr(token), _ptr(cost), tile_shift, vocab, groups, beams, keep, 0)
+        super().__init__("hs_op_beam_select", rule, args, (dist, tops, base, finished, parent, token, cost))
+
+
+class CacheReorder(_DeviceOp):
+    """hs_op_cache_reorder."""
+
+    def __init__(self, device: CudaDevice, cache: KvCache, groups: int, beams: int, parent, rows, slots=None):
+        args = CacheReorderArgs(cache.args, _ptr(slots), _ptr(parent), _ptr(rows), groups, beams)
+        super().__init__("hs_op_cache_reorder", device, args, (cache, slots, parent, rows))
+
+
+class CacheCommit(_DeviceOp):
+    """hs_op_cache_commit."""
+
+    def __init__(self, device: CudaDevice, cache: KvCache, seqs, n_seq: int, path, path_ld: int, length):
+        args = CacheCommitArgs(cache.args, _ptr(seqs), _ptr(path), _ptr(length), n_seq, path_ld)
+        super().__init__("hs_op_cache_commit", device, args, (cache, seqs, path, length))

@@ -10,6 +10,10 @@
 // is launched with more CTAs than scratch slots. The first code written stays.
 constexpr int ERR_CODER_DIVISION = 40;
 constexpr int ERR_ATTN_SCRATCH = 41;
+// The draft operators: a sequence record, a parent or slot, or a path that is not valid.
+constexpr int ERR_DRAFT_SEQ = 42;
+constexpr int ERR_DRAFT_PARENT = 43;
+constexpr int ERR_DRAFT_PATH = 44;
 
 namespace hs {
 

@@ -1,0 +1,75 @@
+// The kernels of drafts that branch: attention of draft trees, beam selection, and the moves of
+// cache rows (beams' states, accepted paths). Launchers; every argument is checked by the caller.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "hs_device.hpp"
+
+namespace hs {
+
+constexpr int MAX_TREE = 128;
+constexpr int MAX_BEAMS = 32;
+constexpr int MAX_KEEP = 64;
+constexpr int ATTN_TABLE_MAX = 8192;
+
+// A cache and its geometry (hs_kv_cache with the stride filled in).
+struct CacheView {
+    int8_t* k;
+    int8_t* v;
+    uint64_t slot_stride;
+    uint32_t slots, planes;
+    int n_ctx, hd;
+    bool vec;  // 16-byte vectors fit every row of k and v
+};
+
+struct AttnRuleView {
+    int32_t sm, om;
+    int ss, os, P, tlen;
+    const int32_t* table;  // padded to 4 entries
+};
+
+// hs_tree_seq on the device.
+struct TreeSeq {
+    uint32_t first_row, count, slot, prefix;
+};
+
+struct TreeArgs {
+    CacheView cache;
+    AttnRuleView rule;
+    const int8_t* q;
+    int8_t* out;
+    uint64_t q_stride, out_stride;
+    const TreeSeq* seqs;
+    const uint32_t* mask;
+    uint32_t plane0, n_rows, n_seq;
+    int n_head, n_kv, max_count, max_keys, mask_words;
+};
+
+// hs_beam_select, with the table of the weight rule.
+struct BeamArgs {
+    const uint16_t* dist;
+    const int64_t* tops;
+    uint64_t dist_stride, tops_stride;
+    const int64_t* base;
+    const uint8_t* finished;
+    uint32_t* parent;
+    uint32_t* token;
+    int64_t* cost;
+    const uint64_t* table;
+    int tlen, last_weight;  // the last entry that is not 0
+    int tsh, vocab, groups, beams, keep;
+};
+
+cudaError_t configure_draft_kernels();
+cudaError_t launch_tree_attention(const TreeArgs& a, int num_sms, int* err, cudaStream_t st);
+cudaError_t launch_beam_select(const BeamArgs& a, int num_sms, cudaStream_t st);
+cudaError_t launch_cache_reorder(const CacheView& c, const uint32_t* slots, const uint32_t* parents,
+                                 const uint32_t* rows, uint32_t groups, uint32_t beams, int num_sms, int* err,
+                                 cudaStream_t st);
+cudaError_t launch_cache_commit(const CacheView& c, const TreeSeq* seqs, const uint32_t* path, const uint32_t* lengths,
+                                uint32_t n_seq, uint32_t path_stride, int num_sms, int* err, cudaStream_t st);
+
+}  // namespace hs

@@ -14,11 +14,23 @@ int host_fail(int code, const std::string& msg);
 #include <cstdint>
 #include <vector>
 
+struct hs_dev;
 struct hs_model;
 struct hs_batch;
 struct hs_tokenizer;
 
 namespace hs {
+
+// Counts one kernel launch of the process (hs_launch_count).
+void count_launch();
+
+// The device of a handle: its ordinal, its SM count and the error word of the device-resident
+// operators (apart from the batches' own).
+struct DevInfo {
+    int ordinal, num_sms;
+    int* op_err;
+};
+DevInfo dev_info(const hs_dev* dev);
 
 // The model of a batch, and its slot count.
 hs_model* batch_model(hs_batch* b);

@@ -23,6 +23,7 @@
 
 #include "../../include/hardshell_b200.h"
 #include "hs_device.hpp"
+#include "hs_draft.hpp"
 #include "hs_kernels.cuh"
 #include "hs_host.hpp"
 #include "hsm_file.hpp"
@@ -78,7 +79,8 @@ struct hs_dev {
     int ordinal = 0;
     int num_sms = 0;
     std::string name;
-    int* d_err = nullptr;
+    int* d_err = nullptr;     // the batches' error word
+    int* d_op_err = nullptr;  // the error word of the device-resident operators
     EncodeTiledFn encode = nullptr;
 };
 
@@ -1355,11 +1357,13 @@ int hs_open(int ordinal, hs_dev** out) {
     CK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
     if (!fn || q != cudaDriverEntryPointSuccess) return fail(HS_CUDA, "cuTensorMapEncodeTiled is not available");
     d->encode = (EncodeTiledFn)fn;
-    CK(cudaMalloc(&d->d_err, sizeof(int)));
-    CK(cudaMemset(d->d_err, 0, sizeof(int)));
+    CK(cudaMalloc(&d->d_err, 2 * sizeof(int)));
+    CK(cudaMemset(d->d_err, 0, 2 * sizeof(int)));
+    d->d_op_err = d->d_err + 1;
     CK(configure_core_kernels());
     CK(configure_tc_kernels());
     CK(configure_attn_tc());
+    CK(configure_draft_kernels());
     *out = d.release();
     return HS_OK;
 }
@@ -1832,6 +1836,8 @@ int hs_op_linear_act(hs_dev* dev, int path, const int8_t* A, const int8_t* W, co
 
 }  // extern "C"
 
+void hs::count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+hs::DevInfo hs::dev_info(const hs_dev* dev) { return DevInfo{dev->ordinal, dev->num_sms, dev->d_op_err}; }
 hs_model* hs::batch_model(hs_batch* b) { return b->model; }
 uint32_t hs::batch_slots(const hs_batch* b) { return (uint32_t)b->slots; }
 uint32_t hs::batch_max_rows(const hs_batch* b) { return (uint32_t)b->max_rows; }
