@@ -172,6 +172,56 @@ int hs_batch_room(hs_batch* batch, uint32_t slot, uint64_t* room);
  * the last one. The slot does not change on an error. */
 int hs_batch_truncate(hs_batch* batch, uint32_t slot, uint64_t len);
 
+/* No token (a node without a parent, a beam without a next token), and the largest tree of a slot. */
+#define HS_NO_TOKEN 0xFFFFFFFFu
+#define HS_MAX_TREE 128
+
+/* ---- drafts that branch ----
+ *
+ * No counterpart in the reference, whose speculative decoding drafts one chain and truncates it
+ * (batch/stream.rs). A drafter proposes several continuations of a slot as a tree; one pass gives
+ * the tables of all its nodes; the caller walks the tree with its range decoder and commits the
+ * path that was right. All results equal those of the tokens run one by one. */
+
+/* One pass over draft trees: node i is token tokens[i] after its parent, node parents[i] < i of the
+ * same slot, or after the slot's context (HS_NO_TOKEN). The nodes of a slot are together, at most
+ * HS_MAX_TREE, and fit in its context (hs_batch_room; a tree never restarts a context); all nodes
+ * fit in one pass (max_rows). Query q asks the table after node query_nodes[q], as
+ * hs_batch_run_coded asks (kinds, values, out); a node may be asked any number of times, or not. The
+ * positions and streams of the slots do not change: hs_batch_tree_commit takes the accepted
+ * nodes. The trees end with the next call of the batch that runs rows, truncates or commits; a
+ * reset ends its slot's. After an error no position changed and there are no trees. */
+int hs_batch_run_tree(hs_batch* batch, uint32_t n, const uint32_t* slots, const uint32_t* tokens, const uint32_t* parents,
+                      uint32_t n_queries, const uint32_t* query_nodes, const uint32_t* kinds, const uint64_t* values,
+                      uint32_t freq_bits, hs_interval* out);
+
+/* More queries on the tables of the last hs_batch_run_tree, before or after its commit (a target
+ * that is known only once the intervals before it are consumed). HS_BAD_ARGUMENT once another call
+ * ran rows on the batch. */
+int hs_batch_tree_query(hs_batch* batch, uint32_t n, const uint32_t* nodes, const uint32_t* kinds, const uint64_t* values,
+                        uint32_t freq_bits, hs_interval* out);
+
+/* The nodes become inputs of their slots, as if hs_batch_run_coded had run their tokens: for each
+ * slot a path from its context, each node the parent of the next, the nodes of a slot together.
+ * Slots without a node stay as they were before the trees. All trees end. The cache rows move on
+ * the GPU without a wait. Nothing changes on an error. */
+int hs_batch_tree_commit(hs_batch* batch, uint32_t n, const uint32_t* nodes);
+
+/* One step of a beam search with the model (a drafter): beam j of group g, i = g * beams + j, runs
+ * token tokens[i] in slot slots[i] (distinct slots, contexts that are not full); of all
+ * continuations of a group the `beams` cheapest become its new beams, by the costs of
+ * hs_op_beam_select (whole units of the model's logit table) on top of costs[i] (below 2^62;
+ * negative: a dead beam, not run). finished (may be NULL): a beam whose byte is not 0 does not run
+ * and competes with its cost as it is. On return new beam i has its slot, next token, cost, parent
+ * (the place in its group it came from) and finished byte in the same arrays, cheapest first; a
+ * beam that carries on a finished one has token HS_NO_TOKEN; without enough candidates the last
+ * beams are dead (parent HS_NO_TOKEN, cost -1) and their slots empty. The states of the slots follow
+ * the beams: the first child of a beam stays in its slot, the others get copies. A slot that
+ * received a copy cannot truncate before its last context restart. After an error the costs,
+ * tokens and slots are as before, no position changed. */
+int hs_batch_beam_step(hs_batch* batch, uint32_t groups, uint32_t beams, uint32_t* slots, uint32_t* tokens, int64_t* costs,
+                       uint8_t* finished, uint32_t* parents);
+
 /* The unfold of n coded blocks with the range decoder on the device. It replaces the host loop
  * of crates/taco/src/gpu_unfold.rs:100-160 (codec.rs BlockDecoder over run_coded with Decode
  * queries, one host round trip per token) for the coded blocks of a job. Block i is reset into
@@ -448,7 +498,6 @@ void hs_attn_rule_free(hs_attn_rule* rule);
 /* One draft tree: its nodes are rows first_row .. first_row + count - 1 of q and out, and cache
  * rows prefix .. prefix + count - 1 of `slot` hold their keys and values; the slot's context is
  * cache rows 0 .. prefix - 1. */
-#define HS_MAX_TREE 128
 typedef struct hs_tree_seq {
     uint32_t first_row, count, slot, prefix;
 } hs_tree_seq;
@@ -479,7 +528,6 @@ typedef struct hs_weight_rule hs_weight_rule;
 int hs_weight_rule_new(hs_dev* dev, const uint64_t* table, uint32_t table_len, hs_weight_rule** out);
 void hs_weight_rule_free(hs_weight_rule* rule);
 
-#define HS_NO_TOKEN 0xFFFFFFFFu
 #define HS_MAX_BEAMS 32
 #define HS_MAX_KEEP 64
 

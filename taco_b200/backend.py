@@ -203,6 +203,10 @@ def lib() -> ctypes.CDLL:
     L.hs_op_linear_act.argtypes = [vp, i32, vp, vp, vp, vp, u32, u32, u32, u32, vp, vp]
     L.hs_op_linear_act_noalloc.argtypes = [vp, i32, vp, vp, vp, vp, u32, u32, u32, u32, vp, vp]
     L.hs_op_linear_bench.argtypes = [vp, i32, u32, u32, u32, u64, i32, i32, ctypes.POINTER(ctypes.c_double)]
+    L.hs_batch_run_tree.argtypes = [vp, u32, vp, vp, vp, u32, vp, vp, vp, u32, vp]
+    L.hs_batch_tree_query.argtypes = [vp, u32, vp, vp, vp, u32, vp]
+    L.hs_batch_tree_commit.argtypes = [vp, u32, vp]
+    L.hs_batch_beam_step.argtypes = [vp, u32, u32, vp, vp, vp, vp, vp]
     L.hs_dev_check.argtypes = [vp, vp]
     L.hs_attn_rule_new.argtypes = [vp, ctypes.c_int32, u32, ctypes.c_int32, u32, u32, vp, u32, ctypes.POINTER(vp)]
     L.hs_attn_rule_free.argtypes = [vp]
@@ -807,6 +811,53 @@ class CudaBatch:
     def truncate(self, slot: int, length: int):
         """CudaBatch::truncate: keep the first `length` inputs of `slot`."""
         _check(lib().hs_batch_truncate(self.h, slot, length))
+
+    def run_tree(self, slots, tokens, parents, query_nodes=(), kinds=(), values=(), freq_bits: int = 32) -> np.ndarray:
+        """hs_batch_run_tree: one pass over draft trees; parents[i] is a node before i of its slot, or
+        NO_TOKEN (or -1) for a child of the context. The answers of the queries."""
+        s = np.ascontiguousarray(slots, dtype=np.uint32)
+        t = np.ascontiguousarray(tokens, dtype=np.uint32)
+        p = np.ascontiguousarray(np.asarray(parents, dtype=np.int64) & 0xFFFFFFFF, dtype=np.uint32)
+        if not s.size == t.size == p.size:
+            raise HardShellError(HS_LENGTH_MISMATCH, "slots, tokens and parents differ in length")
+        nodes, k, v, out = self._queries(query_nodes, kinds, values)
+        _check(lib().hs_batch_run_tree(self.h, s.size, _p(s), _p(t), _p(p), nodes.size, _p(nodes), _p(k), _p(v),
+                                       freq_bits, _p(out)))
+        return out
+
+    @staticmethod
+    def _queries(nodes, kinds, values):
+        n = np.ascontiguousarray(nodes, dtype=np.uint32)
+        k = np.ascontiguousarray(kinds, dtype=np.uint32)
+        v = np.ascontiguousarray(values, dtype=np.uint64)
+        if not n.size == k.size == v.size:
+            raise HardShellError(HS_LENGTH_MISMATCH, "the nodes and the queries differ in length")
+        return n, k, v, np.zeros(n.size, dtype=INTERVAL_DTYPE)
+
+    def tree_query(self, nodes, kinds, values, freq_bits: int = 32) -> np.ndarray:
+        """hs_batch_tree_query: more answers from the tables of the last run_tree."""
+        n, k, v, out = self._queries(nodes, kinds, values)
+        _check(lib().hs_batch_tree_query(self.h, n.size, _p(n), _p(k), _p(v), freq_bits, _p(out)))
+        return out
+
+    def tree_commit(self, nodes):
+        """hs_batch_tree_commit: the nodes (a path from the context for each slot) become inputs."""
+        n = np.ascontiguousarray(nodes, dtype=np.uint32)
+        _check(lib().hs_batch_tree_commit(self.h, n.size, _p(n)))
+
+    def beam_step(self, groups: int, beams: int, slots, tokens, costs, finished=None):
+        """hs_batch_beam_step: (slots, tokens, costs, finished, parents) of the new beams."""
+        n = groups * beams
+        s = np.array(slots, dtype=np.uint32)
+        t = np.array(tokens, dtype=np.uint32)
+        c = np.array(costs, dtype=np.int64)
+        f = np.zeros(n, np.uint8) if finished is None else np.array(finished, dtype=np.uint8)
+        if not s.size == t.size == c.size == f.size == n:
+            raise HardShellError(HS_LENGTH_MISMATCH, "the beams' arrays need groups * beams entries")
+        parents = np.zeros(n, dtype=np.uint32)
+        _check(lib().hs_batch_beam_step(self.h, groups, beams, _p(s), _p(t), _p(c),
+                                        None if finished is None else _p(f), _p(parents)))
+        return s, t, c, f, parents
 
     def decode_blocks(self, slots, payloads, counts, freq_bits: int = 32):
         """hs_batch_decode_blocks: block i (the range-coded bytes payloads[i], counts[i] tokens) is

@@ -45,8 +45,9 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_select(const BeamArgs a) 
             s_best[b][0] = 0;
         }
         if (dead || fin) continue;
-        const uint16_t* dist = a.dist + row * a.dist_stride;
-        const int64_t* tops = a.tops + row * a.tops_stride;
+        const size_t lrow = a.row_of ? a.row_of[row] : row;
+        const uint16_t* dist = a.dist + lrow * a.dist_stride;
+        const int64_t* tops = a.tops + lrow * a.tops_stride;
         __syncthreads();
         if (tid == 0) {
             s_max = INT64_MIN;

@@ -53,6 +53,7 @@ struct BeamArgs {
     const uint16_t* dist;
     const int64_t* tops;
     uint64_t dist_stride, tops_stride;
+    const uint32_t* row_of;  // the logits row of each beam (null: beam i has row i)
     const int64_t* base;
     const uint8_t* finished;
     uint32_t* parent;

@@ -53,11 +53,11 @@ __device__ uint64_t block_sum64(uint64_t v, uint64_t* sh) {
 // ---- embeddings (crates/hardshell/src/gpt2/ops.rs:52 embed) ----
 
 __global__ void k_embed(const RowInfo* rows, int R, const int8_t* wte, int ldw, const int32_t* em, int es,
-                        const int8_t* wpe, const int32_t* pm, int ps, int d, int32_t* x) {
+                        const int8_t* wpe, const int32_t* pm, int ps, int d, const uint32_t* at, int32_t* x) {
     int r = blockIdx.x;  // rows in x: a pass can have more than 65,535 of them
     int j = blockIdx.y * blockDim.x + threadIdx.x;
     if (r >= R || j >= d) return;
-    uint32_t tok = rows[r].token, pos = rows[r].pos;
+    uint32_t tok = rows[r].token, pos = at ? at[r] : rows[r].pos;
     int64_t a = rescale64(wte[(size_t)tok * ldw + j], em[tok], es);
     int64_t b = rescale64(wpe[(size_t)pos * d + j], pm[pos], ps);
     x[(size_t)r * d + j] = (int32_t)clamp64(a + b, -RESIDUAL_LIMIT, RESIDUAL_LIMIT);
@@ -767,7 +767,7 @@ constexpr int CODER_MAX_STEPS = 32;  // steps of 256 symbols per warp: V <= 8 * 
 __global__ void __launch_bounds__(CODER_THREADS) k_coder(const uint16_t* d16, int ldd, const int64_t* tmax, int ldt,
                                                          int tsh, int R, int V, const uint64_t* table, int tlen,
                                                          int head, uint32_t bits, const RowInfo* rows, uint64_t* out,
-                                                         int* err) {
+                                                         int* err, const int* lrow) {
     extern __shared__ __align__(16) uint32_t F[];  // counts, then 1 + floor(table[j] * spare / W), j <= dmax
     __shared__ int64_t red[32];
     __shared__ uint64_t redu[32];
@@ -775,8 +775,9 @@ __global__ void __launch_bounds__(CODER_THREADS) k_coder(const uint16_t* d16, in
     __shared__ uint64_t steps[CODER_WARPS][CODER_MAX_STEPS];
     const int r = blockIdx.x;
     if (r >= R) return;
-    const uint16_t* dr = d16 + (size_t)r * ldd;
-    const int64_t* tr = tmax + (size_t)r * ldt;
+    const size_t lr = lrow ? (size_t)lrow[r] : (size_t)r;  // the logits row of the query
+    const uint16_t* dr = d16 + lr * ldd;
+    const int64_t* tr = tmax + lr * ldt;
     const int VT = (V + (1 << tsh) - 1) >> tsh;  // logits tiles of 2^tsh columns
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int32_t last = tlen - 1;
@@ -1534,10 +1535,11 @@ cudaError_t configure_core_kernels() {
 }
 
 void launch_embed(const RowInfo* rows, int R, const int8_t* wte, int ldw, const int32_t* em, int es,
-                  const int8_t* wpe, const int32_t* pm, int ps, int d, int32_t* x, cudaStream_t st) {
+                  const int8_t* wpe, const int32_t* pm, int ps, int d, int32_t* x, cudaStream_t st,
+                  const uint32_t* at) {
     if (R <= 0) return;
     dim3 grid(R, (d + 255) / 256);
-    k_embed<<<grid, 256, 0, st>>>(rows, R, wte, ldw, em, es, wpe, pm, ps, d, x);
+    k_embed<<<grid, 256, 0, st>>>(rows, R, wte, ldw, em, es, wpe, pm, ps, d, at, x);
 }
 
 void launch_layernorm(const int32_t* x, int R, int d, const LnDev& ln, int ln_k, int ln_j, uint64_t eps,
@@ -1611,10 +1613,10 @@ void launch_attention(const RowInfo* rows, int R, const int* rowlist, int n, con
 
 void launch_coder(const uint16_t* d16, int ldd, const int64_t* tmax, int ldt, int tsh, int R, int V,
                   const uint64_t* table, int tlen, int head, uint32_t bits, const RowInfo* rows, uint64_t* out,
-                  int* err, cudaStream_t st) {
+                  int* err, cudaStream_t st, const int* lrow) {
     if (R <= 0) return;
     k_coder<<<R, CODER_THREADS, (size_t)tlen * 4, st>>>(d16, ldd, tmax, ldt, tsh, R, V, table, tlen, head, bits,
-                                                         rows, out, err);
+                                                         rows, out, err, lrow);
 }
 
 void launch_coder_mix(const uint16_t* d16, int ldd, const int64_t* tmax, int ldt, int tsh, int R, int V,

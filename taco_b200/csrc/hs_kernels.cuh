@@ -24,8 +24,11 @@ struct ModelConsts {
     int softmax_p;
 };
 
+// at (may be null): the position of each row's embedding, where it is not its cache row rows[r].pos
+// (the nodes of a draft tree).
 void launch_embed(const RowInfo* rows, int R, const int8_t* wte, int ldw, const int32_t* em, int es,
-                  const int8_t* wpe, const int32_t* pm, int ps, int d, int32_t* x, cudaStream_t st);
+                  const int8_t* wpe, const int32_t* pm, int ps, int d, int32_t* x, cudaStream_t st,
+                  const uint32_t* at = nullptr);
 
 // out_lo != nullptr: 16-bit outputs (ln_f_bits = 16) as two i8 planes, hi in `out` and lo in
 // `out_lo` (v = 256 hi + lo + 128).
@@ -114,10 +117,11 @@ void launch_attention_tc(const void* tmQ, const void* tmK, const void* tmV, cons
 
 // The coder op: from the d16/tmax output of the logits GEMM, the interval of each row's query
 // in the table of taco_coder::FreqTable::from_weights(weights, bits). out: 3 u64 per row. `head`
-// is the last index j with table[j] == table[0] (the table is not increasing).
+// is the last index j with table[j] == table[0] (the table is not increasing). Query r asks the
+// logits row lrow[r] (null: row r), so that one row can answer several queries.
 void launch_coder(const uint16_t* d16, int ldd, const int64_t* tmax, int ldt, int tsh, int R, int V,
                   const uint64_t* table, int tlen, int head, uint32_t bits, const RowInfo* rows, uint64_t* out,
-                  int* err, cudaStream_t st);
+                  int* err, cudaStream_t st, const int* lrow = nullptr);
 
 // The mixed coder op of the profile logs, in two phases around a host step. Phase 0 (the stats
 // kernel): out = {W, w[p], top} of the GPT-2 weights of each row, p = mix[r].p. Phase 1: the

@@ -185,6 +185,8 @@ struct hs_model {
     uint64_t* logits_exp = nullptr;
     int logits_len = 0;
     int logits_head = 0;  // the last index j with logits_exp[j] == logits_exp[0]
+    int logits_last_weight = 0;  // the last index j with logits_exp[j] != 0
+    uint64_t logits_first = 0;   // logits_exp[0]
 
     ~hs_model() {
         if (dev && cudaSetDevice(dev->ordinal) != cudaSuccess) cudaGetLastError();
@@ -199,6 +201,23 @@ struct hs_model {
 struct StreamSt {
     uint32_t len = 0, first = 0, written = 0;
     int32_t prev_first = -1;
+};
+
+// The draft trees of the last hs_batch_run_tree: its nodes (the rows of the pass) with their parents
+// (-1: the context) and depths, and the tree of each slot that took part. The logits of the rows stay in
+// d16c until the next call that runs rows.
+struct TreePass {
+    struct Slot {
+        uint32_t slot, first, count, prefix;
+    };
+    std::vector<uint32_t> slots, tokens;  // per node
+    std::vector<int32_t> parents;
+    std::vector<Slot> trees;
+    bool logits = false;  // d16c holds the rows' logits
+    void clear() {
+        trees.clear();
+        logits = false;
+    }
 };
 
 struct hs_batch {
@@ -271,6 +290,21 @@ struct hs_batch {
     uint16_t* mx_d16[2] = {nullptr, nullptr};
     int64_t* mx_tmax[2] = {nullptr, nullptr};
     alignas(128) CUtensorMap mx_ts_d16[2];
+    // Draft trees (made on their first use): the trees of the pass, the embedding position of each
+    // row, the masks (TREE_WORDS words a row), and the queries (one logits row can answer several).
+    TreePass tree;
+    TreeSeq* d_tree_seqs = nullptr;
+    uint32_t* d_tree_at = nullptr;
+    uint32_t* d_tree_mask = nullptr;
+    RowInfo* d_queries = nullptr;
+    int* d_query_rows = nullptr;
+    uint32_t* d_path = nullptr;  // a path of MAX_TREE nodes for each slot, then the lengths
+    int tree_n = 0;              // trees of the pass in flight (0: no tree pass)
+    int tree_count = 0, tree_keys = 0;
+    // Beams (made on their first use): per beam the logits row, cost, finished byte, and the answers.
+    uint32_t* d_beam_u32 = nullptr;  // [5][Rcap]: logits rows, slots, parents / moves, tokens, rows held
+    int64_t* d_beam_cost = nullptr;  // [2][Rcap]: before, after
+    uint8_t* d_beam_fin = nullptr;
     uint64_t bytes = 0;
     // Per-op device time (CUDA events on the batch stream) when profiling is on.
     bool profiling = false;
@@ -319,9 +353,10 @@ namespace {
 // The ops of one pass, for the profile (the reference's CudaBatch::profile op names).
 // OP_PASS spans a whole pass (first kernel to the coder, gaps included); it is not a launch.
 enum Op { OP_EMBED, OP_LN, OP_GEMM_QKV, OP_KV, OP_ATTN, OP_GEMM_PROJ, OP_GEMM_FC, OP_GEMM_MLP, OP_GEMM_LOGITS,
-          OP_CODER, OP_DECODER, OP_PASS, OP_COUNT };
+          OP_CODER, OP_DECODER, OP_PASS, OP_BEAM, OP_CACHE_MOVE, OP_COUNT };
 const char* OP_NAMES[OP_COUNT] = {"embed", "layernorm", "gemm_qkv", "kv_store", "attention", "gemm_proj",
-                                  "gemm_fc", "gemm_mlp", "gemm_logits", "coder", "decoder", "pass"};
+                                  "gemm_fc", "gemm_mlp", "gemm_logits", "coder", "decoder", "pass",
+                                  "beam_select", "cache_move"};
 
 // Kernel launches of this process (the bench reports the launches of its timed region). Several
 // host threads launch at once in the multi-GPU fold and unfold, so the count is atomic.
@@ -415,6 +450,16 @@ int upload_ln(hs_model* m, const hsm::LayerNormP& L, LnDev& D) {
     return HS_OK;
 }
 
+constexpr int TREE_WORDS = MAX_TREE / 32;
+
+// The cache of a batch as the draft operators take it: a plane is one layer and head.
+CacheView cache_of(const hs_batch* b) {
+    const ModelConsts& c = b->model->c;
+    const uint64_t slot = (uint64_t)c.L * c.n_ctx * c.d;
+    return CacheView{b->kc, b->vc, slot, (uint32_t)b->slots, (uint32_t)(c.L * c.H), c.n_ctx, c.hd,
+                     c.n_ctx % 16 == 0 && c.hd % 16 == 0};
+}
+
 // The forward pass of R rows (the rows are in b->d_rows): the layers and ln_f into b->a; the
 // LM head is logits() (run_logits_chunks or the mixed pass).
 int forward(hs_batch* b, int R) {
@@ -423,7 +468,8 @@ int forward(hs_batch* b, int R) {
     cudaStream_t st = b->stream;
     {
         ProfScope p(b, OP_EMBED, 0);
-        launch_embed(b->d_rows, R, m->wte, c.Dp, m->em, m->es, m->wpe, m->pm, m->ps, c.d, b->x, st);
+        launch_embed(b->d_rows, R, m->wte, c.Dp, m->em, m->es, m->wpe, m->pm, m->ps, c.d, b->x, st,
+                     b->tree_n ? b->d_tree_at : nullptr);
     }
     // The attention work of this pass: 2 * 2 * hd * (pos + 1) per row and head (q.k and p.v).
     uint64_t attn_ops = 0;
@@ -485,7 +531,26 @@ int forward(hs_batch* b, int R) {
             ProfScope p(b, OP_KV, 0);
             launch_v_scatter(b->d_rows, R, b->att, c.Dp, c.d, c.H, c.hd, c.L, l, c.n_ctx, b->vc, st);
         }
-        {
+        if (b->tree_n) {
+            ProfScope p(b, OP_ATTN, attn_ops);
+            TreeArgs t{};
+            t.cache = cache_of(b);
+            t.rule = AttnRuleView{Ld.score_m, Ld.out_m, Ld.score_s, Ld.out_s, c.softmax_p, m->attn_len, m->attn_exp};
+            t.q = b->qkv;
+            t.out = b->att;
+            t.q_stride = (uint64_t)c.QKVp;
+            t.out_stride = (uint64_t)c.Dp;
+            t.seqs = b->d_tree_seqs;
+            t.mask = b->d_tree_mask;
+            t.plane0 = (uint32_t)(l * c.H);
+            t.n_rows = (uint32_t)R;
+            t.n_seq = (uint32_t)b->tree_n;
+            t.n_head = t.n_kv = c.H;
+            t.max_count = b->tree_count;
+            t.max_keys = b->tree_keys;
+            t.mask_words = TREE_WORDS;
+            CK(launch_tree_attention(t, m->dev->num_sms, m->dev->d_err, st));
+        } else {
             ProfScope p(b, OP_ATTN, attn_ops);
             launch_attention_tc(&b->tm_q, &b->tm_k, &b->tm_v, b->d_groups, b->n_groups, c.L, l, c.H, c.n_ctx,
                                 Ld.score_m, Ld.score_s, Ld.out_m, Ld.out_s, m->attn_exp, m->attn_len, c.softmax_p,
@@ -598,6 +663,8 @@ int check_device_error(hs_batch* b) {
         cudaMemset(dev->d_err, 0, sizeof(int));
         if (herr == ERR_CODER_DIVISION)
             return fail(HS_CUDA, "the coder op's frequency division did not converge (code " + std::to_string(herr) + ")");
+        if (herr >= ERR_DRAFT_SEQ && herr <= ERR_DRAFT_PATH)
+            return fail(HS_CUDA, "a draft kernel refused a record of this library (code " + std::to_string(herr) + ")");
         if (herr == ERR_ATTN_SCRATCH)
             return fail(HS_CUDA, "the prefill attention ran a CTA without a scratch slot (code " +
                                      std::to_string(herr) + ")");
@@ -833,6 +900,7 @@ int run(hs_batch* b, const uint32_t* slots, const uint32_t* tokens, const uint32
         if ((rc = dalloc(&b->weights, (size_t)b->Rcap * c.V, b->owned))) return rc;
         b->bytes += (uint64_t)b->Rcap * c.V * 8;
     }
+    b->tree.clear();
     Planner plan(b, slots, tokens, n, b->hist_work);
     auto& passes = plan.passes;
     // Coder answers: pass k uses half k & 1 of the host buffers, and the host prepares pass k + 1
@@ -1054,6 +1122,7 @@ int decode_blocks(hs_batch* b, uint32_t n, const uint32_t* slots, const uint8_t*
     int rc = set_device(m->dev);
     if (rc) return rc;
     cudaGetLastError();
+    b->tree.clear();
     cudaStream_t st = b->stream;
     const int n_ctx = c.n_ctx;
     std::vector<uint32_t> order(n);
@@ -1266,6 +1335,7 @@ int truncate_slot(hs_batch* b, uint32_t slot, uint64_t len) {
     const uint64_t drop = ss.len - len;
     const uint64_t here = pos > ss.first ? pos - ss.first : 0;
     if (drop <= here) {
+        b->tree.clear();
         b->streams[slot].len = (uint32_t)len;
         b->pos[slot] = (int)(pos - drop);
         return HS_OK;
@@ -1279,6 +1349,7 @@ int truncate_slot(hs_batch* b, uint32_t slot, uint64_t len) {
     int rc = set_device(b->model->dev);
     if (rc) return rc;
     cudaGetLastError();
+    b->tree.clear();
     std::vector<PlanRow> rows;
     for (uint32_t p = 0; p < std::min(target, ss.written); p++) rows.push_back({slot, old[p], p, -1});
     if ((rc = run_rows(b, rows))) return rc;
@@ -1289,6 +1360,410 @@ int truncate_slot(hs_batch* b, uint32_t slot, uint64_t len) {
     st.prev_first = -1;
     st.written = (uint32_t)n_ctx;
     b->pos[slot] = (int)target;
+    return HS_OK;
+}
+
+// An entry point's body: C++ exceptions (memory) end here.
+template <class F>
+int guarded(F&& f) {
+    try {
+        return f();
+    } catch (const std::exception& e) {
+        return fail(HS_CUDA, std::string("a host error: ") + e.what());
+    }
+}
+
+// ---- draft trees ----
+
+// The answers of nq queries on the logits of the rows of the last tree pass (d16c), in chunks of the
+// query buffers' Rcap.
+int tree_queries(hs_batch* b, uint32_t nq, const uint32_t* rows, const uint32_t* kinds, const uint64_t* values,
+                 uint32_t bits, hs_interval* out) {
+    hs_model* m = b->model;
+    const ModelConsts& c = m->c;
+    std::vector<RowInfo> q;
+    std::vector<int> at;
+    std::vector<uint64_t> iv;
+    for (uint32_t q0 = 0; q0 < nq; q0 += (uint32_t)b->Rcap) {
+        const uint32_t k = std::min<uint32_t>(nq - q0, (uint32_t)b->Rcap);
+        q.resize(k);
+        at.resize(k);
+        iv.resize(3 * (size_t)k);
+        for (uint32_t i = 0; i < k; i++) {
+            q[i] = RowInfo{0, 0, 0, kinds[q0 + i], values[q0 + i]};
+            at[i] = (int)rows[q0 + i];
+        }
+        CK(cudaMemcpyAsync(b->d_queries, q.data(), sizeof(RowInfo) * k, cudaMemcpyHostToDevice, b->stream));
+        CK(cudaMemcpyAsync(b->d_query_rows, at.data(), sizeof(int) * k, cudaMemcpyHostToDevice, b->stream));
+        {
+            ProfScope p(b, OP_CODER, 0);
+            launch_coder(b->d16c, c.Vp, b->tmaxc, c.VT, c.tsh, (int)k, c.V, m->logits_exp, m->logits_len,
+                         m->logits_head, bits, b->d_queries, b->intervals, m->dev->d_err, b->stream, b->d_query_rows);
+        }
+        CK(cudaMemcpyAsync(iv.data(), b->intervals, sizeof(uint64_t) * iv.size(), cudaMemcpyDeviceToHost, b->stream));
+        int rc = check_device_error(b);
+        if (rc) return rc;
+        for (uint32_t i = 0; i < k; i++) {
+            hs_interval& o = out[q0 + i];
+            o.symbol = (uint32_t)iv[3 * (size_t)i];
+            o.start = iv[3 * (size_t)i + 1];
+            o.freq = iv[3 * (size_t)i + 2];
+            o.is_last = o.symbol + 1 == (uint32_t)c.V;
+            o.reserved = 0;
+        }
+    }
+    if (b->profiling) prof_collect(b);
+    return HS_OK;
+}
+
+// The checks of the queries of a tree pass of n rows.
+int check_queries(hs_batch* b, uint32_t n, uint32_t nq, const uint32_t* rows, const uint32_t* kinds,
+                  const uint64_t* values, uint32_t bits) {
+    const ModelConsts& c = b->model->c;
+    if (bits == 0 || bits > 32 || (uint64_t)c.V > (1ULL << bits))
+        return fail(HS_UNSUPPORTED, "freq_bits must be in 1..=32 and 2^freq_bits >= vocab");
+    for (uint32_t i = 0; i < nq; i++) {
+        if (rows[i] >= n) return fail(HS_BAD_ARGUMENT, "a query asks a row that is no node of the trees");
+        const bool ok = (kinds[i] == 0 && values[i] < (uint64_t)c.V) || (kinds[i] == 1 && values[i] < (1ULL << bits));
+        if (!ok) return fail(HS_UNSUPPORTED, "a coder token or target is out of range");
+    }
+    return HS_OK;
+}
+
+// hs_batch_run_tree: one pass over the nodes of all trees. Node i of a slot takes cache row prefix +
+// i, so the K and V stores of the pass are those of any other rows; its embedding has the position
+// prefix + depth, and the attention is the tree kernel's.
+int run_tree(hs_batch* b, uint32_t n, const uint32_t* slots, const uint32_t* tokens, const uint32_t* parents,
+             uint32_t nq, const uint32_t* q_rows, const uint32_t* kinds, const uint64_t* values, uint32_t bits,
+             hs_interval* out) {
+    hs_model* m = b->model;
+    const ModelConsts& c = m->c;
+    b->tree.clear();
+    TreePass next;
+    next.slots.assign(slots, slots + n);
+    next.tokens.assign(tokens, tokens + n);
+    next.parents.resize(n);
+    std::vector<uint32_t> at(n), mask((size_t)n * TREE_WORDS, 0);
+    std::vector<char> seen(b->slots, 0);
+    int most = 0, keys = 0;
+    for (uint32_t i = 0; i < n; i++) {
+        const uint32_t s = slots[i];
+        if (s >= (uint32_t)b->slots)
+            return fail(HS_BAD_SLOT, "slot " + std::to_string(s) + " is not valid in a batch of " +
+                                         std::to_string(b->slots) + " slots");
+        if (tokens[i] >= (uint32_t)c.V)
+            return fail(HS_TOKEN_RANGE, "token " + std::to_string(tokens[i]) + " is not in the vocabulary of " +
+                                            std::to_string(c.V) + " tokens");
+        if (i == 0 || slots[i - 1] != s) {
+            if (seen[s]) return fail(HS_BAD_ARGUMENT, "the nodes of a slot are not together");
+            seen[s] = 1;
+            next.trees.push_back({s, i, 0, (uint32_t)b->pos[s]});
+        }
+        TreePass::Slot& t = next.trees.back();
+        const uint32_t node = t.count++;
+        if (t.count > (uint32_t)MAX_TREE) return fail(HS_UNSUPPORTED, "a tree has at most 128 nodes");
+        if (t.prefix + t.count > (uint32_t)c.n_ctx)
+            return fail(HS_UNSUPPORTED, "the tree of slot " + std::to_string(s) + " does not fit in its context");
+        uint32_t* mk = &mask[(size_t)i * TREE_WORDS];
+        if (parents[i] == HS_NO_TOKEN) {
+            next.parents[i] = -1;
+            at[i] = t.prefix;
+        } else {
+            if (parents[i] < t.first || parents[i] >= i)
+                return fail(HS_BAD_ARGUMENT, "a node's parent is not an earlier node of its slot");
+            next.parents[i] = (int32_t)parents[i];
+            at[i] = at[parents[i]] + 1;
+            memcpy(mk, &mask[(size_t)parents[i] * TREE_WORDS], sizeof(uint32_t) * TREE_WORDS);
+        }
+        mk[node >> 5] |= 1u << (node & 31);
+        most = std::max(most, (int)t.count);
+        keys = std::max(keys, (int)(t.prefix + t.count));
+    }
+    int rc = check_queries(b, n, nq, q_rows, kinds, values, bits);
+    if (rc) return rc;
+    if (n > (uint32_t)b->max_rows || n > (uint32_t)b->lchunk)
+        return fail(HS_UNSUPPORTED, "more nodes than one pass of the batch takes");
+    if (n == 0) return HS_OK;
+    if ((rc = set_device(m->dev))) return rc;
+    cudaGetLastError();
+    if (!b->d_path) {
+        const size_t R = (size_t)b->Rcap, S = (size_t)b->slots;
+        if ((rc = dalloc(&b->d_tree_seqs, S, b->owned)) || (rc = dalloc(&b->d_tree_at, R, b->owned)) ||
+            (rc = dalloc(&b->d_tree_mask, R * TREE_WORDS, b->owned)) || (rc = dalloc(&b->d_queries, R, b->owned)) ||
+            (rc = dalloc(&b->d_query_rows, R, b->owned)) || (rc = dalloc(&b->d_path, S * (MAX_TREE + 1), b->owned)))
+            return rc;
+        b->bytes += S * (sizeof(TreeSeq) + 4 * (MAX_TREE + 1)) + R * (sizeof(RowInfo) + 8 + 4 * TREE_WORDS);
+    }
+    std::vector<TreeSeq> seqs;
+    for (const TreePass::Slot& t : next.trees) {
+        seqs.push_back({t.first, t.count, t.slot, t.prefix});
+        // The rows behind the position are no longer the old context's (a truncation rebuilds them).
+        StreamSt& ss = b->streams[t.slot];
+        ss.written = std::max(ss.written, t.prefix + t.count);
+        for (uint32_t i = 0; i < t.count; i++)
+            b->h_rows[t.first + i] = RowInfo{t.slot, tokens[t.first + i], t.prefix + i, 0, 0};
+    }
+    CK(cudaMemcpyAsync(b->d_rows, b->h_rows, sizeof(RowInfo) * n, cudaMemcpyHostToDevice, b->stream));
+    CK(cudaMemcpyAsync(b->d_tree_seqs, seqs.data(), sizeof(TreeSeq) * seqs.size(), cudaMemcpyHostToDevice, b->stream));
+    CK(cudaMemcpyAsync(b->d_tree_at, at.data(), sizeof(uint32_t) * n, cudaMemcpyHostToDevice, b->stream));
+    CK(cudaMemcpyAsync(b->d_tree_mask, mask.data(), sizeof(uint32_t) * mask.size(), cudaMemcpyHostToDevice, b->stream));
+    b->n_groups = 0;
+    b->n_rowlist = 0;
+    b->v_scatter = false;
+    for (int r0 = 0; r0 < (int)n && !b->v_scatter; r0 += 32) b->v_scatter = !vt_run_host(b->h_rows, r0, (int)n, c.n_ctx);
+    {
+        struct InFlight {
+            hs_batch* b;
+            ~InFlight() { b->tree_n = 0; }
+        } in_flight{b};
+        b->tree_n = (int)seqs.size();
+        b->tree_count = most;
+        b->tree_keys = keys;
+        ProfScope pass_scope(b, OP_PASS, (uint64_t)n);
+        if ((rc = forward(b, (int)n))) return rc;
+        logits(b, 0, (int)n, b->d16c, b->tmaxc, &b->ts_d16c);
+    }
+    if ((rc = nq ? tree_queries(b, nq, q_rows, kinds, values, bits, out) : check_device_error(b))) return rc;
+    if (b->profiling) prof_collect(b);
+    b->tree = std::move(next);
+    b->tree.logits = true;
+    return HS_OK;
+}
+
+// hs_batch_tree_commit: the accepted nodes of every tree become inputs of their slots. The cache rows of
+// a path move down to the slot's position (no wait: later passes follow in the stream).
+int tree_commit(hs_batch* b, uint32_t n, const uint32_t* nodes) {
+    hs_model* m = b->model;
+    const size_t S = (size_t)b->slots;
+    if (b->tree.trees.empty()) {
+        if (n) return fail(HS_BAD_ARGUMENT, "no trees to commit: another call ran since hs_batch_run_tree");
+        return HS_OK;
+    }
+    struct Accept {
+        const TreePass::Slot* tree;
+        uint32_t first, count;
+    };
+    std::vector<Accept> acc;
+    std::vector<char> seen(b->slots, 0);
+    for (uint32_t i = 0; i < n; i++) {
+        const uint32_t v = nodes[i];
+        if (v >= b->tree.slots.size()) return fail(HS_BAD_ARGUMENT, "a node to commit is no node of the trees");
+        const uint32_t s = b->tree.slots[v];
+        if (acc.empty() || acc.back().tree->slot != s) {
+            if (seen[s]) return fail(HS_BAD_ARGUMENT, "the nodes of a slot are not together");
+            seen[s] = 1;
+            const TreePass::Slot* t = nullptr;
+            for (const TreePass::Slot& x : b->tree.trees)
+                if (x.slot == s && x.count) t = &x;
+            if (!t) return fail(HS_BAD_ARGUMENT, "the slot of a node was reset since the trees ran");
+            acc.push_back({t, i, 0});
+        }
+        Accept& a = acc.back();
+        const int32_t want = a.count ? (int32_t)nodes[i - 1] : -1;
+        if (b->tree.parents[v] != want) return fail(HS_BAD_ARGUMENT, "the nodes of a slot are not a path from its context");
+        a.count++;
+    }
+    int rc = set_device(m->dev);
+    if (rc) return rc;
+    cudaGetLastError();
+    std::vector<TreeSeq> seqs;
+    std::vector<uint32_t> path, lens;
+    for (const Accept& a : acc) {
+        uint32_t moved = a.count;  // a path that starts as the first nodes leaves those where they are
+        if (nodes[a.first + a.count - 1] - a.tree->first == a.count - 1) moved = 0;
+        if (!moved) continue;
+        seqs.push_back({0, a.tree->count, a.tree->slot, a.tree->prefix});
+        lens.push_back(a.count);
+        path.resize(seqs.size() * MAX_TREE, 0);
+        for (uint32_t j = 0; j < a.count; j++)
+            path[(seqs.size() - 1) * MAX_TREE + j] = nodes[a.first + j] - a.tree->first;
+    }
+    if (!seqs.empty()) {
+        uint32_t* d_len = b->d_path + S * MAX_TREE;
+        CK(cudaMemcpyAsync(b->d_tree_seqs, seqs.data(), sizeof(TreeSeq) * seqs.size(), cudaMemcpyHostToDevice, b->stream));
+        CK(cudaMemcpyAsync(b->d_path, path.data(), sizeof(uint32_t) * path.size(), cudaMemcpyHostToDevice, b->stream));
+        CK(cudaMemcpyAsync(d_len, lens.data(), sizeof(uint32_t) * lens.size(), cudaMemcpyHostToDevice, b->stream));
+        ProfScope p(b, OP_CACHE_MOVE, 0);
+        CK(launch_cache_commit(cache_of(b), b->d_tree_seqs, b->d_path, d_len, (uint32_t)seqs.size(), MAX_TREE,
+                               m->dev->num_sms, m->dev->d_err, b->stream));
+    }
+    for (const Accept& a : acc) {
+        const uint32_t s = a.tree->slot;
+        uint32_t* h = &b->hist[(size_t)s * m->c.n_ctx];
+        for (uint32_t j = 0; j < a.count; j++) h[a.tree->prefix + j] = b->tree.tokens[nodes[a.first + j]];
+        b->pos[s] = (int)(a.tree->prefix + a.count);
+        b->streams[s].len += a.count;
+    }
+    b->tree.trees.clear();  // the logits of the rows stay for hs_batch_tree_query
+    return HS_OK;
+}
+
+// ---- beams ----
+
+// hs_batch_beam_step. The rows of the living beams run as one pass, the selection answers on their
+// logits, and the states follow: a new beam keeps its parent's slot if it is the first child there, the
+// other children take the slots of beams that ended, copied in one launch.
+int beam_step(hs_batch* b, uint32_t groups, uint32_t beams, uint32_t* slots, uint32_t* tokens, int64_t* costs,
+              uint8_t* finished, uint32_t* parents) {
+    hs_model* m = b->model;
+    const ModelConsts& c = m->c;
+    if (groups == 0 || beams == 0) return HS_OK;
+    if (beams > (uint32_t)MAX_BEAMS) return fail(HS_UNSUPPORTED, "a group has 1 to 32 beams");
+    if (groups > (uint32_t)b->slots || groups * beams > (uint32_t)b->slots || groups * beams > (uint32_t)b->Rcap)
+        return fail(HS_UNSUPPORTED, "more beams than the batch has slots or rows");
+    if (m->logits_first > UINT64_MAX / (uint64_t)c.V)
+        return fail(HS_UNSUPPORTED, "vocab times the largest weight does not fit in 64 bits");
+    const uint32_t n = groups * beams;
+    std::vector<char> seen(b->slots, 0);
+    std::vector<uint32_t> row_of(n, 0);
+    uint32_t R = 0;
+    for (uint32_t i = 0; i < n; i++) {
+        const uint32_t s = slots[i];
+        if (s >= (uint32_t)b->slots)
+            return fail(HS_BAD_SLOT, "slot " + std::to_string(s) + " is not valid in a batch of " +
+                                         std::to_string(b->slots) + " slots");
+        if (seen[s]) return fail(HS_BAD_ARGUMENT, "two beams in one slot");
+        seen[s] = 1;
+        if (costs[i] >= (1LL << 62)) return fail(HS_BAD_ARGUMENT, "a beam's cost is 2^62 or more");
+        if (costs[i] < 0 || (finished && finished[i])) continue;
+        if (tokens[i] >= (uint32_t)c.V)
+            return fail(HS_TOKEN_RANGE, "token " + std::to_string(tokens[i]) + " is not in the vocabulary of " +
+                                            std::to_string(c.V) + " tokens");
+        if (b->pos[s] >= c.n_ctx)
+            return fail(HS_UNSUPPORTED, "the context of slot " + std::to_string(s) + " is full");
+        row_of[i] = R++;
+    }
+    if (R > (uint32_t)b->max_rows || R > (uint32_t)b->lchunk)
+        return fail(HS_UNSUPPORTED, "more beams than one pass of the batch takes");
+    int rc = set_device(m->dev);
+    if (rc) return rc;
+    cudaGetLastError();
+    const size_t Rc = (size_t)b->Rcap;
+    if (!b->d_beam_fin) {
+        if ((rc = dalloc(&b->d_beam_u32, 5 * Rc, b->owned)) || (rc = dalloc(&b->d_beam_cost, 2 * Rc, b->owned)) ||
+            (rc = dalloc(&b->d_beam_fin, Rc, b->owned)))
+            return rc;
+        b->bytes += 37 * Rc;
+    }
+    b->tree.clear();
+    uint32_t *d_row_of = b->d_beam_u32, *d_slots = d_row_of + Rc, *d_parent = d_slots + Rc, *d_token = d_parent + Rc,
+             *d_held = d_token + Rc;
+    std::vector<uint32_t> row_pos(n, 0);
+    if (R) {
+        for (uint32_t i = 0; i < n; i++) {
+            if (costs[i] < 0 || (finished && finished[i])) continue;
+            StreamSt& ss = b->streams[slots[i]];
+            ss.written = std::max(ss.written, (uint32_t)b->pos[slots[i]] + 1);
+            b->h_rows[row_of[i]] = RowInfo{slots[i], tokens[i], (uint32_t)b->pos[slots[i]], 0, 0};
+        }
+        CK(cudaMemcpyAsync(b->d_rows, b->h_rows, sizeof(RowInfo) * R, cudaMemcpyHostToDevice, b->stream));
+        b->n_groups = 0;
+        b->n_rowlist = 0;
+        b->v_scatter = true;
+        ProfScope pass_scope(b, OP_PASS, (uint64_t)R);
+        if ((rc = forward(b, (int)R))) return rc;
+        logits(b, 0, (int)R, b->d16c, b->tmaxc, &b->ts_d16c);
+    }
+    std::vector<uint8_t> fin(n, 0);
+    if (finished) fin.assign(finished, finished + n);
+    CK(cudaMemcpyAsync(d_row_of, row_of.data(), sizeof(uint32_t) * n, cudaMemcpyHostToDevice, b->stream));
+    CK(cudaMemcpyAsync(b->d_beam_cost, costs, sizeof(int64_t) * n, cudaMemcpyHostToDevice, b->stream));
+    CK(cudaMemcpyAsync(b->d_beam_fin, fin.data(), n, cudaMemcpyHostToDevice, b->stream));
+    BeamArgs a{};
+    a.dist = b->d16c;
+    a.tops = b->tmaxc;
+    a.dist_stride = (uint64_t)c.Vp;
+    a.tops_stride = (uint64_t)c.VT;
+    a.row_of = d_row_of;
+    a.base = b->d_beam_cost;
+    a.finished = b->d_beam_fin;
+    a.parent = d_parent;
+    a.token = d_token;
+    a.cost = b->d_beam_cost + Rc;
+    a.table = m->logits_exp;
+    a.tlen = m->logits_len;
+    a.last_weight = m->logits_last_weight;
+    a.tsh = c.tsh;
+    a.vocab = c.V;
+    a.groups = (int)groups;
+    a.beams = a.keep = (int)beams;
+    {
+        ProfScope p(b, OP_BEAM, 0);
+        CK(launch_beam_select(a, m->dev->num_sms, b->stream));
+    }
+    std::vector<uint32_t> par(n), tok(n);
+    std::vector<int64_t> cost(n);
+    CK(cudaMemcpyAsync(par.data(), d_parent, sizeof(uint32_t) * n, cudaMemcpyDeviceToHost, b->stream));
+    CK(cudaMemcpyAsync(tok.data(), d_token, sizeof(uint32_t) * n, cudaMemcpyDeviceToHost, b->stream));
+    CK(cudaMemcpyAsync(cost.data(), a.cost, sizeof(int64_t) * n, cudaMemcpyDeviceToHost, b->stream));
+    if ((rc = check_device_error(b))) return rc;
+    if (b->profiling) prof_collect(b);
+    // The inputs of this step, in the slots that ran.
+    for (uint32_t i = 0; i < n; i++) {
+        if (costs[i] < 0 || (finished && finished[i])) continue;
+        const uint32_t s = slots[i];
+        b->hist[(size_t)s * c.n_ctx + b->pos[s]] = tokens[i];
+        b->pos[s]++;
+        b->streams[s].len++;
+    }
+    // The slots of the new beams, and the copies (moves[p]: the place whose state place p takes).
+    std::vector<uint32_t> new_slots(n), moves(n), held(n);
+    bool any = false;
+    for (uint32_t g = 0; g < groups; g++) {
+        const uint32_t o = g * beams;
+        std::vector<int> place(beams, -1);
+        std::vector<char> kept(beams, 0);
+        for (uint32_t j = 0; j < beams; j++) {
+            moves[o + j] = j;
+            held[o + j] = (uint32_t)b->pos[slots[o + j]];
+            const uint32_t p = par[o + j];
+            if (p < beams && !kept[p]) {
+                kept[p] = 1;
+                place[j] = (int)p;
+            }
+        }
+        uint32_t next = 0;
+        for (uint32_t j = 0; j < beams; j++) {
+            if (place[j] < 0) {
+                while (kept[next]) next++;
+                kept[next] = 1;
+                place[j] = (int)next;
+                if (par[o + j] < beams) {
+                    moves[o + next] = par[o + j];
+                    any = true;
+                }
+            }
+            new_slots[o + j] = slots[o + place[j]];
+        }
+    }
+    if (any) {
+        CK(cudaMemcpyAsync(d_slots, slots, sizeof(uint32_t) * n, cudaMemcpyHostToDevice, b->stream));
+        CK(cudaMemcpyAsync(d_parent, moves.data(), sizeof(uint32_t) * n, cudaMemcpyHostToDevice, b->stream));
+        CK(cudaMemcpyAsync(d_held, held.data(), sizeof(uint32_t) * n, cudaMemcpyHostToDevice, b->stream));
+        ProfScope p(b, OP_CACHE_MOVE, 0);
+        CK(launch_cache_reorder(cache_of(b), d_slots, d_parent, d_held, groups, beams, m->dev->num_sms,
+                                m->dev->d_err, b->stream));
+    }
+    for (uint32_t i = 0; i < n; i++) {
+        const uint32_t dst = slots[i], src = slots[i / beams * beams + moves[i]];
+        if (dst == src) continue;
+        b->pos[dst] = b->pos[src];
+        std::copy_n(b->hist.begin() + (size_t)src * c.n_ctx, held[i / beams * beams + moves[i]],
+                    b->hist.begin() + (size_t)dst * c.n_ctx);
+        b->streams[dst] = b->streams[src];
+        b->streams[dst].prev_first = -1;  // the rows of the context before the last restart do not move
+    }
+    for (uint32_t i = 0; i < n; i++) {
+        if (par[i] == HS_NO_TOKEN) {  // no candidate: the beam is dead, its slot empty
+            b->pos[new_slots[i]] = 0;
+            b->streams[new_slots[i]] = StreamSt{};
+        }
+        slots[i] = new_slots[i];
+        if (finished) finished[i] = par[i] != HS_NO_TOKEN && tok[i] == HS_NO_TOKEN;
+    }
+    std::copy(par.begin(), par.end(), parents);
+    std::copy(tok.begin(), tok.end(), tokens);
+    std::copy(cost.begin(), cost.end(), costs);
     return HS_OK;
 }
 
@@ -1517,6 +1992,9 @@ int hs_model_load(hs_dev* dev, const uint8_t* file, size_t len, hs_model** out) 
     if ((rc = upload(&m->logits_exp, M.logits_exp.data(), M.logits_exp.size(), m->owned))) return rc;
     m->logits_len = (int)M.logits_exp.size();
     while (m->logits_head + 1 < m->logits_len && M.logits_exp[m->logits_head + 1] == M.logits_exp[0]) m->logits_head++;
+    m->logits_first = M.logits_exp[0];
+    while (m->logits_last_weight + 1 < m->logits_len && M.logits_exp[m->logits_last_weight + 1] != 0)
+        m->logits_last_weight++;
     m->weight_bytes += M.wpe.size() + 8 * M.logits_exp.size() + 4 * M.attn_exp.size();
     CK(cudaDeviceSynchronize());
     *out = m.release();
@@ -1659,6 +2137,8 @@ int hs_batch_set_overlap(hs_batch* b, uint16_t k) {
 int hs_batch_reset(hs_batch* b, uint32_t slot) {
     if (!b) return fail(HS_BAD_ARGUMENT, "null argument");
     if (slot < (uint32_t)b->slots) {
+        for (TreePass::Slot& t : b->tree.trees)
+            if (t.slot == slot) t.count = 0;  // its nodes can no longer be committed
         b->pos[slot] = 0;
         b->streams[slot] = StreamSt{};
     }
@@ -1750,6 +2230,40 @@ int hs_batch_room(hs_batch* b, uint32_t slot, uint64_t* room) {
 int hs_batch_truncate(hs_batch* b, uint32_t slot, uint64_t len) {
     if (!b) return fail(HS_BAD_ARGUMENT, "null argument");
     return truncate_slot(b, slot, len);
+}
+
+int hs_batch_run_tree(hs_batch* b, uint32_t n, const uint32_t* slots, const uint32_t* tokens, const uint32_t* parents,
+                      uint32_t n_queries, const uint32_t* query_nodes, const uint32_t* kinds, const uint64_t* values,
+                      uint32_t freq_bits, hs_interval* out) {
+    if (!b || (n && (!slots || !tokens || !parents)) || (n_queries && (!query_nodes || !kinds || !values || !out)))
+        return fail(HS_BAD_ARGUMENT, "null argument");
+    return guarded([&] {
+        return run_tree(b, n, slots, tokens, parents, n_queries, query_nodes, kinds, values, freq_bits, out);
+    });
+}
+
+int hs_batch_tree_query(hs_batch* b, uint32_t n, const uint32_t* nodes, const uint32_t* kinds, const uint64_t* values,
+                        uint32_t freq_bits, hs_interval* out) {
+    if (!b || (n && (!nodes || !kinds || !values || !out))) return fail(HS_BAD_ARGUMENT, "null argument");
+    return guarded([&]() -> int {
+        if (!b->tree.logits)
+            return fail(HS_BAD_ARGUMENT, "no trees to ask: another call ran since hs_batch_run_tree");
+        int rc = check_queries(b, (uint32_t)b->tree.slots.size(), n, nodes, kinds, values, freq_bits);
+        if (rc || (rc = set_device(b->model->dev))) return rc;
+        cudaGetLastError();
+        return n ? tree_queries(b, n, nodes, kinds, values, freq_bits, out) : HS_OK;
+    });
+}
+
+int hs_batch_tree_commit(hs_batch* b, uint32_t n, const uint32_t* nodes) {
+    if (!b || (n && !nodes)) return fail(HS_BAD_ARGUMENT, "null argument");
+    return guarded([&] { return tree_commit(b, n, nodes); });
+}
+
+int hs_batch_beam_step(hs_batch* b, uint32_t groups, uint32_t beams, uint32_t* slots, uint32_t* tokens, int64_t* costs,
+                       uint8_t* finished, uint32_t* parents) {
+    if (!b || (groups && beams && (!slots || !tokens || !costs || !parents))) return fail(HS_BAD_ARGUMENT, "null argument");
+    return guarded([&] { return beam_step(b, groups, beams, slots, tokens, costs, finished, parents); });
 }
 
 int hs_batch_decode_blocks(hs_batch* b, uint32_t n, const uint32_t* slots, const uint8_t* payload,
