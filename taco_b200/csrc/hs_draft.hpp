@@ -64,7 +64,8 @@ struct BeamArgs {
     int tsh, vocab, groups, beams, keep;
 };
 
-cudaError_t configure_draft_kernels();
+cudaError_t configure_draft_kernels();  // the attention's, then the others'
+cudaError_t configure_beam();
 cudaError_t launch_tree_attention(const TreeArgs& a, int num_sms, int* err, cudaStream_t st);
 cudaError_t launch_beam_select(const BeamArgs& a, int num_sms, cudaStream_t st);
 cudaError_t launch_cache_reorder(const CacheView& c, const uint32_t* slots, const uint32_t* parents,
