@@ -61,8 +61,16 @@ struct BeamArgs {
     int64_t* cost;
     const uint64_t* table;
     int tlen, last_weight;  // the last entry that is not 0
+    int cut_bits;           // the low bits of a weight that a 32-bit look-up leaves out
     int tsh, vocab, groups, beams, keep;
 };
+
+// The bits of table[0] above 32.
+inline int weight_cut_bits(uint64_t first) {
+    int bits = 0;
+    while ((first >> bits) >> 32) bits++;
+    return bits;
+}
 
 cudaError_t configure_draft_kernels();  // the attention's, then the others'
 cudaError_t configure_beam();

@@ -320,6 +320,7 @@ int hs_op_beam_select(hs_weight_rule* rule, const hs_beam_select* a, void* strea
         b.table = rule->table;
         b.tlen = rule->len;
         b.last_weight = rule->last_weight;
+        b.cut_bits = weight_cut_bits(rule->first);
         b.tsh = (int)a->tile_shift;
         b.vocab = (int)a->vocab;
         b.groups = (int)a->groups;

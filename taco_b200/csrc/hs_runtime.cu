@@ -1683,6 +1683,7 @@ int beam_step(hs_batch* b, uint32_t groups, uint32_t beams, uint32_t* slots, uin
     a.table = m->logits_exp;
     a.tlen = m->logits_len;
     a.last_weight = m->logits_last_weight;
+    a.cut_bits = weight_cut_bits(m->logits_first);
     a.tsh = c.tsh;
     a.vocab = c.V;
     a.groups = (int)groups;

@@ -649,3 +649,32 @@ def test_the_current_device_and_the_launch_count(dev):
     run_tree(dev, c)
     assert B.launch_count() == before + 1
     assert torch.cuda.current_device() == 0
+
+
+@pytest.mark.parametrize("vocab", [2, 3, 100, 1000])
+def test_beam_sums_next_to_a_border(dev, vocab):
+    """Weights whose low bits decide the normaliser: 32 bits of each do not, the whole ones do."""
+    c = beam_case(33, 4, 2, vocab)
+    c["dist"][:, :vocab] = 0
+    c["tops"][...] = 0
+    for low in (0, 1, 255, 511):
+        top = (1 << 40) + low
+        for near in (0, 1, -1):
+            # table[1] * (vocab * table[0]) against table[0]^2: just below, at and above the border.
+            c["table"] = np.array([top, top // vocab + near, 1, 0])
+            check_beam(dev, c, 3)
+    c["table"] = np.array([1 << 40] + [(1 << 40) // vocab + 2 - i for i in range(5)] + [511, 511, 3])
+    c["dist"][:, :vocab] = np.random.default_rng(34).integers(0, 9, (8, vocab))
+    c["dist"][:, 0] = 0
+    check_beam(dev, c, 3)
+
+
+def test_beam_weights_below_the_looked_up_bits(dev):
+    """A row without a symbol at distance 0 whose weights are all small."""
+    c = beam_case(35, 1, 2, 700)
+    c["table"] = np.array([1 << 45] + [100] * 50 + [3])
+    c["dist"][:, :700] = np.random.default_rng(36).integers(1, 60, (2, 700))
+    c["tops"][...] = 0
+    check_beam(dev, c, 20)
+    c["finished"] = np.array([1, 0])
+    check_beam(dev, c, 20)
