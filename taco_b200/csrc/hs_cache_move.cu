@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "hs_common.cuh"
 #include "hs_draft.hpp"
@@ -16,9 +17,9 @@ namespace {
 constexpr int MOVE_THREADS = 256;
 
 // T: the unit of a move (16 bytes where n_ctx and head_dim are multiples of 16, else a byte). B: the
-// most beams of a group. blockIdx.y is the group. The units of a plane are its keys (rows * hd bytes
-// from row 0), then its values (the first `rows` bytes of each channel's row): a unit of values may
-// pass the last row, and then goes byte by byte.
+// most beams of a group. blockIdx.y is the group, blockIdx.x a plane's keys (rows * hd bytes from row 0)
+// or values (the first `rows` bytes of each channel's row): a unit of values may pass the last row, and
+// then goes byte by byte.
 template <typename T, int B>
 __global__ void __launch_bounds__(MOVE_THREADS) k_cache_reorder(const CacheView c, const uint32_t* slots,
                                                                 const uint32_t* parents, const uint32_t* rows,
@@ -57,83 +58,131 @@ __global__ void __launch_bounds__(MOVE_THREADS) k_cache_reorder(const CacheView 
         }
         __syncthreads();
         const int n = (int)s_n;
-        if (s_bad && threadIdx.x == 0 && blockIdx.x == 0) atomicCAS(err, 0, ERR_DRAFT_PARENT);
+        if (s_bad && threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.z == 0) atomicCAS(err, 0, ERR_DRAFT_PARENT);
         if (n == 0) continue;
-        const uint32_t most = s_most;
-        const size_t ku = (size_t)most * c.hd / W;          // units of a plane's keys
-        const size_t vu = ((size_t)most + W - 1) / W;       // units of a channel's values
-        const size_t per_plane = ku + vu * c.hd, total = per_plane * c.planes;
-        const size_t plane_bytes = (size_t)c.n_ctx * c.hd;
-        for (size_t u = (size_t)blockIdx.x * MOVE_THREADS + threadIdx.x; u < total;
-             u += (size_t)gridDim.x * MOVE_THREADS) {
-            const size_t plane = u / per_plane, r = u % per_plane;
+        const size_t plane = (size_t)(blockIdx.x >> 1) * c.n_ctx * c.hd;  // (blockIdx.z: a part of its units)
+        const bool values = blockIdx.x & 1;
+        int8_t* base = (values ? c.v : c.k) + plane;
+        // Units of a channel's values, and of the plane's keys or values in all (at most 8192 * 1024).
+        const uint32_t vu = (s_most + W - 1) / W, total = values ? vu * c.hd : s_most * c.hd / W;
+#pragma unroll 1
+        for (uint32_t u = blockIdx.z * MOVE_THREADS + threadIdx.x; u < total; u += gridDim.z * MOVE_THREADS) {
+            const uint32_t ch = values ? u / vu : 0, x = (values ? u - ch * vu : u) * W;  // the unit's first byte
+            int8_t* at = base + (size_t)ch * c.n_ctx + x;
+            const uint32_t row = values ? 1 : c.hd;  // bytes of a row in this run of bytes
             T val[B];
-            if (r < ku) {
-                const size_t off = plane * plane_bytes + r * W;
 #pragma unroll
-                for (int j = 0; j < B; j++)
-                    if (j < n && r * W < (size_t)s_rows[j] * c.hd)
-                        val[j] = *reinterpret_cast<const T*>(c.k + s_src[j] * c.slot_stride + off);
+            for (int j = 0; j < B; j++)
+                if (j < n && x < s_rows[j] * row) val[j] = *reinterpret_cast<const T*>(at + s_src[j] * c.slot_stride);
 #pragma unroll
-                for (int j = 0; j < B; j++)
-                    if (j < n && r * W < (size_t)s_rows[j] * c.hd)
-                        *reinterpret_cast<T*>(c.k + s_dst[j] * c.slot_stride + off) = val[j];
-            } else {
-                const size_t ch = (r - ku) / vu, x = (r - ku) % vu * W;
-                const size_t off = plane * plane_bytes + ch * c.n_ctx + x;
-#pragma unroll
-                for (int j = 0; j < B; j++)
-                    if (j < n && x < s_rows[j])
-                        val[j] = *reinterpret_cast<const T*>(c.v + s_src[j] * c.slot_stride + off);
-#pragma unroll
-                for (int j = 0; j < B; j++) {
-                    if (j >= n || x >= s_rows[j]) continue;
-                    int8_t* to = c.v + s_dst[j] * c.slot_stride + off;
-                    if (x + W <= s_rows[j]) {
-                        *reinterpret_cast<T*>(to) = val[j];
-                    } else {
-                        const int8_t* b = reinterpret_cast<const int8_t*>(&val[j]);
-                        for (int i = 0; i < (int)(s_rows[j] - x); i++) to[i] = b[i];
-                    }
+            for (int j = 0; j < B; j++) {
+                if (j >= n || x >= s_rows[j] * row) continue;
+                int8_t* to = at + s_dst[j] * c.slot_stride;
+                if (W == 1 || x + W <= s_rows[j] * row) {
+                    *reinterpret_cast<T*>(to) = val[j];
+                } else {
+                    // The last rows of a channel's values end inside the unit.
+                    const int8_t* bytes = reinterpret_cast<const int8_t*>(&val[j]);
+                    for (uint32_t i = 0; i < s_rows[j] - x; i++) to[i] = bytes[i];
                 }
             }
         }
     }
 }
 
-// One block per (tree, plane). Row prefix + path[j] -> prefix + j with path strictly increasing, so
-// path[j] >= j and a source not yet read is above every row written: a thread moves its bytes in
-// ascending order of j.
-__global__ void __launch_bounds__(128) k_cache_commit(const CacheView c, const TreeSeq* seqs, const uint32_t* path,
-                                                      const uint32_t* lengths, uint32_t n_seq, uint32_t path_stride,
-                                                      int* err) {
-    __shared__ uint32_t s_path[MAX_TREE];
-    __shared__ int s_bad;
+// A warp moves parts of planes of one tree: a plane's keys (part 0) or some channels of its values.
+// path is strictly increasing, so path[j] >= j: taken in ascending runs, all of a run's rows read before
+// any is written, no row is written before it is read. The bytes of a path lie in a few 32-byte sectors of
+// each channel's row of values: that traffic is the cost (a lane takes a path's byte).
+constexpr int COMMIT_DEEP = 16, COMMIT_WARPS = 8, COMMIT_BLOCKS = 5;
+
+// The lanes that a channel of a path of m rows takes.
+__host__ __device__ inline int commit_width(uint32_t m) { return m <= 4 ? 4 : m <= 8 ? 8 : m <= 16 ? 16 : 32; }
+
+template <bool VEC>
+__global__ void __launch_bounds__(32 * COMMIT_WARPS, COMMIT_BLOCKS) k_cache_commit(const CacheView c, const TreeSeq* seqs,
+                                                                   const uint32_t* path, const uint32_t* lengths,
+                                                                   uint32_t path_stride, int unit_ch, int parts, uint32_t units,
+                                                                   int* err) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t first = blockIdx.y * (uint32_t)COMMIT_WARPS + (threadIdx.x >> 5);  // unit of the tree
     const uint32_t i = blockIdx.x;
+    // Lane l holds the path's entries l, l + 32, ...; the ones past its end stay where they are.
+    uint32_t p[MAX_TREE / 32];
+#pragma unroll
+    for (int k = 0; k < MAX_TREE / 32; k++) {
+        const uint32_t j = 32 * k + lane;
+        p[k] = j < path_stride ? path[(size_t)i * path_stride + j] : j;  // with the record and the length
+    }
     const TreeSeq s = seqs[i];
     const uint32_t m = lengths[i];
-    if (threadIdx.x == 0) s_bad = 0;
-    __syncthreads();
-    bool bad = m > path_stride || m > s.count || s.count > MAX_TREE || s.slot >= c.slots ||
+    bool bad = m > path_stride || m > s.count || s.count > (uint32_t)MAX_TREE || s.slot >= c.slots ||
                s.prefix > (uint32_t)c.n_ctx || s.count > (uint32_t)c.n_ctx - s.prefix;
-    if (!bad && threadIdx.x < m) {
-        const uint32_t p = path[(size_t)i * path_stride + threadIdx.x];
-        s_path[threadIdx.x] = p;
-        bad = p >= s.count || (threadIdx.x > 0 && p <= path[(size_t)i * path_stride + threadIdx.x - 1]);
+    uint32_t before = 0;  // the last entry of the run before, plus one
+    if (!bad) {
+#pragma unroll
+        for (int k = 0; k < MAX_TREE / 32; k++) {
+            const uint32_t j = 32 * k + lane;
+            p[k] = j < m ? p[k] : j;
+            uint32_t up = __shfl_up_sync(0xffffffffu, p[k], 1);
+            if (lane == 0) up = before - 1;
+            bad = bad || (j < m && (p[k] >= s.count || (j > 0 && p[k] <= up)));
+            before = __shfl_sync(0xffffffffu, p[k], 31) + 1;
+        }
     }
-    if (bad) s_bad = 1;
-    __syncthreads();
-    if (s_bad) {
-        if (threadIdx.x == 0) atomicCAS(err, 0, ERR_DRAFT_PATH);
+    if (__any_sync(0xffffffffu, bad)) {
+        if (lane == 0 && first == 0) atomicCAS(err, 0, ERR_DRAFT_PATH);
         return;
     }
-    const size_t base = s.slot * c.slot_stride + (size_t)blockIdx.y * ((size_t)c.n_ctx * c.hd);
-    int8_t* K = c.k + base + (size_t)s.prefix * c.hd;
-    int8_t* V = c.v + base + s.prefix;
-    for (int b = threadIdx.x; b < c.hd; b += 128) {
-        for (uint32_t j = 0; j < m; j++) {
-            K[(size_t)j * c.hd + b] = K[(size_t)s_path[j] * c.hd + b];
-            V[(size_t)b * c.n_ctx + j] = V[(size_t)b * c.n_ctx + s_path[j]];
+    for (uint32_t unit = first; unit < units; unit += gridDim.y * COMMIT_WARPS) {
+        const uint32_t plane = unit / (uint32_t)parts, part = unit % (uint32_t)parts;
+        const size_t base = s.slot * c.slot_stride + (size_t)plane * ((size_t)c.n_ctx * c.hd);
+        if (part == 0) {
+            int8_t* K = c.k + base + (size_t)s.prefix * c.hd;
+            using T = typename std::conditional<VEC, uint4, uint8_t>::type;
+            const uint32_t pieces = c.hd / (uint32_t)sizeof(T);  // of a row
+            for (uint32_t k0 = 0; k0 * 32 < m; k0++) {
+                // Runs of 8 rows (an entry of the path from the lane that holds it).
+                for (uint32_t j0 = 32 * k0; j0 < 32 * k0 + 32 && j0 < m; j0 += 8) {
+                    for (uint32_t x0 = 0; x0 < pieces; x0 += 4) {
+                        const uint32_t j = j0 + (lane >> 2), x = x0 + (lane & 3);
+                        const uint32_t from = __shfl_sync(0xffffffffu, k0 == 0 ? p[0] : k0 == 1 ? p[1] : k0 == 2 ? p[2] : p[3],
+                                                          (int)(j & 31));
+                        const bool move = j < m && x < pieces && from != j;
+                        T val;
+                        if (move) val = reinterpret_cast<const T*>(K + (size_t)from * c.hd)[x];
+                        __syncwarp();
+                        if (move) reinterpret_cast<T*>(K + (size_t)j * c.hd)[x] = val;
+                        __syncwarp();
+                    }
+                }
+            }
+            continue;
+        }
+        // Short paths share the warp between channels: `width` lanes of a channel.
+        const int ch0 = (int)(part - 1) * unit_ch, width = commit_width(m);
+        const int step = 32 / width, end = min(ch0 + unit_ch, c.hd);
+        for (uint32_t k0 = 0; k0 * 32 < m; k0++) {
+            const uint32_t pk = k0 == 0 ? p[0] : k0 == 1 ? p[1] : k0 == 2 ? p[2] : p[3];
+            const uint32_t j = 32 * k0 + lane % width, from = __shfl_sync(0xffffffffu, pk, lane % width);
+            const bool move = j < m && from != j;
+            const size_t next = (size_t)step * c.n_ctx;
+            for (int ch = ch0; ch < end; ch += COMMIT_DEEP * step) {
+                // This lane's channels ch + lane / width + q step.
+                const int mine = move ? (end - ch - lane / width + step - 1) / step : 0;
+                int8_t* V = c.v + base + (size_t)(ch + lane / width) * c.n_ctx + s.prefix;
+                const int8_t* of = V + from;
+                int8_t* to = V + j;
+                int8_t val[COMMIT_DEEP];
+#pragma unroll
+                for (int q = 0; q < COMMIT_DEEP; q++, of += next)
+                    if (q < mine) val[q] = *of;
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < COMMIT_DEEP; q++, to += next)
+                    if (q < mine) *to = val[q];
+            }
+            __syncwarp();
         }
     }
 }
@@ -153,9 +202,13 @@ cudaError_t launch_cache_reorder(const CacheView& c, const uint32_t* slots, cons
                                  const uint32_t* rows, uint32_t groups, uint32_t beams, int num_sms, int* err,
                                  cudaStream_t st) {
     if (groups == 0 || beams < 2) return cudaSuccess;
-    const uint32_t gy = groups < 65535u ? groups : 65535u;
-    const uint32_t gx = (uint32_t)(num_sms * 8 + (int)gy - 1) / gy;
-    const dim3 grid(gx < 1 ? 1 : gx, gy);
+    // Blocks beyond one for each group and plane's keys or values: up to 16 for an SM, so that few groups
+    // have many loads in flight, each with at least two units a thread at a full context.
+    const uint64_t blocks = 2ull * c.planes * groups, full = (uint64_t)c.n_ctx * c.hd / (c.vec ? 16 : 1);
+    uint64_t parts = (16ull * num_sms + blocks - 1) / blocks;
+    const uint64_t most = (full + 2 * MOVE_THREADS - 1) / (2 * MOVE_THREADS);
+    parts = parts < most ? parts : most;
+    const dim3 grid(2 * c.planes, groups < 65535u ? groups : 65535u, (unsigned)(parts < 64 ? parts : 64));
     if (c.vec) reorder<uint4>(c, slots, parents, rows, groups, beams, grid, err, st);
     else reorder<uint8_t>(c, slots, parents, rows, groups, beams, grid, err, st);
     return cudaGetLastError();
@@ -165,7 +218,14 @@ cudaError_t launch_cache_commit(const CacheView& c, const TreeSeq* seqs, const u
                                 uint32_t n_seq, uint32_t path_stride, int num_sms, int* err, cudaStream_t st) {
     (void)num_sms;
     if (n_seq == 0) return cudaSuccess;
-    k_cache_commit<<<dim3(n_seq, c.planes), 128, 0, st>>>(c, seqs, path, lengths, n_seq, path_stride, err);
+    const int unit_ch = COMMIT_DEEP * (32 / commit_width(path_stride)), parts = 1 + (c.hd + unit_ch - 1) / unit_ch;
+    const uint32_t units = c.planes * (uint32_t)parts;
+    const uint32_t blocks = (units + COMMIT_WARPS - 1) / COMMIT_WARPS;
+    const dim3 grid(n_seq, blocks < 65535u ? blocks : 65535u);
+    if (c.vec)
+        k_cache_commit<true><<<grid, 32 * COMMIT_WARPS, 0, st>>>(c, seqs, path, lengths, path_stride, unit_ch, parts, units, err);
+    else
+        k_cache_commit<false><<<grid, 32 * COMMIT_WARPS, 0, st>>>(c, seqs, path, lengths, path_stride, unit_ch, parts, units, err);
     return cudaGetLastError();
 }
 

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <vector>
 
 #include "hs_device.hpp"
 
@@ -60,6 +61,8 @@ struct BeamArgs {
     uint32_t* token;
     int64_t* cost;
     const uint64_t* table;
+    const uint32_t* high;   // table[j] >> cut_bits, then zeros to the next multiple of 4 past tlen
+    uint64_t first;         // table[0]
     int tlen, last_weight;  // the last entry that is not 0
     int cut_bits;           // the low bits of a weight that a 32-bit look-up leaves out
     int tsh, vocab, groups, beams, keep;
@@ -70,6 +73,14 @@ inline int weight_cut_bits(uint64_t first) {
     int bits = 0;
     while ((first >> bits) >> 32) bits++;
     return bits;
+}
+
+// BeamArgs::high of a table.
+inline std::vector<uint32_t> weight_high(const uint64_t* table, size_t n) {
+    std::vector<uint32_t> t((n + 4) / 4 * 4, 0);
+    const int bits = weight_cut_bits(table[0]);
+    for (size_t j = 0; j < n; j++) t[j] = (uint32_t)(table[j] >> bits);
+    return t;
 }
 
 cudaError_t configure_draft_kernels();  // the attention's, then the others'

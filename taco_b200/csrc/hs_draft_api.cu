@@ -28,7 +28,8 @@ struct hs_weight_rule {
     DevInfo dev;
     uint64_t first = 0;
     int len = 0, last_weight = 0;
-    uint64_t* table = nullptr;
+    uint64_t* table = nullptr;  // then the 32-bit look-ups
+    uint32_t* high = nullptr;
 };
 
 namespace {
@@ -264,12 +265,13 @@ int hs_weight_rule_new(hs_dev* dev, const uint64_t* table, uint32_t table_len, h
         while (r->last_weight + 1 < r->len && table[r->last_weight + 1] != 0) r->last_weight++;
         DeviceScope on(r->dev.ordinal);
         if (on.e != cudaSuccess) return cuda_fail("cudaSetDevice", on.e);
-        std::vector<uint64_t> t(table, table + table_len);
-        t.resize((t.size() + 1) & ~(size_t)1, 0);
-        cudaError_t e = cudaMalloc(&r->table, 8 * t.size());
+        const std::vector<uint32_t> high = weight_high(table, table_len);
+        const size_t bytes = 8 * (((size_t)table_len + 1) & ~(size_t)1);  // `high` starts 16-byte aligned
+        cudaError_t e = cudaMalloc(&r->table, bytes + 4 * high.size());
         if (e != cudaSuccess) return cuda_fail("cudaMalloc", e);
-        e = cudaMemcpy(r->table, t.data(), 8 * t.size(), cudaMemcpyHostToDevice);
-        if (e != cudaSuccess) {
+        r->high = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(r->table) + bytes);
+        if ((e = cudaMemcpy(r->table, table, 8 * (size_t)table_len, cudaMemcpyHostToDevice)) != cudaSuccess ||
+            (e = cudaMemcpy(r->high, high.data(), 4 * high.size(), cudaMemcpyHostToDevice)) != cudaSuccess) {
             cudaFree(r->table);
             return cuda_fail("cudaMemcpy", e);
         }
@@ -318,9 +320,11 @@ int hs_op_beam_select(hs_weight_rule* rule, const hs_beam_select* a, void* strea
         b.token = a->token;
         b.cost = a->cost;
         b.table = rule->table;
+        b.high = rule->high;
         b.tlen = rule->len;
         b.last_weight = rule->last_weight;
         b.cut_bits = weight_cut_bits(rule->first);
+        b.first = rule->first;
         b.tsh = (int)a->tile_shift;
         b.vocab = (int)a->vocab;
         b.groups = (int)a->groups;

@@ -183,6 +183,7 @@ struct hs_model {
     int32_t* attn_exp = nullptr;
     int attn_len = 0;
     uint64_t* logits_exp = nullptr;
+    uint32_t* logits_high = nullptr;  // their upper 32 bits (BeamArgs::high)
     int logits_len = 0;
     int logits_head = 0;  // the last index j with logits_exp[j] == logits_exp[0]
     int logits_last_weight = 0;  // the last index j with logits_exp[j] != 0
@@ -1681,9 +1682,11 @@ int beam_step(hs_batch* b, uint32_t groups, uint32_t beams, uint32_t* slots, uin
     a.token = d_token;
     a.cost = b->d_beam_cost + Rc;
     a.table = m->logits_exp;
+    a.high = m->logits_high;
     a.tlen = m->logits_len;
     a.last_weight = m->logits_last_weight;
     a.cut_bits = weight_cut_bits(m->logits_first);
+    a.first = m->logits_first;
     a.tsh = c.tsh;
     a.vocab = c.V;
     a.groups = (int)groups;
@@ -1994,6 +1997,10 @@ int hs_model_load(hs_dev* dev, const uint8_t* file, size_t len, hs_model** out) 
     m->logits_len = (int)M.logits_exp.size();
     while (m->logits_head + 1 < m->logits_len && M.logits_exp[m->logits_head + 1] == M.logits_exp[0]) m->logits_head++;
     m->logits_first = M.logits_exp[0];
+    {
+        const std::vector<uint32_t> high = weight_high(M.logits_exp.data(), M.logits_exp.size());
+        if ((rc = upload(&m->logits_high, high.data(), high.size(), m->owned))) return rc;
+    }
     while (m->logits_last_weight + 1 < m->logits_len && M.logits_exp[m->logits_last_weight + 1] != 0)
         m->logits_last_weight++;
     m->weight_bytes += M.wpe.size() + 8 * M.logits_exp.size() + 4 * M.attn_exp.size();
