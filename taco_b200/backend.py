@@ -907,7 +907,7 @@ class _Rule:
         self.h = ctypes.c_void_p()
 
     def close(self):
-        if getattr(self, "h", None):
+        if getattr(self, "h", None) and lib is not None:  # (None while the interpreter ends)
             getattr(lib(), self._free)(self.h)
             self.h = None
 

@@ -133,18 +133,49 @@ __global__ void __launch_bounds__(ANY_THREADS) k_tree_attention_any(const TreeAr
 
 constexpr int TW = 8;              // warps of a block
 constexpr int TTHREADS = 32 * TW;
-constexpr int CH = 16;             // channels of O at a time
-constexpr int PSTRIDE = CH + 2;    // 64-bit words of a row of the warps' O (padded against bank conflicts)
+constexpr int TMAXC = 8;           // blocks of a cluster
+constexpr int CH = 64;             // channels of O that the warps' parts hold at a time
 
 __device__ __forceinline__ void mma_s8s8(int32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The first product of a sum: C is 0.
+__device__ __forceinline__ void mma_s8s8_first(int32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+}
+__device__ __forceinline__ void mma_u8s8_first(int32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+}
 __device__ __forceinline__ void mma_u8s8(int32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// ceil_pow2_div (hs_common.cuh) without a 64-bit division. The residual R = 2^sh - x s of the first estimate
+// x is at most 2^11 s in magnitude, so the double quotient R / s is within 2^-40 of the exact one, and with
+// its whole part taken off |R| is at most s + 12 (s < 2^44). Up to two unit steps then make x the least
+// value with x s >= 2^sh, which has -s < R <= 0.
+__device__ __forceinline__ uint64_t ceil_pow2_div_near(int sh, uint64_t s) {
+    const double inv = 1.0 / (double)s;
+    uint64_t x = (uint64_t)(inv * pow2_double(sh));
+    int64_t R = (int64_t)((1ull << (sh & 63)) * (sh < 64 ? 1ull : 0ull) - x * s);  // mod 2^64: |R| < 2^63
+    const int64_t d = (int64_t)((double)R * inv);
+    x += (uint64_t)d;
+    R -= d * (int64_t)s;
+    if (R > 0) {
+        x += 1;
+        R -= (int64_t)s;
+    }
+    if (R > 0) x += 1;
+    if (R <= -(int64_t)s) x -= 1;
+    return x;
 }
 
 // The bits of the keys first .. first + 31 that a row sees: the context (below `prefix`) and the tree's
@@ -161,25 +192,34 @@ __device__ __forceinline__ uint32_t seen_word(const uint32_t* mask, int first, i
     return __funnelshift_r(word(t >> 5), word((t >> 5) + 1), t & 31);
 }
 
-// What the rows of an item share: per row the maximum's score, then the multiplier and shift of p.
-struct RowState {
-    int64_t top;
-    uint32_t mh, ml;
-    int shift;
-};
+// clamp(rescale(256 x + y, om, os), -127, 127) for |y| <= 2^28, in single precision where `fast`: os <= 95 and
+// |om 2^-os| <= 2^-19. The estimate z of the value plus 1/2 takes the two parts, their sum, the factor and
+// the product with a rounding each: an error of at most 2^-22 |z| + 32 |om 2^-os|, below 2^-13 for |z| <
+// 256. Values nearer than that to a whole number take the exact rule.
+__device__ __forceinline__ int32_t output_of(int2 o, int32_t om, int os, float fsc, double omsc, bool fast) {
+    const float z = fmaf(fmaf((float)o.x, 256.0f, (float)o.y), fsc, 0.5f);
+    const float fl = floorf(z), fr = z - fl;
+    if (fast) {
+        if (fabsf(z) >= 256.0f) return z > 0 ? 127 : -127;
+        if (fr > 1.220703125e-4f && fr < 1.0f - 1.220703125e-4f) return min(max((int32_t)fl, -127), 127);
+    }
+    return rescale_clamp127((int64_t)o.x * 256 + o.y, om, os, omsc);
+}
 
+// O of a row and channel in two whole numbers, sum (p >> 8) v and sum (p & 255) v: with sum p <= 2^30 and
+// |v| <= 128 the first is at most 2^29 in magnitude over all keys, the second at most 8192 * 2^15 = 2^28.
 struct TreeSmem {
-    int32_t wmax[TW][16];
-    uint64_t wsum[TW][16];
-    int32_t bmax[16];   // of this block
-    uint64_t bsum[16];
-    RowState row[16];
-    int64_t part[2][TW][16][PSTRIDE];  // O of each warp, 16 channels, two buffers
+    // O of each warp. The channels of odd rows are 8 pairs off (exclusive or), so that the two rows of a
+    // quarter warp's stores take all the banks.
+    __align__(16) int2 part[TW][16][CH];
+    // By slice of the item, the row maxima and sums (each block of a cluster has all of them).
+    uint64_t wsum[TW * TMAXC][16];
 };
+__device__ __forceinline__ int part_at(int row, int ch) { return ch ^ ((row & 1) << 3); }
 
-template <int HD>
-constexpr size_t tree_smem() {
-    return 4 * ATTN_TABLE_MAX + sizeof(TreeSmem) + 8 * 16 * HD;
+// (a single block takes TW slices of wsum, then wmax behind them)
+constexpr size_t tree_smem(int C) {
+    return 4 * ATTN_TABLE_MAX + 8 * TW * 16 * CH + (size_t)TW * C * 16 * 12;
 }
 
 template <int HD, int NT, bool NARROW, bool SSHI>
@@ -188,24 +228,54 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
     constexpr int S = 8 * NT;        // keys of a warp
     constexpr int TK = 2 * NT;       // keys of a thread
     constexpr int KB = HD / 64;      // 16-byte pieces of a key's row per thread
+    constexpr int VB = TK / 4;       // words of a channel's values per thread
     extern __shared__ __align__(16) uint8_t s_tree[];
     int32_t* sT = reinterpret_cast<int32_t*>(s_tree);
     TreeSmem& sm = *reinterpret_cast<TreeSmem*>(s_tree + 4 * ATTN_TABLE_MAX);
-    int64_t* sO = reinterpret_cast<int64_t*>(s_tree + 4 * ATTN_TABLE_MAX + sizeof(TreeSmem));  // [16][HD] (clusters)
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    int32_t(*wmax)[16] = reinterpret_cast<int32_t(*)[16]>(&sm.wsum[TW * C]);
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
     const int32_t m = a.rule.sm;
     const int ss = a.rule.ss, last = a.rule.tlen - 1, G = a.n_head / a.n_kv;
     const int64_t half = ss >= 1 && ss <= 62 ? 1LL << (ss - 1) : 0;  // the narrow rule
     const double omsc = (double)a.rule.om * exp2_neg(a.rule.os);
+    const float fsc = (float)omsc;
+    const bool fast = a.rule.os <= 95 && fabs(omsc) <= 1.9073486328125e-6;
     for (int i = tid; i < (a.rule.tlen + 3) / 4; i += TTHREADS)
         reinterpret_cast<int4*>(sT)[i] = reinterpret_cast<const int4*>(a.rule.table)[i];
-    __syncthreads();
+    auto meet = [&]() {  // of all the item's warps
+        if (C > 1) cl.sync();
+        else __syncthreads();
+    };
+    // No block of the cluster writes to another before that one runs.
+    meet();
 
-    for (int item = blockIdx.x / C; item < items; item += gridDim.x / C) {
+    // The keys and values of an item's slice of this warp, on their way into L2.
+    auto ask = [&](const TreeSeq& s, int kv, int tile, bool keys) {
+        const int n = (int)(s.prefix + s.count), k0 = (w * C + rank) * S;
+        if (!tree_seq_ok(s, a.n_rows, a.cache.slots, a.max_count, a.max_keys) || k0 >= n || 16 * tile >= (int)s.count * G)
+            return;
+        const size_t plane = (size_t)s.slot * a.cache.slot_stride +
+                             (size_t)(a.plane0 + kv) * ((size_t)a.cache.n_ctx * HD);
+        if (keys) {
+            const int8_t* K = a.cache.k + plane + (size_t)k0 * HD;
+            for (int x = lane * 128; x < min(S, n - k0) * HD; x += 32 * 128)
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(K + x));
+        }
+        const int8_t* V = a.cache.v + plane + k0;
+        for (int ch = lane; ch < HD; ch += 32)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(V + (size_t)ch * a.cache.n_ctx));
+    };
+    const int stride = gridDim.x / C;
+    auto seq_of = [&](int item) { return a.seqs[min(item, items - 1) / tiles / a.n_kv]; };
+    TreeSeq next = seq_of(blockIdx.x / C);
+    ask(next, (int)(blockIdx.x / C) / tiles % a.n_kv, (int)(blockIdx.x / C) % tiles, false);
+
+    for (int item = blockIdx.x / C; item < items; item += stride) {
         const int tile = item % tiles, kv = (item / tiles) % a.n_kv;
-        const TreeSeq s = a.seqs[item / tiles / a.n_kv];
+        const TreeSeq s = next;
+        next = seq_of(item + stride);
         if (!tree_seq_ok(s, a.n_rows, a.cache.slots, a.max_count, a.max_keys)) {
             if (tid == 0) atomicCAS(err, 0, ERR_DRAFT_SEQ);
             continue;
@@ -215,7 +285,7 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
         const int prefix = (int)s.prefix, n = prefix + (int)s.count;
         const int slices = (n + S - 1) / S;
         const int live = (slices - rank + C - 1) / C;  // this block's warps with keys
-        const int k0 = (w * C + rank) * S;
+        const int slice = w * C + rank, k0 = slice * S;
         const bool on = w < live;
         const size_t plane = (size_t)s.slot * a.cache.slot_stride +
                              (size_t)(a.plane0 + kv) * ((size_t)a.cache.n_ctx * HD);
@@ -225,9 +295,6 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
         uint32_t seen[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
         bool whole = true;
         if (on) {
-            // V of this warp's keys on its way into L2 while the scores are made.
-            for (int ch = lane; ch < HD; ch += 32)
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(V + (size_t)ch * a.cache.n_ctx + k0));
             uint32_t q[2 * KB][4];
 #pragma unroll
             for (int r = 0; r < 2; r++) {
@@ -245,16 +312,36 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
                 }
             }
             const int kcol = k0 + (g >> 1) * TK + (g & 1);
+            const uint4* kp = reinterpret_cast<const uint4*>(K + (size_t)kcol * HD) + t;
+            constexpr int DEEP = KB == 1 ? NT : NT < 8 ? NT : 8;  // tiles in flight
+            const int rest = n - kcol;
 #pragma unroll
-            for (int i = 0; i < NT; i++) {
-                c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0;
-                const int key = kcol + 2 * i;
-                const uint4* p = reinterpret_cast<const uint4*>(K + (size_t)key * HD) + t;
+            for (int i0 = 0; i0 < NT; i0 += DEEP) {
+                uint4 kw[DEEP][KB];
+                // Keys past the last row of the context are not read (their weights are 0 by the mask).
+                if (k0 + S <= n) {
 #pragma unroll
-                for (int b = 0; b < KB; b++) {
-                    const uint4 v = key < n ? __ldg(p + 4 * b) : make_uint4(0, 0, 0, 0);
-                    mma_s8s8(c[i], q[2 * b], v.x, v.y);
-                    mma_s8s8(c[i], q[2 * b + 1], v.z, v.w);
+                    for (int i = 0; i < DEEP; i++)
+#pragma unroll
+                        for (int b = 0; b < KB; b++) kw[i][b] = __ldg(kp + 2 * (i0 + i) * (HD / 16) + 4 * b);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < DEEP; i++)
+#pragma unroll
+                        for (int b = 0; b < KB; b++) {
+                            kw[i][b] = make_uint4(0, 0, 0, 0);
+                            if (2 * (i0 + i) < rest) kw[i][b] = __ldg(kp + 2 * (i0 + i) * (HD / 16) + 4 * b);
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < DEEP; i++) {
+                    mma_s8s8_first(c[i0 + i], q[0], kw[i][0].x, kw[i][0].y);
+                    mma_s8s8(c[i0 + i], q[1], kw[i][0].z, kw[i][0].w);
+#pragma unroll
+                    for (int b = 1; b < KB; b++) {
+                        mma_s8s8(c[i0 + i], q[2 * b], kw[i][b].x, kw[i][b].y);
+                        mma_s8s8(c[i0 + i], q[2 * b + 1], kw[i][b].z, kw[i][b].w);
+                    }
                 }
             }
             // Slices inside the context are whole for every row.
@@ -267,12 +354,10 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
                     seen[r] = x < rows ? seen_word(a.mask + at * a.mask_words, k0 + t * TK, prefix, (int)s.count) : 0;
                 }
             }
-        }
-        // The row extremes of the dots: score() rises with the dot, or falls if the multiplier is negative.
-        const int32_t none = m >= 0 ? INT32_MIN : INT32_MAX;
-        int32_t ext[2] = {none, none};
-        if (on) {
-            auto scan = [&](auto better) {
+            // The row extremes of the dots: score() rises with the dot, or falls if the multiplier is negative.
+            int32_t ext[2];
+            auto scan = [&](auto better, int32_t none) {
+                ext[0] = ext[1] = none;
                 if (whole) {
 #pragma unroll
                     for (int i = 0; i < NT; i++) {
@@ -291,36 +376,39 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
 #pragma unroll
                     for (int r = 0; r < 2; r++) ext[r] = better(ext[r], __shfl_xor_sync(0xffffffffu, ext[r], o));
             };
-            if (m >= 0) scan([](int32_t x, int32_t y) { return max(x, y); });
-            else scan([](int32_t x, int32_t y) { return min(x, y); });
-            if (t == 0) {
-                sm.wmax[w][g] = ext[0];
-                sm.wmax[w][g + 8] = ext[1];
+            if (m >= 0) scan([](int32_t x, int32_t y) { return max(x, y); }, INT32_MIN);
+            else scan([](int32_t x, int32_t y) { return min(x, y); }, INT32_MAX);
+            // Lane t of a quad gives it to the blocks t, t + 4.
+            for (int b = t; b < C; b += 4) {
+                int32_t* to = C > 1 ? cl.map_shared_rank(&wmax[slice][0], b) : wmax[slice];
+                to[g] = ext[0];
+                to[g + 8] = ext[1];
             }
         }
-        __syncthreads();
-        if (tid < 16) {
-            int32_t e = none;
-            for (int i = 0; i < live; i++) e = m >= 0 ? max(e, sm.wmax[i][tid]) : min(e, sm.wmax[i][tid]);
-            sm.bmax[tid] = e;
-        }
-        if (C > 1) cl.sync();
-        if (tid < 16) {
-            int32_t e = sm.bmax[tid];
-            for (int i = 0; i < C; i++) {
-                const int32_t o = *cl.map_shared_rank(&sm.bmax[tid], i);
-                e = m >= 0 ? max(e, o) : min(e, o);
-            }
-            sm.row[tid].top = e == none ? 0 : NARROW ? ((int64_t)e * m + half) >> ss : tree_score(e, m, ss);
-        }
-        __syncthreads();
-        // The weights and their sums.
+        meet();
+        if (item + stride < items) ask(next, (item + stride) / tiles % a.n_kv, (item + stride) % tiles, true);
+        uint32_t mh[2] = {}, ml[2] = {};
+        int shift[2] = {};
         if (on) {
-            const int64_t top[2] = {sm.row[g].top, sm.row[g + 8].top};
+            // Lane l has row l % 16: its maximum's score, for the lanes of the row.
+            int32_t e = m >= 0 ? INT32_MIN : INT32_MAX;
+            const int32_t none = e;
+            for (int i = 0; i < slices; i++) e = m >= 0 ? max(e, wmax[i][lane & 15]) : min(e, wmax[i][lane & 15]);
+            const int64_t mine = e == none ? 0 : NARROW ? ((int64_t)e * m + half) >> ss : tree_score(e, m, ss);
+            int64_t top[2];
+            if constexpr (NARROW) {
+                top[0] = __shfl_sync(0xffffffffu, (int32_t)mine, g);
+                top[1] = __shfl_sync(0xffffffffu, (int32_t)mine, g + 8);
+            } else {
+                top[0] = __shfl_sync(0xffffffffu, mine, g);
+                top[1] = __shfl_sync(0xffffffffu, mine, g + 8);
+            }
+            // The weights and their sums.
             uint64_t sum[2] = {0, 0};
             auto weigh = [&](auto all) {
 #pragma unroll
                 for (int i = 0; i < NT; i++) {
+                    uint32_t both[2] = {0, 0};  // two weights, below 2^32 together
 #pragma unroll
                     for (int x = 0; x < 4; x++) {
                         int32_t d;
@@ -339,8 +427,10 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
                         if constexpr (!decltype(all)::value)
                             if (((seen[x >> 1] >> (2 * i + (x & 1))) & 1) == 0) e = 0;
                         c[i][x] = (int32_t)e;
-                        sum[x >> 1] += e;
+                        both[x >> 1] += e;
                     }
+                    sum[0] += both[0];
+                    sum[1] += both[1];
                 }
             };
             if (whole) weigh(std::true_type{});
@@ -349,34 +439,53 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
             for (int o = 1; o <= 2; o <<= 1)
 #pragma unroll
                 for (int r = 0; r < 2; r++) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], o);
-            if (t == 0) {
-                sm.wsum[w][g] = sum[0];
-                sm.wsum[w][g + 8] = sum[1];
+            for (int b = t; b < C; b += 4) {
+                uint64_t* to = C > 1 ? cl.map_shared_rank(&sm.wsum[slice][0], b) : sm.wsum[slice];
+                to[g] = sum[0];
+                to[g + 8] = sum[1];
             }
         }
-        __syncthreads();
-        if (tid < 16) {
-            uint64_t v = 0;
-            for (int i = 0; i < live; i++) v += sm.wsum[i][tid];
-            sm.bsum[tid] = v;
-        }
-        if (C > 1) cl.sync();
-        if (tid < 16) {
-            uint64_t v = 0;
-            for (int i = 0; i < C; i++) v += *cl.map_shared_rank(&sm.bsum[tid], i);
-            if (v == 0) v = 1;
-            int l = 64 - __clzll((long long)(v - 1));  // v <= 2^l
-            if (l < 1) l = 1;
-            const uint64_t mg = ceil_pow2_div(31 + a.rule.P + l, v);
-            sm.row[tid].mh = (uint32_t)(mg >> 32);
-            sm.row[tid].ml = (uint32_t)mg;
-            sm.row[tid].shift = l - 1;
-        }
-        __syncthreads();
-        // The probabilities as byte planes, in the fragments of the second product: c[4 s + plane]
-        // becomes the four A words of plane `plane` for the 32 keys of step s.
+        meet();
+        // The words of this thread's keys in the row of a channel.
+        const int kt = k0 + t * TK;
+        const bool inside = k0 + S <= a.cache.n_ctx;
+        auto load_v = [&](int ch, uint32_t (&v)[VB]) {
+            const int8_t* vr = V + (size_t)(ch + g) * a.cache.n_ctx + kt;
+            if constexpr (TK >= 16) {
+#pragma unroll
+                for (int b = 0; b < TK / 16; b++) {
+                    // (past n the probabilities are 0: any bytes of the row do)
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (inside || kt + 16 * b < a.cache.n_ctx) x = __ldg(reinterpret_cast<const uint4*>(vr) + b);
+                    v[4 * b] = x.x;
+                    v[4 * b + 1] = x.y;
+                    v[4 * b + 2] = x.z;
+                    v[4 * b + 3] = x.w;
+                }
+            } else {
+                uint2 x = make_uint2(0, 0);
+                if (inside || kt < a.cache.n_ctx) x = __ldg(reinterpret_cast<const uint2*>(vr));
+                v[0] = x.x;
+                v[1] = x.y;
+            }
+        };
+        uint32_t v[2][VB];
         if (on) {
-            const RowState r0 = sm.row[g], r1 = sm.row[g + 8];
+            load_v(0, v[0]);
+            uint64_t z = 0;
+            for (int i = 0; i < slices; i++) z += sm.wsum[i][lane & 15];
+            if (z == 0) z = 1;
+            int l = 64 - __clzll((long long)(z - 1));  // z <= 2^l
+            if (l < 1) l = 1;
+            const uint64_t mg = ceil_pow2_div_near(31 + a.rule.P + l, z);
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                mh[r] = __shfl_sync(0xffffffffu, (uint32_t)(mg >> 32), g + 8 * r);
+                ml[r] = __shfl_sync(0xffffffffu, (uint32_t)mg, g + 8 * r);
+                shift[r] = __shfl_sync(0xffffffffu, l - 1, g + 8 * r);
+            }
+            // The probabilities as byte planes, in the fragments of the second product: c[4 s + plane]
+            // becomes the four A words of plane `plane` for the 32 keys of step s.
 #pragma unroll
             for (int i = 0; i < NT; i += 4) {
                 uint32_t pl[4][4];
@@ -388,9 +497,8 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             const uint32_t e = (uint32_t)c[i + 2 * h + (k >> 1)][2 * r + (k & 1)];
-                            const RowState& z = r ? r1 : r0;
-                            const uint64_t u = (uint64_t)e * z.mh + __umulhi(e, z.ml);
-                            p[k] = (uint32_t)(u >> z.shift);
+                            const uint64_t u = (uint64_t)e * mh[r] + __umulhi(e, ml[r]);
+                            p[k] = (uint32_t)(u >> shift[r]);
                         }
                         const uint32_t x0 = __byte_perm(p[0], p[1], 0x5140), x1 = __byte_perm(p[0], p[1], 0x7362);
                         const uint32_t y0 = __byte_perm(p[2], p[3], 0x5140), y1 = __byte_perm(p[2], p[3], 0x7362);
@@ -405,72 +513,82 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
                     for (int x = 0; x < 4; x++) c[i + k][x] = (int32_t)pl[k][x];
             }
         }
-        // O, 16 channels at a time: each warp its keys' part, then the sum over the warps.
-        const int orow = tid / CH, och = tid % CH;
-#pragma unroll 1
+        // O, CH channels at a time: each warp its keys' part, then the sum over the warps.
+        const int row = tid / (CH / 4), ch = tid % (CH / 4) * 4;
+        int2 acc[HD / CH][4] = {};
+        auto put = [&](int r, int at, const int2 (&o)[4]) {
+            const size_t node = (size_t)s.first_row + (16 * tile + r) / G;
+            int8_t* to = a.out + node * a.out_stride + (size_t)(kv * G + (16 * tile + r) % G) * HD + at;
+#pragma unroll
+            for (int x = 0; x < 4; x++) to[x] = (int8_t)output_of(o[x], a.rule.om, a.rule.os, fsc, omsc, fast);
+        };
+#pragma unroll
         for (int ch0 = 0; ch0 < HD; ch0 += CH) {
-            int64_t(*part)[16][PSTRIDE] = sm.part[(ch0 / CH) & 1];
             if (on) {
 #pragma unroll
                 for (int j = 0; j < CH / 8; j++) {
-                    // The bytes of this thread's keys in the row of channel ch0 + 8 j + g.
-                    uint32_t v[TK / 4];
-                    const int8_t* vr = V + (size_t)(ch0 + 8 * j + g) * a.cache.n_ctx;
-                    const int kt = k0 + t * TK;
-                    if constexpr (TK >= 16) {
-#pragma unroll
-                        for (int b = 0; b < TK / 16; b++) {
-                            const uint4 x = kt + 16 * b < n ? __ldg(reinterpret_cast<const uint4*>(vr + kt) + b)
-                                                            : make_uint4(0, 0, 0, 0);
-                            v[4 * b] = x.x;
-                            v[4 * b + 1] = x.y;
-                            v[4 * b + 2] = x.z;
-                            v[4 * b + 3] = x.w;
-                        }
-                    } else {
-                        const uint2 x = kt < n ? __ldg(reinterpret_cast<const uint2*>(vr + kt)) : make_uint2(0, 0);
-                        v[0] = x.x;
-                        v[1] = x.y;
-                    }
-                    int32_t o[4][4] = {};
+                    // The next 8 channels' values while these are multiplied.
+                    if (ch0 + 8 * j + 8 < HD) load_v(ch0 + 8 * j + 8, v[(j + 1) & 1]);
+                    int32_t o[4][4];
 #pragma unroll
                     for (int st = 0; st < NT / 4; st++)
 #pragma unroll
                         for (int pl = 0; pl < 4; pl++) {
                             const uint32_t A[4] = {(uint32_t)c[4 * st + pl][0], (uint32_t)c[4 * st + pl][1],
                                                    (uint32_t)c[4 * st + pl][2], (uint32_t)c[4 * st + pl][3]};
-                            mma_u8s8(o[pl], A, v[2 * st], v[2 * st + 1]);
+                            if (st == 0) mma_u8s8_first(o[pl], A, v[j & 1][0], v[j & 1][1]);
+                            else mma_u8s8(o[pl], A, v[j & 1][2 * st], v[j & 1][2 * st + 1]);
                         }
-                    // A plane's sum is at most S * 255 * 128 < 2^22 in magnitude.
 #pragma unroll
-                    for (int x = 0; x < 4; x++)
-                        part[w][g + 8 * (x >> 1)][8 * j + 2 * t + (x & 1)] =
-                            (int64_t)(o[2][x] + o[3][x] * 256) * 65536 + (o[0][x] + o[1][x] * 256);
+                    for (int r = 0; r < 2; r++) {
+                        int4 x;
+                        x.x = o[1][2 * r] + (o[2][2 * r] + o[3][2 * r] * 256) * 256;
+                        x.y = o[0][2 * r];
+                        x.z = o[1][2 * r + 1] + (o[2][2 * r + 1] + o[3][2 * r + 1] * 256) * 256;
+                        x.w = o[0][2 * r + 1];
+                        *reinterpret_cast<int4*>(&sm.part[w][g + 8 * r][part_at(g, 8 * j + 2 * t)]) = x;
+                    }
                 }
             }
             __syncthreads();
-            int64_t acc = 0;
-            for (int i = 0; i < live; i++) acc += part[i][orow][och];
-            if (C > 1) {
-                sO[orow * HD + ch0 + och] = acc;
-            } else if (orow < rows) {
-                const size_t at = (size_t)s.first_row + (16 * tile + orow) / G;
-                a.out[at * a.out_stride + (size_t)(kv * G + (16 * tile + orow) % G) * HD + ch0 + och] =
-                    (int8_t)rescale_clamp127(acc, a.rule.om, a.rule.os, omsc);
-            }
+            // Four channels of a row a thread.
+            for (int i = 0; i < live; i++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const int4 y = *reinterpret_cast<const int4*>(&sm.part[i][row][part_at(row, ch + 2 * x)]);
+                    acc[ch0 / CH][2 * x].x += y.x;
+                    acc[ch0 / CH][2 * x].y += y.y;
+                    acc[ch0 / CH][2 * x + 1].x += y.z;
+                    acc[ch0 / CH][2 * x + 1].y += y.w;
+                }
+            if (HD > CH) __syncthreads();  // the parts are read
         }
         if (C > 1) {
+            // The block's sums in the place of its warps' parts (with one round of channels a thread writes
+            // where it alone has read), then each block sums some rows over the cluster.
+#pragma unroll
+            for (int h = 0; h < HD / CH; h++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) sm.part[h][row][ch + x] = acc[h][x];
             cl.sync();
-            for (int i = rank * TTHREADS + tid; i < 16 * HD; i += C * TTHREADS) {
-                int64_t acc = 0;
-                for (int b = 0; b < C; b++) acc += *cl.map_shared_rank(&sO[i], b);
-                const int r = i / HD;
-                if (r < rows) {
-                    const size_t at = (size_t)s.first_row + (16 * tile + r) / G;
-                    a.out[at * a.out_stride + (size_t)(kv * G + (16 * tile + r) % G) * HD + i % HD] =
-                        (int8_t)rescale_clamp127(acc, a.rule.om, a.rule.os, omsc);
+            constexpr int QUADS = HD / 4;
+            for (int i = rank * TTHREADS + tid; i < 16 * QUADS; i += C * TTHREADS) {
+                const int r = i / QUADS, c4 = i % QUADS * 4;
+                int2 sum4[4] = {};
+                for (int b = 0; b < C; b++) {
+                    const int2* of = cl.map_shared_rank(&sm.part[c4 / CH][r][c4 % CH], b);
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        sum4[x].x += of[x].x;
+                        sum4[x].y += of[x].y;
+                    }
                 }
+                if (r < rows) put(r, c4, sum4);
             }
+            cl.sync();  // (the parts are written again after two more meetings; this one is for HD > CH)
+        } else if (row < rows) {
+#pragma unroll
+            for (int h = 0; h < HD / CH; h++) put(row, h * CH + ch, acc[h]);
         }
     }
     if (C > 1) cl.sync();  // no block leaves while another reads its memory
@@ -484,7 +602,7 @@ cudaError_t launch_tree_mma(const TreeArgs& a, int C, int num_sms, int* err, cud
     const int clusters = 2 * num_sms / C;
     cfg.gridDim = dim3((unsigned)(items < clusters ? items : clusters) * C);
     cfg.blockDim = dim3(TTHREADS);
-    cfg.dynamicSmemBytes = tree_smem<HD>();
+    cfg.dynamicSmemBytes = tree_smem(C);
     cfg.stream = st;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;
@@ -508,18 +626,21 @@ cudaError_t launch_tree_rule(const TreeArgs& a, int C, int num_sms, int* err, cu
 
 template <int HD>
 cudaError_t launch_tree_width(const TreeArgs& a, int num_sms, int* err, cudaStream_t st) {
+    // Short contexts: smaller slices, so that all the warps of a block have keys.
+    if (a.max_keys <= TW * 32) return launch_tree_rule<HD, 4>(a, 1, num_sms, err, st);
+    if (a.max_keys <= TW * 64) return launch_tree_rule<HD, 8>(a, 1, num_sms, err, st);
     int C = 1;
     while (C * TW * 128 < a.max_keys) C *= 2;
     return launch_tree_rule<HD, 16>(a, C, num_sms, err, st);
 }
 
-template <int HD>
+template <int HD, int NT>
 cudaError_t configure_tree() {
-    const void* fns[3] = {(const void*)k_tree_attention<HD, 16, true, true>,
-                          (const void*)k_tree_attention<HD, 16, true, false>,
-                          (const void*)k_tree_attention<HD, 16, false, false>};
+    const void* fns[3] = {(const void*)k_tree_attention<HD, NT, true, true>,
+                          (const void*)k_tree_attention<HD, NT, true, false>,
+                          (const void*)k_tree_attention<HD, NT, false, false>};
     for (const void* f : fns) {
-        const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tree_smem<HD>());
+        const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tree_smem(TMAXC));
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -540,8 +661,12 @@ cudaError_t launch_tree_attention(const TreeArgs& a, int num_sms, int* err, cuda
 }
 
 cudaError_t configure_draft_kernels() {
-    cudaError_t e = configure_tree<64>();
-    if (e == cudaSuccess) e = configure_tree<128>();
+    cudaError_t e = configure_tree<64, 4>();
+    if (e == cudaSuccess) e = configure_tree<64, 8>();
+    if (e == cudaSuccess) e = configure_tree<64, 16>();
+    if (e == cudaSuccess) e = configure_tree<128, 4>();
+    if (e == cudaSuccess) e = configure_tree<128, 8>();
+    if (e == cudaSuccess) e = configure_tree<128, 16>();
     if (e == cudaSuccess) e = configure_beam();
     if (e != cudaSuccess) return e;
     return cudaFuncSetAttribute((const void*)k_tree_attention_any, cudaFuncAttributeMaxDynamicSharedMemorySize,
