@@ -9,6 +9,7 @@
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <type_traits>
 
@@ -613,14 +614,19 @@ cudaError_t launch_tree_mma(const TreeArgs& a, int C, int num_sms, int* err, cud
     return cudaLaunchKernelEx(&cfg, k_tree_attention<HD, NT, NARROW, SSHI>, a, tiles, items, err);
 }
 
+// Which score rule fits: 0 wide; 1 narrow: every |score| is below 2^30, so distances fit in 32 bits and no
+// score reaches the clamp; 2 narrow with a shift of at least 32.
+int score_rule(const AttnRuleView& r, int hd) {
+    const uint64_t m = (uint64_t)(r.sm < 0 ? -(int64_t)r.sm : (int64_t)r.sm);
+    const bool narrow = r.ss >= 1 && r.ss <= 62 && ((m * ((uint64_t)hd << 14)) >> r.ss) + 1 < (1ull << 30);
+    return narrow ? r.ss >= 32 ? 2 : 1 : 0;
+}
+
 template <int HD, int NT>
 cudaError_t launch_tree_rule(const TreeArgs& a, int C, int num_sms, int* err, cudaStream_t st) {
-    // Narrow: every |score| is below 2^30, so distances fit in 32 bits and no score reaches the clamp.
-    const int ss = a.rule.ss;
-    const uint64_t m = (uint64_t)(a.rule.sm < 0 ? -(int64_t)a.rule.sm : (int64_t)a.rule.sm);
-    const bool narrow = ss >= 1 && ss <= 62 && ((m * ((uint64_t)HD << 14)) >> ss) + 1 < (1ull << 30);
-    if (narrow && ss >= 32) return launch_tree_mma<HD, NT, true, true>(a, C, num_sms, err, st);
-    if (narrow) return launch_tree_mma<HD, NT, true, false>(a, C, num_sms, err, st);
+    const int rule = score_rule(a.rule, HD);
+    if (rule == 2) return launch_tree_mma<HD, NT, true, true>(a, C, num_sms, err, st);
+    if (rule == 1) return launch_tree_mma<HD, NT, true, false>(a, C, num_sms, err, st);
     return launch_tree_mma<HD, NT, false, false>(a, C, num_sms, err, st);
 }
 
@@ -628,10 +634,12 @@ template <int HD>
 cudaError_t launch_tree_width(const TreeArgs& a, int num_sms, int* err, cudaStream_t st) {
     // Short contexts: smaller slices, so that all the warps of a block have keys.
     if (a.max_keys <= TW * 32) return launch_tree_rule<HD, 4>(a, 1, num_sms, err, st);
-    if (a.max_keys <= TW * 64) return launch_tree_rule<HD, 8>(a, 1, num_sms, err, st);
-    int C = 1;
-    while (C * TW * 128 < a.max_keys) C *= 2;
-    return launch_tree_rule<HD, 16>(a, C, num_sms, err, st);
+    if (HD == 64 || a.max_keys <= TW * 64) return launch_tree_rule<HD, 8>(a, 1, num_sms, err, st);
+    if constexpr (HD > 64) {
+        int C = 1;
+        while (C * TW * 128 < a.max_keys) C *= 2;
+        return launch_tree_rule<HD, 16>(a, C, num_sms, err, st);
+    }
 }
 
 template <int HD, int NT>
@@ -646,12 +654,513 @@ cudaError_t configure_tree() {
     return cudaSuccess;
 }
 
+// ---- head width 64: keys and values by bulk copies ----
+//
+// The mathematics and the fragments of the kernel above, with the operands ahead of the work: a producer
+// warp copies the keys (up to 1,024 rows) and the transposed values of a tree's kv head into shared memory,
+// the next head's keys while this one's probabilities are made and its values multiplied, the next values
+// while this one's scores are made. One block per SM, 16 warps for the rows:
+//   GROUPS = 2: two groups of 8 warps take the 16-row tiles of the head in turn, 128 keys a warp. The
+//     groups meet only within themselves, so one multiplies while the other weighs.
+//   GROUPS = 1: 16 warps share the only tile, 64 keys a warp.
+// Contexts over 1,024 keys take a cluster, a block for each 1,024 keys; the row maxima and sums go to every
+// block's shared memory, the blocks' O to the block that owns the row, with an mbarrier of the group for
+// each meeting.
+// The warps of a group add their O into shared memory with integer atomics (whole numbers: no order).
+
+constexpr int BK = 1024;                 // keys of a block
+constexpr int BWARPS = 16;               // warps for the rows; one more copies
+constexpr int BTHREADS = 32 * (BWARPS + 1);
+constexpr int VROW = BK + 16;            // bytes of a channel's values (padded: two rows in a quarter warp's banks)
+constexpr int OROW = 68;                 // words of a row of O: even channels, then odd ones, all banks a store
+
+template <int GROUPS>
+struct __align__(16) TreeBulk {
+    uint8_t k[BK * 64];
+    uint8_t v[64 * VROW];
+    int32_t table[ATTN_TABLE_MAX];
+    int32_t o[GROUPS][2][16][OROW];      // this block's O
+    int32_t whole[GROUPS][2][16][OROW];  // of the rows that this block owns, over the cluster
+    uint64_t k_full, k_empty, v_full, v_empty;
+    uint64_t met[GROUPS][3];             // the meetings of a cluster's groups: maxima, sums, O
+};
+// (behind it per group: wsum [slices][16] u64 and wmax [slices][16] i32, slices = C * warps of a group)
+template <int GROUPS>
+constexpr size_t bulk_smem(int C) {
+    return sizeof(TreeBulk<GROUPS>) + (size_t)GROUPS * C * (BWARPS / GROUPS) * 16 * 12;
+}
+static_assert(bulk_smem<2>(8) <= 227 * 1024 && bulk_smem<1>(8) <= 227 * 1024, "a block's shared memory");
+
+__device__ __forceinline__ int o_at(int ch) { return (ch & 1) * 32 + (ch >> 1); }
+
+// Arrives on the mbarrier at the same place of block `rank` of the cluster, after this thread's writes.
+__device__ __forceinline__ void mbar_arrive_cluster(uint64_t* bar, int rank) {
+    asm volatile(
+        "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, %1;\n\t"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(rank)
+        : "memory");
+}
+__device__ __forceinline__ void mbar_wait_cluster(uint64_t* bar, uint32_t phase, int* err, int code) {
+    for (uint32_t i = 0; i < (1u << 26); i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(phase)
+            : "memory");
+        if (ok) return;
+        if (i > 64) __nanosleep(32);
+        if ((i & 1023) == 0 && *(volatile int*)err != 0) return;
+    }
+    atomicCAS(err, 0, code);
+}
+
+// A wait that gives up sets the error word and lets its thread go on: every barrier still gets its arrivals,
+// every later wait returns at once, and the call's results count for nothing.
+template <int GROUPS, bool NARROW, bool SSHI>
+__global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __grid_constant__ TreeArgs a, int works,
+                                                                     int* err) {
+    constexpr int HD = 64, WPG = BWARPS / GROUPS, NT = BK / WPG / 8, S = 8 * NT, TK = 2 * NT, VB = TK / 4;
+    constexpr int GTHREADS = 32 * WPG, PER = 16 * HD / GTHREADS;  // outputs of a thread
+    extern __shared__ __align__(128) uint8_t s_bulk[];
+    TreeBulk<GROUPS>& sm = *reinterpret_cast<TreeBulk<GROUPS>*>(s_bulk);
+    cg::cluster_group cl = cg::this_cluster();
+    const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int G = a.n_head / a.n_kv, first = blockIdx.x / C, stride = gridDim.x / C;
+    if (tid == 0) {
+        mbar_init(&sm.k_full, 1);
+        mbar_init(&sm.k_empty, BWARPS);
+        mbar_init(&sm.v_full, 1);
+        mbar_init(&sm.v_empty, BWARPS);
+        for (int i = 0; i < GROUPS; i++)
+            for (int k = 0; k < 3; k++) mbar_init(&sm.met[i][k], WPG * C);
+        fence_barrier_init();
+    }
+    for (int i = tid; i < GROUPS * 2 * 16 * OROW; i += BTHREADS) {
+        (&sm.o[0][0][0][0])[i] = 0;
+        (&sm.whole[0][0][0][0])[i] = 0;
+    }
+    for (int i = tid; i < (a.rule.tlen + 3) / 4; i += BTHREADS)
+        reinterpret_cast<int4*>(sm.table)[i] = reinterpret_cast<const int4*>(a.rule.table)[i];
+    if (C > 1) cl.sync();
+    else __syncthreads();
+
+    if (warp == BWARPS) {
+        // The producer.
+        uint32_t count = 0;  // works copied
+        for (int work = first; work < works; work += stride) {
+            const TreeSeq s = a.seqs[work / a.n_kv];
+            if (!tree_seq_ok(s, a.n_rows, a.cache.slots, a.max_count, a.max_keys)) {
+                if (lane == 0) atomicCAS(err, 0, ERR_DRAFT_SEQ);
+                continue;
+            }
+            if (s.count == 0) continue;
+            const int n = (int)(s.prefix + s.count), k0 = rank * BK, kn = max(0, min(BK, n - k0));
+            const size_t plane = (size_t)s.slot * a.cache.slot_stride +
+                                 (size_t)(a.plane0 + work % a.n_kv) * ((size_t)a.cache.n_ctx * HD);
+            const uint32_t phase = (count & 1) ^ 1, vbytes = (uint32_t)(kn + 15) & ~15u;  // (n_ctx % 16 == 0)
+            if (!mbar_wait(&sm.k_empty, phase, err, 50)) break;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&sm.k_full, (uint32_t)kn * HD);
+                if (kn) bulk_load(sm.k, a.cache.k + plane + (size_t)k0 * HD, (uint32_t)kn * HD, &sm.k_full);
+            }
+            if (!mbar_wait(&sm.v_empty, phase, err, 51)) break;
+            if (lane == 0) mbar_arrive_expect_tx(&sm.v_full, vbytes * HD);
+            __syncwarp();
+            if (kn)
+                for (int ch = lane; ch < HD; ch += 32)
+                    bulk_load(sm.v + ch * VROW, a.cache.v + plane + (size_t)ch * a.cache.n_ctx + k0, vbytes, &sm.v_full);
+            count++;
+        }
+    } else {
+        const int grp = warp / WPG, w = warp % WPG, gtid = tid - grp * GTHREADS;
+        const int g = lane >> 2, t = lane & 3;
+        const int slice = rank * WPG + w;
+        uint64_t(*wsum)[16] = reinterpret_cast<uint64_t(*)[16]>(s_bulk + sizeof(TreeBulk<GROUPS>)) + grp * C * WPG;
+        int32_t(*wmax)[16] = reinterpret_cast<int32_t(*)[16]>(
+            reinterpret_cast<uint64_t(*)[16]>(s_bulk + sizeof(TreeBulk<GROUPS>)) + GROUPS * C * WPG) + grp * C * WPG;
+        const int32_t m = a.rule.sm;
+        const int ss = a.rule.ss, last = a.rule.tlen - 1;
+        const int64_t half = ss >= 1 && ss <= 62 ? 1LL << (ss - 1) : 0;  // the narrow rule
+        const double omsc = (double)a.rule.om * exp2_neg(a.rule.os);
+        const float fsc = (float)omsc;
+        const bool fast = a.rule.os <= 95 && fabs(omsc) <= 1.9073486328125e-6;
+        uint32_t met = 0;  // rounds of the group's meetings
+        // The group's warps, of all blocks of the cluster, at meeting k of this round.
+        auto meet = [&](int k) {
+            if (C > 1) {
+                __syncwarp();
+                if (lane < C) mbar_arrive_cluster(&sm.met[grp][k], lane);
+                mbar_wait_cluster(&sm.met[grp][k], met & 1, err, 52 + k);
+                __syncwarp();
+            } else {
+                __syncwarp();
+                named_bar(1 + grp, GTHREADS);
+            }
+        };
+        uint32_t count = 0;
+        for (int work = first; work < works; work += stride) {
+            const TreeSeq s = a.seqs[work / a.n_kv];
+            if (!tree_seq_ok(s, a.n_rows, a.cache.slots, a.max_count, a.max_keys) || s.count == 0) continue;
+            const int kv = work % a.n_kv, prefix = (int)s.prefix, n = prefix + (int)s.count;
+            const int total = (int)s.count * G, tiles = (total + 15) / 16, slices = (n + S - 1) / S;
+            const bool on = slice < slices;
+            const int k0 = slice * S;  // of the context; the block's copy starts at rank * BK
+            const uint32_t phase = count & 1;
+            count++;
+            const uint8_t* ks = sm.k + (size_t)(w * S) * HD;
+            const uint8_t* vs = sm.v + w * S + t * TK;
+            for (int tile = grp; tile < tiles; tile += GROUPS) {
+                const int rows = total - 16 * tile;
+                int32_t c[NT][4];
+                uint32_t seen[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+                bool whole = true;
+                if (on) {
+                    uint32_t q[2][4];
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        const int x = 16 * tile + g + 8 * r;
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (x < total)
+                            v = reinterpret_cast<const uint4*>(a.q + ((size_t)s.first_row + x / G) * a.q_stride +
+                                                               (size_t)(kv * G + x % G) * HD)[t];
+                        q[0][r] = v.x;
+                        q[0][2 + r] = v.y;
+                        q[1][r] = v.z;
+                        q[1][2 + r] = v.w;
+                    }
+                    // Slices inside the context are whole for every row.
+                    if (k0 + S > prefix) {
+                        whole = false;
+#pragma unroll
+                        for (int r = 0; r < 2; r++) {
+                            const int x = 16 * tile + g + 8 * r;
+                            seen[r] = x < total ? seen_word(a.mask + ((size_t)s.first_row + x / G) * a.mask_words,
+                                                            k0 + t * TK, prefix, (int)s.count)
+                                                : 0;
+                        }
+                    }
+                    if (tile == grp) mbar_wait(&sm.k_full, phase, err, 55);
+                    const uint4* kp = reinterpret_cast<const uint4*>(ks + ((g >> 1) * TK + (g & 1)) * HD) + t;
+#pragma unroll
+                    for (int i = 0; i < NT; i++) {
+                        const uint4 kw = kp[2 * i * (HD / 16)];
+                        mma_s8s8_first(c[i], q[0], kw.x, kw.y);
+                        mma_s8s8(c[i], q[1], kw.z, kw.w);
+                    }
+                } else if (tile == grp) {
+                    mbar_wait(&sm.k_full, phase, err, 55);
+                }
+                if (tile + GROUPS >= tiles) {  // the group's last scores of this head
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.k_empty);
+                }
+                if (on) {
+                    // The row extremes of the dots: score() rises with the dot, or falls if the multiplier is
+                    // negative.
+                    int32_t ext[2];
+                    auto scan = [&](auto better, int32_t none) {
+                        ext[0] = ext[1] = none;
+                        if (whole) {
+#pragma unroll
+                            for (int i = 0; i < NT; i++) {
+                                ext[0] = better(ext[0], better(c[i][0], c[i][1]));
+                                ext[1] = better(ext[1], better(c[i][2], c[i][3]));
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < NT; i++)
+#pragma unroll
+                                for (int x = 0; x < 4; x++)
+                                    if ((seen[x >> 1] >> (2 * i + (x & 1))) & 1) ext[x >> 1] = better(ext[x >> 1], c[i][x]);
+                        }
+#pragma unroll
+                        for (int o = 1; o <= 2; o <<= 1)
+#pragma unroll
+                            for (int r = 0; r < 2; r++) ext[r] = better(ext[r], __shfl_xor_sync(0xffffffffu, ext[r], o));
+                    };
+                    if (m >= 0) scan([](int32_t x, int32_t y) { return max(x, y); }, INT32_MIN);
+                    else scan([](int32_t x, int32_t y) { return min(x, y); }, INT32_MAX);
+                    // Lane t of a quad gives them to the blocks t, t + 4.
+                    for (int b = t; b < C; b += 4) {
+                        int32_t* to = C > 1 ? cl.map_shared_rank(&wmax[slice][0], b) : wmax[slice];
+                        to[g] = ext[0];
+                        to[g + 8] = ext[1];
+                    }
+                }
+                meet(0);
+                if (on) {
+                    // Lane l has row l % 16: its maximum's score, for the lanes of the row.
+                    const int32_t none = m >= 0 ? INT32_MIN : INT32_MAX;
+                    int32_t e = none;
+                    for (int i = 0; i < slices; i++) e = m >= 0 ? max(e, wmax[i][lane & 15]) : min(e, wmax[i][lane & 15]);
+                    const int64_t mine = e == none ? 0 : NARROW ? ((int64_t)e * m + half) >> ss : tree_score(e, m, ss);
+                    int64_t top[2];
+                    if constexpr (NARROW) {
+                        top[0] = __shfl_sync(0xffffffffu, (int32_t)mine, g);
+                        top[1] = __shfl_sync(0xffffffffu, (int32_t)mine, g + 8);
+                    } else {
+                        top[0] = __shfl_sync(0xffffffffu, mine, g);
+                        top[1] = __shfl_sync(0xffffffffu, mine, g + 8);
+                    }
+                    // The weights and their sums.
+                    uint64_t sum[2] = {0, 0};
+                    auto weigh = [&](auto all) {
+#pragma unroll
+                        for (int i = 0; i < NT; i++) {
+                            uint32_t both[2] = {0, 0};  // two weights, below 2^32 together
+#pragma unroll
+                            for (int x = 0; x < 4; x++) {
+                                int32_t d;
+                                if constexpr (NARROW) {
+                                    const int64_t p = (int64_t)c[i][x] * (int64_t)m + half;
+                                    int32_t y;
+                                    if constexpr (SSHI) y = (int32_t)(p >> 32) >> (ss - 32);
+                                    else y = (int32_t)__funnelshift_r((uint32_t)p, (uint32_t)((uint64_t)p >> 32), ss);
+                                    d = (int32_t)top[x >> 1] - y;
+                                    d = (uint32_t)d < (uint32_t)last ? d : last;
+                                } else {
+                                    const int64_t dd = top[x >> 1] - tree_score(c[i][x], m, ss);
+                                    d = (int32_t)((uint64_t)dd < (uint64_t)last ? dd : (int64_t)last);
+                                }
+                                uint32_t e = (uint32_t)sm.table[d];
+                                if constexpr (!decltype(all)::value)
+                                    if (((seen[x >> 1] >> (2 * i + (x & 1))) & 1) == 0) e = 0;
+                                c[i][x] = (int32_t)e;
+                                both[x >> 1] += e;
+                            }
+                            sum[0] += both[0];
+                            sum[1] += both[1];
+                        }
+                    };
+                    if (whole) weigh(std::true_type{});
+                    else weigh(std::false_type{});
+#pragma unroll
+                    for (int o = 1; o <= 2; o <<= 1)
+#pragma unroll
+                        for (int r = 0; r < 2; r++) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], o);
+                    for (int b = t; b < C; b += 4) {
+                        uint64_t* to = C > 1 ? cl.map_shared_rank(&wsum[slice][0], b) : wsum[slice];
+                        to[g] = sum[0];
+                        to[g + 8] = sum[1];
+                    }
+                }
+                meet(1);
+                if (on) {
+                    uint64_t z = 0;
+                    for (int i = 0; i < slices; i++) z += wsum[i][lane & 15];
+                    if (z == 0) z = 1;
+                    int l = 64 - __clzll((long long)(z - 1));  // z <= 2^l
+                    if (l < 1) l = 1;
+                    const uint64_t mg = ceil_pow2_div_near(31 + a.rule.P + l, z);
+                    uint32_t mh[2], ml[2];
+                    int shift[2];
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        mh[r] = __shfl_sync(0xffffffffu, (uint32_t)(mg >> 32), g + 8 * r);
+                        ml[r] = __shfl_sync(0xffffffffu, (uint32_t)mg, g + 8 * r);
+                        shift[r] = __shfl_sync(0xffffffffu, l - 1, g + 8 * r);
+                    }
+                    // The probabilities as byte planes, in the fragments of the second product: c[4 s + plane]
+                    // becomes the four A words of plane `plane` for the 32 keys of step s.
+#pragma unroll
+                    for (int i = 0; i < NT; i += 4) {
+                        uint32_t pl[4][4];
+#pragma unroll
+                        for (int r = 0; r < 2; r++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                uint32_t p[4];
+#pragma unroll
+                                for (int k = 0; k < 4; k++) {
+                                    const uint32_t e = (uint32_t)c[i + 2 * h + (k >> 1)][2 * r + (k & 1)];
+                                    const uint64_t u = (uint64_t)e * mh[r] + __umulhi(e, ml[r]);
+                                    p[k] = (uint32_t)(u >> shift[r]);
+                                }
+                                const uint32_t x0 = __byte_perm(p[0], p[1], 0x5140), x1 = __byte_perm(p[0], p[1], 0x7362);
+                                const uint32_t y0 = __byte_perm(p[2], p[3], 0x5140), y1 = __byte_perm(p[2], p[3], 0x7362);
+                                pl[0][2 * h + r] = __byte_perm(x0, y0, 0x5410);
+                                pl[1][2 * h + r] = __byte_perm(x0, y0, 0x7632);
+                                pl[2][2 * h + r] = __byte_perm(x1, y1, 0x5410);
+                                pl[3][2 * h + r] = __byte_perm(x1, y1, 0x7632);
+                            }
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+#pragma unroll
+                            for (int x = 0; x < 4; x++) c[i + k][x] = (int32_t)pl[k][x];
+                    }
+                    if (tile == grp) mbar_wait(&sm.v_full, phase, err, 56);
+                    // O of this warp's keys, added to the group's, 8 channels at a time.
+#pragma unroll 2
+                    for (int j = 0; j < HD / 8; j++) {
+                        uint32_t v[VB];
+#pragma unroll
+                        for (int b = 0; b < TK / 16; b++) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(vs + (8 * j + g) * VROW + 16 * b);
+                            v[4 * b] = x.x;
+                            v[4 * b + 1] = x.y;
+                            v[4 * b + 2] = x.z;
+                            v[4 * b + 3] = x.w;
+                        }
+                        int32_t o[4][4];
+#pragma unroll
+                        for (int st = 0; st < NT / 4; st++)
+#pragma unroll
+                            for (int pl = 0; pl < 4; pl++) {
+                                const uint32_t A[4] = {(uint32_t)c[4 * st + pl][0], (uint32_t)c[4 * st + pl][1],
+                                                       (uint32_t)c[4 * st + pl][2], (uint32_t)c[4 * st + pl][3]};
+                                if (st == 0) mma_u8s8_first(o[pl], A, v[0], v[1]);
+                                else mma_u8s8(o[pl], A, v[2 * st], v[2 * st + 1]);
+                            }
+#pragma unroll
+                        for (int x = 0; x < 4; x++) {
+                            const int row = g + 8 * (x >> 1), at = o_at(8 * j + 2 * t + (x & 1));
+                            atomicAdd(&sm.o[grp][0][row][at], o[1][x] + (o[2][x] + o[3][x] * 256) * 256);
+                            atomicAdd(&sm.o[grp][1][row][at], o[0][x]);
+                        }
+                    }
+                } else if (tile == grp) {
+                    mbar_wait(&sm.v_full, phase, err, 56);
+                }
+                if (tile + GROUPS >= tiles) {  // the group's last product of this head
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.v_empty);
+                }
+                __syncwarp();
+                named_bar(1 + grp, GTHREADS);
+                // PER channels of a row a thread (at each of two parities, PER / 2 words).
+                const int row = gtid / (HD / PER), ch = gtid % (HD / PER) * PER;
+                int2 o[PER];
+#pragma unroll
+                for (int x = 0; x < PER; x++) {
+                    const int at = o_at(ch + x);
+                    o[x] = make_int2(sm.o[grp][0][row][at], sm.o[grp][1][row][at]);
+                    sm.o[grp][0][row][at] = sm.o[grp][1][row][at] = 0;  // for the next tile
+                }
+                if (C > 1) {
+                    // The row's sums to the block that owns it.
+                    const int owner = row % C;
+                    int32_t* to = cl.map_shared_rank(&sm.whole[grp][0][row][0], owner);
+#pragma unroll
+                    for (int x = 0; x < PER; x++) {
+                        atomicAdd(to + o_at(ch + x), o[x].x);
+                        atomicAdd(to + 16 * OROW + o_at(ch + x), o[x].y);
+                    }
+                    meet(2);
+                    if (owner == rank) {
+#pragma unroll
+                        for (int x = 0; x < PER; x++) {
+                            const int at = o_at(ch + x);
+                            o[x] = make_int2(sm.whole[grp][0][row][at], sm.whole[grp][1][row][at]);
+                            sm.whole[grp][0][row][at] = sm.whole[grp][1][row][at] = 0;
+                        }
+                    }
+                    met++;
+                }
+                if (row < rows && (C == 1 || row % C == rank)) {
+                    const int x = 16 * tile + row;
+                    int8_t* to = a.out + ((size_t)s.first_row + x / G) * a.out_stride + (size_t)(kv * G + x % G) * HD + ch;
+#pragma unroll
+                    for (int i = 0; i < PER; i++) to[i] = (int8_t)output_of(o[i], a.rule.om, a.rule.os, fsc, omsc, fast);
+                }
+                __syncwarp();
+            }
+            if (grp >= tiles) {
+                // No tile for this group: the copies are not needed, but each is waited for, so that the
+                // arrivals count for this head.
+                mbar_wait(&sm.k_full, phase, err, 55);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.k_empty);
+                mbar_wait(&sm.v_full, phase, err, 56);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.v_empty);
+            }
+        }
+    }
+    __syncwarp();
+    if (C > 1) cl.sync();  // no block leaves while another writes to it
+}
+
+// The clusters of C blocks of a kernel that the current device holds at once.
+int max_clusters(const void* kernel, int C, int threads, size_t smem) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)C);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)C;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) cudaGetLastError();
+    return n;
+}
+
+// By GROUPS - 1 and log2 C, the resident clusters (found when a device is opened; the GPUs of a host are alike).
+int g_bulk_clusters[2][4];
+
+template <int GROUPS, bool NARROW, bool SSHI>
+cudaError_t launch_bulk(const TreeArgs& a, int C, int num_sms, int* err, cudaStream_t st) {
+    const int works = (int)a.n_seq * a.n_kv;
+    int lg = 0;
+    while (1 << lg < C) lg++;
+    const int fit = C == 1 ? num_sms : g_bulk_clusters[GROUPS - 1][lg], clusters = fit > 0 ? fit : 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)((works < clusters ? works : clusters) * C));
+    cfg.blockDim = dim3(BTHREADS);
+    cfg.dynamicSmemBytes = bulk_smem<GROUPS>(C);
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)C;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_tree_attention_bulk<GROUPS, NARROW, SSHI>, a, works, err);
+}
+
+template <int GROUPS>
+cudaError_t launch_bulk_rule(const TreeArgs& a, int num_sms, int* err, cudaStream_t st) {
+    int C = 1;
+    while (C * BK < a.max_keys) C *= 2;
+    const int rule = score_rule(a.rule, 64);
+    if (rule == 2) return launch_bulk<GROUPS, true, true>(a, C, num_sms, err, st);
+    if (rule == 1) return launch_bulk<GROUPS, true, false>(a, C, num_sms, err, st);
+    return launch_bulk<GROUPS, false, false>(a, C, num_sms, err, st);
+}
+
+template <int GROUPS>
+cudaError_t configure_bulk() {
+    const void* fns[3] = {(const void*)k_tree_attention_bulk<GROUPS, true, true>,
+                          (const void*)k_tree_attention_bulk<GROUPS, true, false>,
+                          (const void*)k_tree_attention_bulk<GROUPS, false, false>};
+    for (const void* f : fns) {
+        const cudaError_t e =
+            cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bulk_smem<GROUPS>(TMAXC));
+        if (e != cudaSuccess) return e;
+    }
+    for (int lg = 1; lg < 4; lg++) {
+        int n = 1 << 30;
+        for (const void* f : fns) n = std::min(n, max_clusters(f, 1 << lg, BTHREADS, bulk_smem<GROUPS>(1 << lg)));
+        g_bulk_clusters[GROUPS - 1][lg] = n;
+    }
+    return cudaSuccess;
+}
+
 }  // namespace
 
 cudaError_t launch_tree_attention(const TreeArgs& a, int num_sms, int* err, cudaStream_t st) {
     if (a.n_seq == 0 || a.max_count == 0) return cudaSuccess;
     const bool vec = a.cache.vec && reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride % 16 == 0 &&
                      a.rule.tlen <= ATTN_TABLE_MAX;
+    if (vec && a.cache.hd == 64 && a.max_keys > TW * 64)
+        return a.max_count * (a.n_head / a.n_kv) > 16 ? launch_bulk_rule<2>(a, num_sms, err, st)
+                                                      : launch_bulk_rule<1>(a, num_sms, err, st);
     if (vec && a.cache.hd == 64) return launch_tree_width<64>(a, num_sms, err, st);
     if (vec && a.cache.hd == 128) return launch_tree_width<128>(a, num_sms, err, st);
     const size_t smem = 4 * (size_t)a.max_keys + (size_t)a.cache.hd;
@@ -663,10 +1172,11 @@ cudaError_t launch_tree_attention(const TreeArgs& a, int num_sms, int* err, cuda
 cudaError_t configure_draft_kernels() {
     cudaError_t e = configure_tree<64, 4>();
     if (e == cudaSuccess) e = configure_tree<64, 8>();
-    if (e == cudaSuccess) e = configure_tree<64, 16>();
     if (e == cudaSuccess) e = configure_tree<128, 4>();
     if (e == cudaSuccess) e = configure_tree<128, 8>();
     if (e == cudaSuccess) e = configure_tree<128, 16>();
+    if (e == cudaSuccess) e = configure_bulk<1>();
+    if (e == cudaSuccess) e = configure_bulk<2>();
     if (e == cudaSuccess) e = configure_beam();
     if (e != cudaSuccess) return e;
     return cudaFuncSetAttribute((const void*)k_tree_attention_any, cudaFuncAttributeMaxDynamicSharedMemorySize,
