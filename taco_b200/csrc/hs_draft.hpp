@@ -30,7 +30,14 @@ struct AttnRuleView {
     int32_t sm, om;
     int ss, os, P, tlen;
     const int32_t* table;  // padded to 4 entries
+    int reach;             // the entries from table[reach - 1] on are equal (table_reach)
 };
+
+// The least length that gives every look-up of table[min(d, n - 1)].
+inline int table_reach(const int32_t* table, int n) {
+    while (n > 1 && table[n - 2] == table[n - 1]) n--;
+    return n;
+}
 
 // hs_tree_seq on the device.
 struct TreeSeq {

@@ -191,7 +191,8 @@ int hs_attn_rule_new(hs_dev* dev, int32_t score_m, uint32_t score_s, int32_t out
             cudaFree(r->table);
             return cuda_fail("cudaMemcpy", e);
         }
-        r->view = AttnRuleView{score_m, out_m, (int)score_s, (int)out_s, (int)softmax_p, (int)table_len, r->table};
+        r->view = AttnRuleView{score_m, out_m, (int)score_s, (int)out_s, (int)softmax_p, (int)table_len, r->table,
+                               table_reach(exp_table, (int)table_len)};
         *out = r.release();
         return HS_OK;
     });

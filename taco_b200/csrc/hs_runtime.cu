@@ -181,7 +181,7 @@ struct hs_model {
     std::vector<std::unique_ptr<DevLinear>> lins;  // 4 per layer (qkv, proj, fc, mlp), then the LM head
     LnDev lnf{};
     int32_t* attn_exp = nullptr;
-    int attn_len = 0;
+    int attn_len = 0, attn_reach = 0;  // (AttnRuleView::reach)
     uint64_t* logits_exp = nullptr;
     uint32_t* logits_high = nullptr;  // their upper 32 bits (BeamArgs::high)
     int logits_len = 0;
@@ -536,7 +536,8 @@ int forward(hs_batch* b, int R) {
             ProfScope p(b, OP_ATTN, attn_ops);
             TreeArgs t{};
             t.cache = cache_of(b);
-            t.rule = AttnRuleView{Ld.score_m, Ld.out_m, Ld.score_s, Ld.out_s, c.softmax_p, m->attn_len, m->attn_exp};
+            t.rule = AttnRuleView{Ld.score_m, Ld.out_m, Ld.score_s, Ld.out_s, c.softmax_p, m->attn_len, m->attn_exp,
+                                  m->attn_reach};
             t.q = b->qkv;
             t.out = b->att;
             t.q_stride = (uint64_t)c.QKVp;
@@ -1993,6 +1994,7 @@ int hs_model_load(hs_dev* dev, const uint8_t* file, size_t len, hs_model** out) 
         if ((rc = upload(&m->attn_exp, t.data(), t.size(), m->owned))) return rc;
     }
     m->attn_len = (int)M.attn_exp.size();
+    m->attn_reach = table_reach(M.attn_exp.data(), m->attn_len);
     if ((rc = upload(&m->logits_exp, M.logits_exp.data(), M.logits_exp.size(), m->owned))) return rc;
     m->logits_len = (int)M.logits_exp.size();
     while (m->logits_head + 1 < m->logits_len && M.logits_exp[m->logits_head + 1] == M.logits_exp[0]) m->logits_head++;

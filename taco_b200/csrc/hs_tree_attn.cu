@@ -207,6 +207,182 @@ __device__ __forceinline__ int32_t output_of(int2 o, int32_t om, int os, float f
     return rescale_clamp127((int64_t)o.x * 256 + o.y, om, os, omsc);
 }
 
+// The row extremes of a warp's dots, for rows g and g + 8 of lane (g, t): score() rises with the dot, or falls
+// if the multiplier is negative. No key seen: INT32_MIN, or INT32_MAX.
+template <int NT>
+__device__ __forceinline__ void tree_extremes(const int32_t (&c)[NT][4], bool whole, const uint32_t (&seen)[2], int32_t m,
+                                              int32_t (&ext)[2]) {
+    auto scan = [&](auto better, int32_t none) {
+        ext[0] = ext[1] = none;
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                ext[0] = better(ext[0], better(c[i][0], c[i][1]));
+                ext[1] = better(ext[1], better(c[i][2], c[i][3]));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    if ((seen[x >> 1] >> (2 * i + (x & 1))) & 1) ext[x >> 1] = better(ext[x >> 1], c[i][x]);
+        }
+#pragma unroll
+        for (int o = 1; o <= 2; o <<= 1)
+#pragma unroll
+            for (int r = 0; r < 2; r++) ext[r] = better(ext[r], __shfl_xor_sync(0xffffffffu, ext[r], o));
+    };
+    if (m >= 0) scan([](int32_t x, int32_t y) { return max(x, y); }, INT32_MIN);
+    else scan([](int32_t x, int32_t y) { return min(x, y); }, INT32_MAX);
+}
+
+// sum + e on the multiply-add pipe (the other integer pipe bounds these kernels).
+__device__ __forceinline__ uint64_t add_wide(uint64_t sum, uint32_t e) {
+    uint64_t r;
+    asm("mad.wide.u32 %0, %1, 1, %2;" : "=l"(r) : "r"(e), "l"(sum));
+    return r;
+}
+
+// The dots become weights e = table[min(M - score, last)] (0 for keys not seen), summed over the quad's keys.
+// ext: the extremes of the whole rows (lane l has row l % 16). The narrow rules take the distance in one
+// multiply-add: M - floor((dot m + h) / 2^ss) = floor((M 2^ss + 2^ss - 1 - h - dot m) / 2^ss), all below 2^54
+// (M 2^ss is within 2^ss of some dot m); a distance is never negative for a key that is seen, and the unsigned
+// minimum keeps the index inside the table for the others.
+template <int NT, bool NARROW, bool SSHI>
+__device__ __forceinline__ void tree_weigh(int32_t (&c)[NT][4], bool whole, const uint32_t (&seen)[2], int32_t ext,
+                                           int32_t m, int ss, const int32_t* table, int last, uint64_t (&sum)[2]) {
+    const int g = (threadIdx.x & 31) >> 2;
+    const bool none = ext == (m >= 0 ? INT32_MIN : INT32_MAX);
+    int64_t mine;
+    if constexpr (NARROW) {
+        const int64_t half = 1LL << (ss - 1), top = none ? 0 : ((int64_t)ext * m + half) >> ss;
+        mine = top * (1LL << ss) + ((1LL << ss) - 1 - half);
+    } else {
+        mine = none ? 0 : tree_score(ext, m, ss);
+    }
+    const int64_t top[2] = {__shfl_sync(0xffffffffu, mine, g), __shfl_sync(0xffffffffu, mine, g + 8)};
+    sum[0] = sum[1] = 0;
+    auto weigh = [&](auto all) {
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                uint32_t d;
+                if constexpr (NARROW) {
+                    const int64_t p = (int64_t)c[i][x] * (int64_t)(-m) + top[x >> 1];
+                    int32_t y;
+                    if constexpr (SSHI) y = (int32_t)(p >> 32) >> (ss - 32);
+                    else y = (int32_t)__funnelshift_r((uint32_t)p, (uint32_t)((uint64_t)p >> 32), ss);
+                    d = min((uint32_t)y, (uint32_t)last);
+                } else {
+                    const int64_t dd = top[x >> 1] - tree_score(c[i][x], m, ss);
+                    d = (uint64_t)dd < (uint64_t)last ? (uint32_t)dd : (uint32_t)last;
+                }
+                uint32_t e = (uint32_t)table[d];
+                if constexpr (!decltype(all)::value)
+                    if (((seen[x >> 1] >> (2 * i + (x & 1))) & 1) == 0) e = 0;
+                c[i][x] = (int32_t)e;
+                sum[x >> 1] = add_wide(sum[x >> 1], e);
+            }
+    };
+    if (whole) weigh(std::true_type{});
+    else weigh(std::false_type{});
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1)
+#pragma unroll
+        for (int r = 0; r < 2; r++) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], o);
+}
+
+// The weights become probabilities p = floor(e 2^P / z) (an exact multiply-shift), as byte planes in the
+// fragments of the second product: c[4 s + plane] the four A words of plane `plane` for the 32 keys of step s.
+// z: the sums of the whole rows (lane l has row l % 16).
+template <int NT>
+__device__ __forceinline__ void tree_planes(int32_t (&c)[NT][4], uint64_t z, int P) {
+    const int g = (threadIdx.x & 31) >> 2;
+    if (z == 0) z = 1;
+    int l = 64 - __clzll((long long)(z - 1));  // z <= 2^l
+    if (l < 1) l = 1;
+    const uint64_t mg = ceil_pow2_div_near(31 + P + l, z);
+    uint32_t mh[2], ml[2];
+    int shift[2];
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        mh[r] = __shfl_sync(0xffffffffu, (uint32_t)(mg >> 32), g + 8 * r);
+        ml[r] = __shfl_sync(0xffffffffu, (uint32_t)mg, g + 8 * r);
+        shift[r] = __shfl_sync(0xffffffffu, l - 1, g + 8 * r);
+    }
+#pragma unroll
+    for (int i = 0; i < NT; i += 4) {
+        uint32_t pl[4][4];
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                uint32_t p[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t e = (uint32_t)c[i + 2 * h + (k >> 1)][2 * r + (k & 1)];
+                    const uint64_t u = (uint64_t)e * mh[r] + __umulhi(e, ml[r]);
+                    p[k] = (uint32_t)(u >> shift[r]);
+                }
+                const uint32_t x0 = __byte_perm(p[0], p[1], 0x5140), x1 = __byte_perm(p[0], p[1], 0x7362);
+                const uint32_t y0 = __byte_perm(p[2], p[3], 0x5140), y1 = __byte_perm(p[2], p[3], 0x7362);
+                pl[0][2 * h + r] = __byte_perm(x0, y0, 0x5410);
+                pl[1][2 * h + r] = __byte_perm(x0, y0, 0x7632);
+                pl[2][2 * h + r] = __byte_perm(x1, y1, 0x5410);
+                pl[3][2 * h + r] = __byte_perm(x1, y1, 0x7632);
+            }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) c[i + k][x] = (int32_t)pl[k][x];
+    }
+}
+
+// O of 8 channels and this warp's keys: the planes times the values v (this thread's keys of channel g), joined
+// to sum (p >> 8) v and sum (p & 255) v: x.x, x.y of channel 2 t and x.z, x.w of 2 t + 1, rows g and g + 8.
+template <int NT>
+__device__ __forceinline__ void tree_multiply(const int32_t (&c)[NT][4], const uint32_t (&v)[NT / 2], int4 (&x)[2]) {
+    int32_t o[4][4];
+#pragma unroll
+    for (int st = 0; st < NT / 4; st++)
+#pragma unroll
+        for (int pl = 0; pl < 4; pl++) {
+            const uint32_t A[4] = {(uint32_t)c[4 * st + pl][0], (uint32_t)c[4 * st + pl][1], (uint32_t)c[4 * st + pl][2],
+                                   (uint32_t)c[4 * st + pl][3]};
+            if (st == 0) mma_u8s8_first(o[pl], A, v[0], v[1]);
+            else mma_u8s8(o[pl], A, v[2 * st], v[2 * st + 1]);
+        }
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        x[r].x = o[1][2 * r] + (o[2][2 * r] + o[3][2 * r] * 256) * 256;
+        x[r].y = o[0][2 * r];
+        x[r].z = o[1][2 * r + 1] + (o[2][2 * r + 1] + o[3][2 * r + 1] * 256) * 256;
+        x[r].w = o[0][2 * r + 1];
+    }
+}
+
+// N outputs (1, 2 or 4 channels from `ch` on) of row x of a tree's kv head, in one store where they are aligned.
+template <int N>
+__device__ __forceinline__ void tree_put(const TreeArgs& a, const TreeSeq& s, int kv, int G, int x, int hd, int ch,
+                                         const int2 (&o)[N], float fsc, double omsc, bool fast) {
+    int8_t* to = a.out + ((size_t)s.first_row + x / G) * a.out_stride + (size_t)(kv * G + x % G) * hd + ch;
+    uint32_t y[N], word = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        y[i] = (uint32_t)output_of(o[i], a.rule.om, a.rule.os, fsc, omsc, fast) & 0xFFu;
+        word |= y[i] << (8 * i);
+    }
+    if (reinterpret_cast<uintptr_t>(to) % N == 0) {
+        if constexpr (N == 4) *reinterpret_cast<uint32_t*>(to) = word;
+        else if constexpr (N == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)word;
+        else *to = (int8_t)word;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) to[i] = (int8_t)y[i];
+    }
+}
+
 // O of a row and channel in two whole numbers, sum (p >> 8) v and sum (p & 255) v: with sum p <= 2^30 and
 // |v| <= 128 the first is at most 2^29 in magnitude over all keys, the second at most 8192 * 2^15 = 2^28.
 struct TreeSmem {
@@ -239,7 +415,6 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
     const int32_t m = a.rule.sm;
     const int ss = a.rule.ss, last = a.rule.tlen - 1, G = a.n_head / a.n_kv;
-    const int64_t half = ss >= 1 && ss <= 62 ? 1LL << (ss - 1) : 0;  // the narrow rule
     const double omsc = (double)a.rule.om * exp2_neg(a.rule.os);
     const float fsc = (float)omsc;
     const bool fast = a.rule.os <= 95 && fabs(omsc) <= 1.9073486328125e-6;
@@ -355,30 +530,8 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
                     seen[r] = x < rows ? seen_word(a.mask + at * a.mask_words, k0 + t * TK, prefix, (int)s.count) : 0;
                 }
             }
-            // The row extremes of the dots: score() rises with the dot, or falls if the multiplier is negative.
             int32_t ext[2];
-            auto scan = [&](auto better, int32_t none) {
-                ext[0] = ext[1] = none;
-                if (whole) {
-#pragma unroll
-                    for (int i = 0; i < NT; i++) {
-                        ext[0] = better(ext[0], better(c[i][0], c[i][1]));
-                        ext[1] = better(ext[1], better(c[i][2], c[i][3]));
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < NT; i++)
-#pragma unroll
-                        for (int x = 0; x < 4; x++)
-                            if ((seen[x >> 1] >> (2 * i + (x & 1))) & 1) ext[x >> 1] = better(ext[x >> 1], c[i][x]);
-                }
-#pragma unroll
-                for (int o = 1; o <= 2; o <<= 1)
-#pragma unroll
-                    for (int r = 0; r < 2; r++) ext[r] = better(ext[r], __shfl_xor_sync(0xffffffffu, ext[r], o));
-            };
-            if (m >= 0) scan([](int32_t x, int32_t y) { return max(x, y); }, INT32_MIN);
-            else scan([](int32_t x, int32_t y) { return min(x, y); }, INT32_MAX);
+            tree_extremes<NT>(c, whole, seen, m, ext);
             // Lane t of a quad gives it to the blocks t, t + 4.
             for (int b = t; b < C; b += 4) {
                 int32_t* to = C > 1 ? cl.map_shared_rank(&wmax[slice][0], b) : wmax[slice];
@@ -388,58 +541,12 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
         }
         meet();
         if (item + stride < items) ask(next, (item + stride) / tiles % a.n_kv, (item + stride) % tiles, true);
-        uint32_t mh[2] = {}, ml[2] = {};
-        int shift[2] = {};
         if (on) {
-            // Lane l has row l % 16: its maximum's score, for the lanes of the row.
+            // Lane l has row l % 16.
             int32_t e = m >= 0 ? INT32_MIN : INT32_MAX;
-            const int32_t none = e;
             for (int i = 0; i < slices; i++) e = m >= 0 ? max(e, wmax[i][lane & 15]) : min(e, wmax[i][lane & 15]);
-            const int64_t mine = e == none ? 0 : NARROW ? ((int64_t)e * m + half) >> ss : tree_score(e, m, ss);
-            int64_t top[2];
-            if constexpr (NARROW) {
-                top[0] = __shfl_sync(0xffffffffu, (int32_t)mine, g);
-                top[1] = __shfl_sync(0xffffffffu, (int32_t)mine, g + 8);
-            } else {
-                top[0] = __shfl_sync(0xffffffffu, mine, g);
-                top[1] = __shfl_sync(0xffffffffu, mine, g + 8);
-            }
-            // The weights and their sums.
-            uint64_t sum[2] = {0, 0};
-            auto weigh = [&](auto all) {
-#pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    uint32_t both[2] = {0, 0};  // two weights, below 2^32 together
-#pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        int32_t d;
-                        if constexpr (NARROW) {
-                            const int64_t p = (int64_t)c[i][x] * (int64_t)m + half;
-                            int32_t y;
-                            if constexpr (SSHI) y = (int32_t)(p >> 32) >> (ss - 32);
-                            else y = (int32_t)__funnelshift_r((uint32_t)p, (uint32_t)((uint64_t)p >> 32), ss);
-                            d = (int32_t)top[x >> 1] - y;
-                            d = (uint32_t)d < (uint32_t)last ? d : last;
-                        } else {
-                            const int64_t dd = top[x >> 1] - tree_score(c[i][x], m, ss);
-                            d = (int32_t)((uint64_t)dd < (uint64_t)last ? dd : (int64_t)last);
-                        }
-                        uint32_t e = (uint32_t)sT[d];
-                        if constexpr (!decltype(all)::value)
-                            if (((seen[x >> 1] >> (2 * i + (x & 1))) & 1) == 0) e = 0;
-                        c[i][x] = (int32_t)e;
-                        both[x >> 1] += e;
-                    }
-                    sum[0] += both[0];
-                    sum[1] += both[1];
-                }
-            };
-            if (whole) weigh(std::true_type{});
-            else weigh(std::false_type{});
-#pragma unroll
-            for (int o = 1; o <= 2; o <<= 1)
-#pragma unroll
-                for (int r = 0; r < 2; r++) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], o);
+            uint64_t sum[2];
+            tree_weigh<NT, NARROW, SSHI>(c, whole, seen, e, m, ss, sT, last, sum);
             for (int b = t; b < C; b += 4) {
                 uint64_t* to = C > 1 ? cl.map_shared_rank(&sm.wsum[slice][0], b) : sm.wsum[slice];
                 to[g] = sum[0];
@@ -475,53 +582,13 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
             load_v(0, v[0]);
             uint64_t z = 0;
             for (int i = 0; i < slices; i++) z += sm.wsum[i][lane & 15];
-            if (z == 0) z = 1;
-            int l = 64 - __clzll((long long)(z - 1));  // z <= 2^l
-            if (l < 1) l = 1;
-            const uint64_t mg = ceil_pow2_div_near(31 + a.rule.P + l, z);
-#pragma unroll
-            for (int r = 0; r < 2; r++) {
-                mh[r] = __shfl_sync(0xffffffffu, (uint32_t)(mg >> 32), g + 8 * r);
-                ml[r] = __shfl_sync(0xffffffffu, (uint32_t)mg, g + 8 * r);
-                shift[r] = __shfl_sync(0xffffffffu, l - 1, g + 8 * r);
-            }
-            // The probabilities as byte planes, in the fragments of the second product: c[4 s + plane]
-            // becomes the four A words of plane `plane` for the 32 keys of step s.
-#pragma unroll
-            for (int i = 0; i < NT; i += 4) {
-                uint32_t pl[4][4];
-#pragma unroll
-                for (int r = 0; r < 2; r++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        uint32_t p[4];
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const uint32_t e = (uint32_t)c[i + 2 * h + (k >> 1)][2 * r + (k & 1)];
-                            const uint64_t u = (uint64_t)e * mh[r] + __umulhi(e, ml[r]);
-                            p[k] = (uint32_t)(u >> shift[r]);
-                        }
-                        const uint32_t x0 = __byte_perm(p[0], p[1], 0x5140), x1 = __byte_perm(p[0], p[1], 0x7362);
-                        const uint32_t y0 = __byte_perm(p[2], p[3], 0x5140), y1 = __byte_perm(p[2], p[3], 0x7362);
-                        pl[0][2 * h + r] = __byte_perm(x0, y0, 0x5410);
-                        pl[1][2 * h + r] = __byte_perm(x0, y0, 0x7632);
-                        pl[2][2 * h + r] = __byte_perm(x1, y1, 0x5410);
-                        pl[3][2 * h + r] = __byte_perm(x1, y1, 0x7632);
-                    }
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-#pragma unroll
-                    for (int x = 0; x < 4; x++) c[i + k][x] = (int32_t)pl[k][x];
-            }
+            tree_planes<NT>(c, z, a.rule.P);
         }
         // O, CH channels at a time: each warp its keys' part, then the sum over the warps.
         const int row = tid / (CH / 4), ch = tid % (CH / 4) * 4;
         int2 acc[HD / CH][4] = {};
         auto put = [&](int r, int at, const int2 (&o)[4]) {
-            const size_t node = (size_t)s.first_row + (16 * tile + r) / G;
-            int8_t* to = a.out + node * a.out_stride + (size_t)(kv * G + (16 * tile + r) % G) * HD + at;
-#pragma unroll
-            for (int x = 0; x < 4; x++) to[x] = (int8_t)output_of(o[x], a.rule.om, a.rule.os, fsc, omsc, fast);
+            tree_put<4>(a, s, kv, G, 16 * tile + r, HD, at, o, fsc, omsc, fast);
         };
 #pragma unroll
         for (int ch0 = 0; ch0 < HD; ch0 += CH) {
@@ -530,25 +597,11 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
                 for (int j = 0; j < CH / 8; j++) {
                     // The next 8 channels' values while these are multiplied.
                     if (ch0 + 8 * j + 8 < HD) load_v(ch0 + 8 * j + 8, v[(j + 1) & 1]);
-                    int32_t o[4][4];
+                    int4 x[2];
+                    tree_multiply<NT>(c, v[j & 1], x);
 #pragma unroll
-                    for (int st = 0; st < NT / 4; st++)
-#pragma unroll
-                        for (int pl = 0; pl < 4; pl++) {
-                            const uint32_t A[4] = {(uint32_t)c[4 * st + pl][0], (uint32_t)c[4 * st + pl][1],
-                                                   (uint32_t)c[4 * st + pl][2], (uint32_t)c[4 * st + pl][3]};
-                            if (st == 0) mma_u8s8_first(o[pl], A, v[j & 1][0], v[j & 1][1]);
-                            else mma_u8s8(o[pl], A, v[j & 1][2 * st], v[j & 1][2 * st + 1]);
-                        }
-#pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        int4 x;
-                        x.x = o[1][2 * r] + (o[2][2 * r] + o[3][2 * r] * 256) * 256;
-                        x.y = o[0][2 * r];
-                        x.z = o[1][2 * r + 1] + (o[2][2 * r + 1] + o[3][2 * r + 1] * 256) * 256;
-                        x.w = o[0][2 * r + 1];
-                        *reinterpret_cast<int4*>(&sm.part[w][g + 8 * r][part_at(g, 8 * j + 2 * t)]) = x;
-                    }
+                    for (int r = 0; r < 2; r++)
+                        *reinterpret_cast<int4*>(&sm.part[w][g + 8 * r][part_at(g, 8 * j + 2 * t)]) = x[r];
                 }
             }
             __syncthreads();
@@ -618,7 +671,7 @@ cudaError_t launch_tree_mma(const TreeArgs& a, int C, int num_sms, int* err, cud
 // score reaches the clamp; 2 narrow with a shift of at least 32.
 int score_rule(const AttnRuleView& r, int hd) {
     const uint64_t m = (uint64_t)(r.sm < 0 ? -(int64_t)r.sm : (int64_t)r.sm);
-    const bool narrow = r.ss >= 1 && r.ss <= 62 && ((m * ((uint64_t)hd << 14)) >> r.ss) + 1 < (1ull << 30);
+    const bool narrow = r.ss >= 1 && r.ss <= 62 && r.sm != INT32_MIN && ((m * ((uint64_t)hd << 14)) >> r.ss) + 1 < (1ull << 30);
     return narrow ? r.ss >= 32 ? 2 : 1 : 0;
 }
 
@@ -634,12 +687,10 @@ template <int HD>
 cudaError_t launch_tree_width(const TreeArgs& a, int num_sms, int* err, cudaStream_t st) {
     // Short contexts: smaller slices, so that all the warps of a block have keys.
     if (a.max_keys <= TW * 32) return launch_tree_rule<HD, 4>(a, 1, num_sms, err, st);
-    if (HD == 64 || a.max_keys <= TW * 64) return launch_tree_rule<HD, 8>(a, 1, num_sms, err, st);
-    if constexpr (HD > 64) {
-        int C = 1;
-        while (C * TW * 128 < a.max_keys) C *= 2;
-        return launch_tree_rule<HD, 16>(a, C, num_sms, err, st);
-    }
+    if (a.max_keys <= TW * 64) return launch_tree_rule<HD, 8>(a, 1, num_sms, err, st);
+    int C = 1;
+    while (C * TW * 128 < a.max_keys) C *= 2;
+    return launch_tree_rule<HD, 16>(a, C, num_sms, err, st);
 }
 
 template <int HD, int NT>
@@ -656,42 +707,40 @@ cudaError_t configure_tree() {
 
 // ---- head width 64: keys and values by bulk copies ----
 //
-// The mathematics and the fragments of the kernel above, with the operands ahead of the work: a producer
-// warp copies the keys (up to 1,024 rows) and the transposed values of a tree's kv head into shared memory,
-// the next head's keys while this one's probabilities are made and its values multiplied, the next values
-// while this one's scores are made. One block per SM, 16 warps for the rows:
+// The mathematics and the fragments of the kernel above, with the operands ahead of the work: bulk copies
+// bring the keys (up to 1,024 rows) and the transposed values of a tree's kv head into shared memory. The
+// last warp that has made its scores of a head asks for the next head's keys, the last that has multiplied
+// asks for its values; no warp waits to copy. One block per SM, 16 warps:
 //   GROUPS = 2: two groups of 8 warps take the 16-row tiles of the head in turn, 128 keys a warp. The
 //     groups meet only within themselves, so one multiplies while the other weighs.
 //   GROUPS = 1: 16 warps share the only tile, 64 keys a warp.
 // Contexts over 1,024 keys take a cluster, a block for each 1,024 keys; the row maxima and sums go to every
 // block's shared memory, the blocks' O to the block that owns the row, with an mbarrier of the group for
-// each meeting.
-// The warps of a group add their O into shared memory with integer atomics (whole numbers: no order).
+// each meeting. The exponent table is held up to its last change (table_reach); a table that leaves no room
+// for the rest takes the kernel above.
 
 constexpr int BK = 1024;                 // keys of a block
-constexpr int BWARPS = 16;               // warps for the rows; one more copies
-constexpr int BTHREADS = 32 * (BWARPS + 1);
+constexpr int BWARPS = 16;
+constexpr int BTHREADS = 32 * BWARPS;
 constexpr int VROW = BK + 16;            // bytes of a channel's values (padded: two rows in a quarter warp's banks)
-constexpr int OROW = 68;                 // words of a row of O: even channels, then odd ones, all banks a store
 
-template <int GROUPS>
 struct __align__(16) TreeBulk {
     uint8_t k[BK * 64];
     uint8_t v[64 * VROW];
-    int32_t table[ATTN_TABLE_MAX];
-    int32_t o[GROUPS][2][16][OROW];      // this block's O
-    int32_t whole[GROUPS][2][16][OROW];  // of the rows that this block owns, over the cluster
-    uint64_t k_full, k_empty, v_full, v_empty;
-    uint64_t met[GROUPS][3];             // the meetings of a cluster's groups: maxima, sums, O
+    uint64_t k_full, v_full;
+    uint32_t k_done, v_done;             // warps that need this head's keys (values) no more
+    uint64_t met[2][4];                  // of a cluster's groups: maxima, sums, O (three meetings)
 };
-// (behind it per group: wsum [slices][16] u64 and wmax [slices][16] i32, slices = C * warps of a group)
-template <int GROUPS>
-constexpr size_t bulk_smem(int C) {
-    return sizeof(TreeBulk<GROUPS>) + (size_t)GROUPS * C * (BWARPS / GROUPS) * 16 * 12;
+// Behind it: the warps' O [BWARPS][16][channels] pairs (32 channels at a time, 16 in clusters, for room), the
+// groups' wsum [slices][16] u64 and wmax [slices][16] i32 (slices: the warps of the group in the cluster), in
+// clusters the owned rows' O [groups][16][64] pairs, and the table.
+__host__ __device__ constexpr int bulk_channels(bool cluster) { return cluster ? 16 : 32; }
+constexpr size_t bulk_smem(int C, int reach) {
+    return sizeof(TreeBulk) + (size_t)BWARPS * 16 * bulk_channels(C > 1) * 8 + (size_t)BWARPS * C * 16 * 12 +
+           (C > 1 ? 2 * 16 * 64 * 8 : 0) + 4 * (((size_t)reach + 3) & ~(size_t)3);
 }
-static_assert(bulk_smem<2>(8) <= 227 * 1024 && bulk_smem<1>(8) <= 227 * 1024, "a block's shared memory");
-
-__device__ __forceinline__ int o_at(int ch) { return (ch & 1) * 32 + (ch >> 1); }
+constexpr size_t BLOCK_SMEM = 227 * 1024;
+static_assert(bulk_smem(1, 7800) <= BLOCK_SMEM && bulk_smem(8, 6200) <= BLOCK_SMEM, "room for the usual tables");
 
 // Arrives on the mbarrier at the same place of block `rank` of the cluster, after this thread's writes.
 __device__ __forceinline__ void mbar_arrive_cluster(uint64_t* bar, int rank) {
@@ -719,369 +768,269 @@ __device__ __forceinline__ void mbar_wait_cluster(uint64_t* bar, uint32_t phase,
 
 // A wait that gives up sets the error word and lets its thread go on: every barrier still gets its arrivals,
 // every later wait returns at once, and the call's results count for nothing.
-template <int GROUPS, bool NARROW, bool SSHI>
+template <int GROUPS, bool CLUSTER, bool NARROW, bool SSHI>
 __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __grid_constant__ TreeArgs a, int works,
                                                                      int* err) {
     constexpr int HD = 64, WPG = BWARPS / GROUPS, NT = BK / WPG / 8, S = 8 * NT, TK = 2 * NT, VB = TK / 4;
-    constexpr int GTHREADS = 32 * WPG, PER = 16 * HD / GTHREADS;  // outputs of a thread
+    constexpr int GTHREADS = 32 * WPG, CC = bulk_channels(CLUSTER), PER = 16 * CC < GTHREADS ? 1 : 16 * CC / GTHREADS;
     extern __shared__ __align__(128) uint8_t s_bulk[];
-    TreeBulk<GROUPS>& sm = *reinterpret_cast<TreeBulk<GROUPS>*>(s_bulk);
+    TreeBulk& sm = *reinterpret_cast<TreeBulk*>(s_bulk);
     cg::cluster_group cl = cg::this_cluster();
-    const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    const int C = CLUSTER ? (int)cl.num_blocks() : 1, rank = CLUSTER ? (int)cl.block_rank() : 0;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int grp = warp / WPG, w = warp % WPG, gtid = tid - grp * GTHREADS, g = lane >> 2, t = lane & 3;
     const int G = a.n_head / a.n_kv, first = blockIdx.x / C, stride = gridDim.x / C;
+    int2(*parts)[16][CC] = reinterpret_cast<int2(*)[16][CC]>(&sm + 1);
+    uint64_t(*wsums)[16] = reinterpret_cast<uint64_t(*)[16]>(parts + BWARPS);
+    int32_t(*wmaxs)[16] = reinterpret_cast<int32_t(*)[16]>(wsums + BWARPS * C);
+    int2(*owns)[16][HD] = reinterpret_cast<int2(*)[16][HD]>(wmaxs + BWARPS * C);
+    int32_t* table = reinterpret_cast<int32_t*>(owns + (CLUSTER ? 2 : 0));
+    const int slice = rank * WPG + w;
+    int2(*part)[16][CC] = parts + grp * WPG;
+    uint64_t(*wsum)[16] = wsums + grp * C * WPG;
+    int32_t(*wmax)[16] = wmaxs + grp * C * WPG;
+    int2(*own)[HD] = owns[CLUSTER ? grp : 0];
+    const int32_t m = a.rule.sm;
+    const int ss = a.rule.ss, last = a.rule.reach - 1;
+    const double omsc = (double)a.rule.om * exp2_neg(a.rule.os);
+    const float fsc = (float)omsc;
+    const bool fast = a.rule.os <= 95 && fabs(omsc) <= 1.9073486328125e-6;
     if (tid == 0) {
         mbar_init(&sm.k_full, 1);
-        mbar_init(&sm.k_empty, BWARPS);
         mbar_init(&sm.v_full, 1);
-        mbar_init(&sm.v_empty, BWARPS);
+        sm.k_done = sm.v_done = 0;
         for (int i = 0; i < GROUPS; i++)
             for (int k = 0; k < 3; k++) mbar_init(&sm.met[i][k], WPG * C);
         fence_barrier_init();
     }
-    for (int i = tid; i < GROUPS * 2 * 16 * OROW; i += BTHREADS) {
-        (&sm.o[0][0][0][0])[i] = 0;
-        (&sm.whole[0][0][0][0])[i] = 0;
-    }
-    for (int i = tid; i < (a.rule.tlen + 3) / 4; i += BTHREADS)
-        reinterpret_cast<int4*>(sm.table)[i] = reinterpret_cast<const int4*>(a.rule.table)[i];
-    if (C > 1) cl.sync();
+    if (CLUSTER)
+        for (int i = tid; i < 2 * 16 * HD; i += BTHREADS) (&owns[0][0][0])[i] = make_int2(0, 0);
+    for (int i = tid; i < (a.rule.reach + 3) / 4; i += BTHREADS)
+        reinterpret_cast<int4*>(table)[i] = reinterpret_cast<const int4*>(a.rule.table)[i];
+    if (CLUSTER) cl.sync();
     else __syncthreads();
 
-    if (warp == BWARPS) {
-        // The producer.
-        uint32_t count = 0;  // works copied
-        for (int work = first; work < works; work += stride) {
+    // The copies of the keys (values) of the first work from `work` on that has rows, by one warp.
+    auto copy = [&](int work, bool values) {
+        for (; work < works; work += stride) {
             const TreeSeq s = a.seqs[work / a.n_kv];
-            if (!tree_seq_ok(s, a.n_rows, a.cache.slots, a.max_count, a.max_keys)) {
-                if (lane == 0) atomicCAS(err, 0, ERR_DRAFT_SEQ);
-                continue;
-            }
-            if (s.count == 0) continue;
+            if (!tree_seq_ok(s, a.n_rows, a.cache.slots, a.max_count, a.max_keys) || s.count == 0) continue;
             const int n = (int)(s.prefix + s.count), k0 = rank * BK, kn = max(0, min(BK, n - k0));
             const size_t plane = (size_t)s.slot * a.cache.slot_stride +
                                  (size_t)(a.plane0 + work % a.n_kv) * ((size_t)a.cache.n_ctx * HD);
-            const uint32_t phase = (count & 1) ^ 1, vbytes = (uint32_t)(kn + 15) & ~15u;  // (n_ctx % 16 == 0)
-            if (!mbar_wait(&sm.k_empty, phase, err, 50)) break;
-            if (lane == 0) {
+            if (values) {
+                const uint32_t bytes = (uint32_t)(kn + 15) & ~15u;  // (n_ctx % 16 == 0)
+                if (lane == 0) mbar_arrive_expect_tx(&sm.v_full, bytes * HD);
+                __syncwarp();
+                if (kn)
+                    for (int ch = lane; ch < HD; ch += 32)
+                        bulk_load(sm.v + ch * VROW, a.cache.v + plane + (size_t)ch * a.cache.n_ctx + k0, bytes, &sm.v_full);
+            } else if (lane == 0) {
                 mbar_arrive_expect_tx(&sm.k_full, (uint32_t)kn * HD);
                 if (kn) bulk_load(sm.k, a.cache.k + plane + (size_t)k0 * HD, (uint32_t)kn * HD, &sm.k_full);
             }
-            if (!mbar_wait(&sm.v_empty, phase, err, 51)) break;
-            if (lane == 0) mbar_arrive_expect_tx(&sm.v_full, vbytes * HD);
-            __syncwarp();
-            if (kn)
-                for (int ch = lane; ch < HD; ch += 32)
-                    bulk_load(sm.v + ch * VROW, a.cache.v + plane + (size_t)ch * a.cache.n_ctx + k0, vbytes, &sm.v_full);
-            count++;
+            break;
         }
-    } else {
-        const int grp = warp / WPG, w = warp % WPG, gtid = tid - grp * GTHREADS;
-        const int g = lane >> 2, t = lane & 3;
-        const int slice = rank * WPG + w;
-        uint64_t(*wsum)[16] = reinterpret_cast<uint64_t(*)[16]>(s_bulk + sizeof(TreeBulk<GROUPS>)) + grp * C * WPG;
-        int32_t(*wmax)[16] = reinterpret_cast<int32_t(*)[16]>(
-            reinterpret_cast<uint64_t(*)[16]>(s_bulk + sizeof(TreeBulk<GROUPS>)) + GROUPS * C * WPG) + grp * C * WPG;
-        const int32_t m = a.rule.sm;
-        const int ss = a.rule.ss, last = a.rule.tlen - 1;
-        const int64_t half = ss >= 1 && ss <= 62 ? 1LL << (ss - 1) : 0;  // the narrow rule
-        const double omsc = (double)a.rule.om * exp2_neg(a.rule.os);
-        const float fsc = (float)omsc;
-        const bool fast = a.rule.os <= 95 && fabs(omsc) <= 1.9073486328125e-6;
-        uint32_t met = 0;  // rounds of the group's meetings
-        // The group's warps, of all blocks of the cluster, at meeting k of this round.
-        auto meet = [&](int k) {
-            if (C > 1) {
-                __syncwarp();
-                if (lane < C) mbar_arrive_cluster(&sm.met[grp][k], lane);
-                mbar_wait_cluster(&sm.met[grp][k], met & 1, err, 52 + k);
-                __syncwarp();
-            } else {
-                __syncwarp();
-                named_bar(1 + grp, GTHREADS);
+    };
+    if (warp == 0) copy(first, false);
+    if (warp == 1) copy(first, true);
+    // This warp has read the keys (values) of `work`: the last one asks for the next.
+    auto done = [&](int work, bool values) {
+        __syncwarp();
+        uint32_t before = 0;
+        if (lane == 0) {
+            __threadfence_block();
+            before = atomicAdd(values ? &sm.v_done : &sm.k_done, 1u);
+            if (before == BWARPS - 1) *(volatile uint32_t*)(values ? &sm.v_done : &sm.k_done) = 0;
+        }
+        if (__shfl_sync(0xffffffffu, before, 0) == BWARPS - 1) {
+            __threadfence_block();
+            fence_async_smem();  // the warps' reads before the copies' writes
+            copy(work + stride, values);
+        }
+        __syncwarp();
+    };
+    auto group_bar = [&]() {
+        __syncwarp();
+        named_bar(1 + grp, GTHREADS);
+    };
+    // The group's warps, of all blocks of the cluster, at meeting k of this round.
+    uint32_t round = 0;
+    auto meet = [&](int k) {
+        if (CLUSTER) {
+            __syncwarp();
+            if (lane < C) mbar_arrive_cluster(&sm.met[grp][k], lane);
+            mbar_wait_cluster(&sm.met[grp][k], round & 1, err, 52 + k);
+            __syncwarp();
+        } else {
+            group_bar();
+        }
+    };
+    uint32_t count = 0;
+    for (int work = first; work < works; work += stride) {
+        const TreeSeq s = a.seqs[work / a.n_kv];
+        if (!tree_seq_ok(s, a.n_rows, a.cache.slots, a.max_count, a.max_keys)) {
+            if (tid == 0) atomicCAS(err, 0, ERR_DRAFT_SEQ);
+            continue;
+        }
+        if (s.count == 0) continue;
+        const int kv = work % a.n_kv, prefix = (int)s.prefix, n = prefix + (int)s.count;
+        const int total = (int)s.count * G, tiles = (total + 15) / 16, slices = (n + S - 1) / S;
+        const int live = CLUSTER ? min(max(slices - rank * WPG, 0), WPG) : slices;  // this block's warps with keys
+        const bool on = slice < slices;
+        const int k0 = slice * S;  // of the context; the block's copy starts at rank * BK
+        const uint32_t phase = count & 1;
+        count++;
+        const uint8_t* ks = sm.k + (size_t)(w * S) * HD;
+        const uint8_t* vs = sm.v + w * S + t * TK;
+        // The rows of a tile: their fragments and what they see of this thread's keys (slices inside the
+        // context are whole for every row), loaded a tile ahead.
+        const bool whole = k0 + S <= prefix;
+        uint32_t q[2][4], seen[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+        auto load_rows = [&](int tile) {
+            if (!on) return;
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int x = 16 * tile + g + 8 * r;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (x < total)
+                    v = reinterpret_cast<const uint4*>(a.q + ((size_t)s.first_row + x / G) * a.q_stride +
+                                                       (size_t)(kv * G + x % G) * HD)[t];
+                q[0][r] = v.x;
+                q[0][2 + r] = v.y;
+                q[1][r] = v.z;
+                q[1][2 + r] = v.w;
+                if (!whole)
+                    seen[r] = x < total ? seen_word(a.mask + ((size_t)s.first_row + x / G) * a.mask_words, k0 + t * TK,
+                                                    prefix, (int)s.count)
+                                        : 0;
             }
         };
-        uint32_t count = 0;
-        for (int work = first; work < works; work += stride) {
-            const TreeSeq s = a.seqs[work / a.n_kv];
-            if (!tree_seq_ok(s, a.n_rows, a.cache.slots, a.max_count, a.max_keys) || s.count == 0) continue;
-            const int kv = work % a.n_kv, prefix = (int)s.prefix, n = prefix + (int)s.count;
-            const int total = (int)s.count * G, tiles = (total + 15) / 16, slices = (n + S - 1) / S;
-            const bool on = slice < slices;
-            const int k0 = slice * S;  // of the context; the block's copy starts at rank * BK
-            const uint32_t phase = count & 1;
-            count++;
-            const uint8_t* ks = sm.k + (size_t)(w * S) * HD;
-            const uint8_t* vs = sm.v + w * S + t * TK;
-            for (int tile = grp; tile < tiles; tile += GROUPS) {
-                const int rows = total - 16 * tile;
-                int32_t c[NT][4];
-                uint32_t seen[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
-                bool whole = true;
-                if (on) {
-                    uint32_t q[2][4];
+        load_rows(grp);
+        for (int tile = grp; tile < tiles; tile += GROUPS) {
+            const int rows = total - 16 * tile;
+            int32_t c[NT][4];
+            if (tile == grp) mbar_wait(&sm.k_full, phase, err, 55);
+            if (on) {
+                const uint4* kp = reinterpret_cast<const uint4*>(ks + ((g >> 1) * TK + (g & 1)) * HD) + t;
 #pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        const int x = 16 * tile + g + 8 * r;
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (x < total)
-                            v = reinterpret_cast<const uint4*>(a.q + ((size_t)s.first_row + x / G) * a.q_stride +
-                                                               (size_t)(kv * G + x % G) * HD)[t];
-                        q[0][r] = v.x;
-                        q[0][2 + r] = v.y;
-                        q[1][r] = v.z;
-                        q[1][2 + r] = v.w;
-                    }
-                    // Slices inside the context are whole for every row.
-                    if (k0 + S > prefix) {
-                        whole = false;
-#pragma unroll
-                        for (int r = 0; r < 2; r++) {
-                            const int x = 16 * tile + g + 8 * r;
-                            seen[r] = x < total ? seen_word(a.mask + ((size_t)s.first_row + x / G) * a.mask_words,
-                                                            k0 + t * TK, prefix, (int)s.count)
-                                                : 0;
-                        }
-                    }
-                    if (tile == grp) mbar_wait(&sm.k_full, phase, err, 55);
-                    const uint4* kp = reinterpret_cast<const uint4*>(ks + ((g >> 1) * TK + (g & 1)) * HD) + t;
-#pragma unroll
-                    for (int i = 0; i < NT; i++) {
-                        const uint4 kw = kp[2 * i * (HD / 16)];
-                        mma_s8s8_first(c[i], q[0], kw.x, kw.y);
-                        mma_s8s8(c[i], q[1], kw.z, kw.w);
-                    }
-                } else if (tile == grp) {
-                    mbar_wait(&sm.k_full, phase, err, 55);
+                for (int i = 0; i < NT; i++) {
+                    const uint4 kw = kp[2 * i * (HD / 16)];
+                    mma_s8s8_first(c[i], q[0], kw.x, kw.y);
+                    mma_s8s8(c[i], q[1], kw.z, kw.w);
                 }
-                if (tile + GROUPS >= tiles) {  // the group's last scores of this head
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sm.k_empty);
+                int32_t ext[2];
+                tree_extremes<NT>(c, whole, seen, m, ext);
+                // Lane t of a quad gives them to the blocks t, t + 4.
+                for (int b = t; b < C; b += 4) {
+                    int32_t* to = CLUSTER ? cl.map_shared_rank(&wmax[slice][0], b) : wmax[slice];
+                    to[g] = ext[0];
+                    to[g + 8] = ext[1];
                 }
-                if (on) {
-                    // The row extremes of the dots: score() rises with the dot, or falls if the multiplier is
-                    // negative.
-                    int32_t ext[2];
-                    auto scan = [&](auto better, int32_t none) {
-                        ext[0] = ext[1] = none;
-                        if (whole) {
-#pragma unroll
-                            for (int i = 0; i < NT; i++) {
-                                ext[0] = better(ext[0], better(c[i][0], c[i][1]));
-                                ext[1] = better(ext[1], better(c[i][2], c[i][3]));
-                            }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < NT; i++)
-#pragma unroll
-                                for (int x = 0; x < 4; x++)
-                                    if ((seen[x >> 1] >> (2 * i + (x & 1))) & 1) ext[x >> 1] = better(ext[x >> 1], c[i][x]);
-                        }
-#pragma unroll
-                        for (int o = 1; o <= 2; o <<= 1)
-#pragma unroll
-                            for (int r = 0; r < 2; r++) ext[r] = better(ext[r], __shfl_xor_sync(0xffffffffu, ext[r], o));
-                    };
-                    if (m >= 0) scan([](int32_t x, int32_t y) { return max(x, y); }, INT32_MIN);
-                    else scan([](int32_t x, int32_t y) { return min(x, y); }, INT32_MAX);
-                    // Lane t of a quad gives them to the blocks t, t + 4.
-                    for (int b = t; b < C; b += 4) {
-                        int32_t* to = C > 1 ? cl.map_shared_rank(&wmax[slice][0], b) : wmax[slice];
-                        to[g] = ext[0];
-                        to[g + 8] = ext[1];
-                    }
+            }
+            if (tile + GROUPS >= tiles) done(work, false);  // the group's last scores of this head
+            meet(0);
+            if (on) {
+                // Lane l has row l % 16.
+                int32_t e = m >= 0 ? INT32_MIN : INT32_MAX;
+                for (int i = 0; i < slices; i++) e = m >= 0 ? max(e, wmax[i][lane & 15]) : min(e, wmax[i][lane & 15]);
+                uint64_t sum[2];
+                tree_weigh<NT, NARROW, SSHI>(c, whole, seen, e, m, ss, table, last, sum);
+                for (int b = t; b < C; b += 4) {
+                    uint64_t* to = CLUSTER ? cl.map_shared_rank(&wsum[slice][0], b) : wsum[slice];
+                    to[g] = sum[0];
+                    to[g + 8] = sum[1];
                 }
-                meet(0);
+            }
+            meet(1);
+            if (tile + GROUPS < tiles) load_rows(tile + GROUPS);
+            if (on) {
+                uint64_t z = 0;
+                for (int i = 0; i < slices; i++) z += wsum[i][lane & 15];
+                tree_planes<NT>(c, z, a.rule.P);
+            }
+            if (tile == grp) mbar_wait(&sm.v_full, phase, err, 56);
+            // O, CC channels at a time: each warp its keys' part, then the sum over the warps, PER channels of
+            // a row a thread. (Odd rows' channels are 8 pairs off, so that the two rows of a quarter warp's
+            // stores take all the banks.)
+            const int row = gtid / (CC / PER), ch = gtid % (CC / PER) * PER;
+            const bool sums = row < 16;  // (a group of 512 threads has more than it needs)
+#pragma unroll 1
+            for (int ch0 = 0; ch0 < HD; ch0 += CC) {
                 if (on) {
-                    // Lane l has row l % 16: its maximum's score, for the lanes of the row.
-                    const int32_t none = m >= 0 ? INT32_MIN : INT32_MAX;
-                    int32_t e = none;
-                    for (int i = 0; i < slices; i++) e = m >= 0 ? max(e, wmax[i][lane & 15]) : min(e, wmax[i][lane & 15]);
-                    const int64_t mine = e == none ? 0 : NARROW ? ((int64_t)e * m + half) >> ss : tree_score(e, m, ss);
-                    int64_t top[2];
-                    if constexpr (NARROW) {
-                        top[0] = __shfl_sync(0xffffffffu, (int32_t)mine, g);
-                        top[1] = __shfl_sync(0xffffffffu, (int32_t)mine, g + 8);
-                    } else {
-                        top[0] = __shfl_sync(0xffffffffu, mine, g);
-                        top[1] = __shfl_sync(0xffffffffu, mine, g + 8);
-                    }
-                    // The weights and their sums.
-                    uint64_t sum[2] = {0, 0};
-                    auto weigh = [&](auto all) {
 #pragma unroll
-                        for (int i = 0; i < NT; i++) {
-                            uint32_t both[2] = {0, 0};  // two weights, below 2^32 together
-#pragma unroll
-                            for (int x = 0; x < 4; x++) {
-                                int32_t d;
-                                if constexpr (NARROW) {
-                                    const int64_t p = (int64_t)c[i][x] * (int64_t)m + half;
-                                    int32_t y;
-                                    if constexpr (SSHI) y = (int32_t)(p >> 32) >> (ss - 32);
-                                    else y = (int32_t)__funnelshift_r((uint32_t)p, (uint32_t)((uint64_t)p >> 32), ss);
-                                    d = (int32_t)top[x >> 1] - y;
-                                    d = (uint32_t)d < (uint32_t)last ? d : last;
-                                } else {
-                                    const int64_t dd = top[x >> 1] - tree_score(c[i][x], m, ss);
-                                    d = (int32_t)((uint64_t)dd < (uint64_t)last ? dd : (int64_t)last);
-                                }
-                                uint32_t e = (uint32_t)sm.table[d];
-                                if constexpr (!decltype(all)::value)
-                                    if (((seen[x >> 1] >> (2 * i + (x & 1))) & 1) == 0) e = 0;
-                                c[i][x] = (int32_t)e;
-                                both[x >> 1] += e;
-                            }
-                            sum[0] += both[0];
-                            sum[1] += both[1];
-                        }
-                    };
-                    if (whole) weigh(std::true_type{});
-                    else weigh(std::false_type{});
-#pragma unroll
-                    for (int o = 1; o <= 2; o <<= 1)
-#pragma unroll
-                        for (int r = 0; r < 2; r++) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], o);
-                    for (int b = t; b < C; b += 4) {
-                        uint64_t* to = C > 1 ? cl.map_shared_rank(&wsum[slice][0], b) : wsum[slice];
-                        to[g] = sum[0];
-                        to[g + 8] = sum[1];
-                    }
-                }
-                meet(1);
-                if (on) {
-                    uint64_t z = 0;
-                    for (int i = 0; i < slices; i++) z += wsum[i][lane & 15];
-                    if (z == 0) z = 1;
-                    int l = 64 - __clzll((long long)(z - 1));  // z <= 2^l
-                    if (l < 1) l = 1;
-                    const uint64_t mg = ceil_pow2_div_near(31 + a.rule.P + l, z);
-                    uint32_t mh[2], ml[2];
-                    int shift[2];
-#pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        mh[r] = __shfl_sync(0xffffffffu, (uint32_t)(mg >> 32), g + 8 * r);
-                        ml[r] = __shfl_sync(0xffffffffu, (uint32_t)mg, g + 8 * r);
-                        shift[r] = __shfl_sync(0xffffffffu, l - 1, g + 8 * r);
-                    }
-                    // The probabilities as byte planes, in the fragments of the second product: c[4 s + plane]
-                    // becomes the four A words of plane `plane` for the 32 keys of step s.
-#pragma unroll
-                    for (int i = 0; i < NT; i += 4) {
-                        uint32_t pl[4][4];
-#pragma unroll
-                        for (int r = 0; r < 2; r++)
-#pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                uint32_t p[4];
-#pragma unroll
-                                for (int k = 0; k < 4; k++) {
-                                    const uint32_t e = (uint32_t)c[i + 2 * h + (k >> 1)][2 * r + (k & 1)];
-                                    const uint64_t u = (uint64_t)e * mh[r] + __umulhi(e, ml[r]);
-                                    p[k] = (uint32_t)(u >> shift[r]);
-                                }
-                                const uint32_t x0 = __byte_perm(p[0], p[1], 0x5140), x1 = __byte_perm(p[0], p[1], 0x7362);
-                                const uint32_t y0 = __byte_perm(p[2], p[3], 0x5140), y1 = __byte_perm(p[2], p[3], 0x7362);
-                                pl[0][2 * h + r] = __byte_perm(x0, y0, 0x5410);
-                                pl[1][2 * h + r] = __byte_perm(x0, y0, 0x7632);
-                                pl[2][2 * h + r] = __byte_perm(x1, y1, 0x5410);
-                                pl[3][2 * h + r] = __byte_perm(x1, y1, 0x7632);
-                            }
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-#pragma unroll
-                            for (int x = 0; x < 4; x++) c[i + k][x] = (int32_t)pl[k][x];
-                    }
-                    if (tile == grp) mbar_wait(&sm.v_full, phase, err, 56);
-                    // O of this warp's keys, added to the group's, 8 channels at a time.
-#pragma unroll 2
-                    for (int j = 0; j < HD / 8; j++) {
+                    for (int j = 0; j < CC / 8; j++) {
                         uint32_t v[VB];
 #pragma unroll
                         for (int b = 0; b < TK / 16; b++) {
-                            const uint4 x = *reinterpret_cast<const uint4*>(vs + (8 * j + g) * VROW + 16 * b);
+                            const uint4 x = *reinterpret_cast<const uint4*>(vs + (ch0 + 8 * j + g) * VROW + 16 * b);
                             v[4 * b] = x.x;
                             v[4 * b + 1] = x.y;
                             v[4 * b + 2] = x.z;
                             v[4 * b + 3] = x.w;
                         }
-                        int32_t o[4][4];
+                        int4 x[2];
+                        tree_multiply<NT>(c, v, x);
 #pragma unroll
-                        for (int st = 0; st < NT / 4; st++)
-#pragma unroll
-                            for (int pl = 0; pl < 4; pl++) {
-                                const uint32_t A[4] = {(uint32_t)c[4 * st + pl][0], (uint32_t)c[4 * st + pl][1],
-                                                       (uint32_t)c[4 * st + pl][2], (uint32_t)c[4 * st + pl][3]};
-                                if (st == 0) mma_u8s8_first(o[pl], A, v[0], v[1]);
-                                else mma_u8s8(o[pl], A, v[2 * st], v[2 * st + 1]);
-                            }
-#pragma unroll
-                        for (int x = 0; x < 4; x++) {
-                            const int row = g + 8 * (x >> 1), at = o_at(8 * j + 2 * t + (x & 1));
-                            atomicAdd(&sm.o[grp][0][row][at], o[1][x] + (o[2][x] + o[3][x] * 256) * 256);
-                            atomicAdd(&sm.o[grp][1][row][at], o[0][x]);
-                        }
+                        for (int r = 0; r < 2; r++)
+                            *reinterpret_cast<int4*>(&part[w][g + 8 * r][part_at(g, 8 * j + 2 * t)]) = x[r];
                     }
-                } else if (tile == grp) {
-                    mbar_wait(&sm.v_full, phase, err, 56);
                 }
-                if (tile + GROUPS >= tiles) {  // the group's last product of this head
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sm.v_empty);
-                }
-                __syncwarp();
-                named_bar(1 + grp, GTHREADS);
-                // PER channels of a row a thread (at each of two parities, PER / 2 words).
-                const int row = gtid / (HD / PER), ch = gtid % (HD / PER) * PER;
+                if (ch0 + CC == HD && tile + GROUPS >= tiles) done(work, true);  // the last product of this head
+                group_bar();
                 int2 o[PER];
 #pragma unroll
-                for (int x = 0; x < PER; x++) {
-                    const int at = o_at(ch + x);
-                    o[x] = make_int2(sm.o[grp][0][row][at], sm.o[grp][1][row][at]);
-                    sm.o[grp][0][row][at] = sm.o[grp][1][row][at] = 0;  // for the next tile
-                }
-                if (C > 1) {
-                    // The row's sums to the block that owns it.
-                    const int owner = row % C;
-                    int32_t* to = cl.map_shared_rank(&sm.whole[grp][0][row][0], owner);
+                for (int x = 0; x < PER; x++) o[x] = make_int2(0, 0);
+                for (int i = 0; i < live && sums; i++)
 #pragma unroll
                     for (int x = 0; x < PER; x++) {
-                        atomicAdd(to + o_at(ch + x), o[x].x);
-                        atomicAdd(to + 16 * OROW + o_at(ch + x), o[x].y);
+                        const int2 y = part[i][row][part_at(row, ch + x)];
+                        o[x].x += y.x;
+                        o[x].y += y.y;
                     }
-                    meet(2);
-                    if (owner == rank) {
+                if constexpr (CLUSTER) {
+                    // To the block that owns the row.
+                    if (live > 0 && sums) {
+                        int2* to = cl.map_shared_rank(&own[row][ch0 + ch], row % C);
 #pragma unroll
                         for (int x = 0; x < PER; x++) {
-                            const int at = o_at(ch + x);
-                            o[x] = make_int2(sm.whole[grp][0][row][at], sm.whole[grp][1][row][at]);
-                            sm.whole[grp][0][row][at] = sm.whole[grp][1][row][at] = 0;
+                            atomicAdd(&to[x].x, o[x].x);
+                            atomicAdd(&to[x].y, o[x].y);
                         }
                     }
-                    met++;
+                } else if (row < rows) {
+                    tree_put<PER>(a, s, kv, G, 16 * tile + row, HD, ch0 + ch, o, fsc, omsc, fast);
                 }
-                if (row < rows && (C == 1 || row % C == rank)) {
-                    const int x = 16 * tile + row;
-                    int8_t* to = a.out + ((size_t)s.first_row + x / G) * a.out_stride + (size_t)(kv * G + x % G) * HD + ch;
+                if (ch0 + CC < HD) group_bar();  // the parts are read
+            }
+            if (CLUSTER) {
+                meet(2);
+                round++;
+                for (int i = gtid; i < 16 * HD / 4; i += GTHREADS) {
+                    const int r = i / (HD / 4), c4 = i % (HD / 4) * 4;
+                    if (r % C != rank) continue;
+                    int2 o[4];
 #pragma unroll
-                    for (int i = 0; i < PER; i++) to[i] = (int8_t)output_of(o[i], a.rule.om, a.rule.os, fsc, omsc, fast);
+                    for (int x = 0; x < 4; x++) {
+                        o[x] = own[r][c4 + x];
+                        own[r][c4 + x] = make_int2(0, 0);  // for the next tile
+                    }
+                    if (r < rows) tree_put<4>(a, s, kv, G, 16 * tile + r, HD, c4, o, fsc, omsc, fast);
                 }
                 __syncwarp();
             }
-            if (grp >= tiles) {
-                // No tile for this group: the copies are not needed, but each is waited for, so that the
-                // arrivals count for this head.
-                mbar_wait(&sm.k_full, phase, err, 55);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.k_empty);
-                mbar_wait(&sm.v_full, phase, err, 56);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.v_empty);
-            }
+        }
+        if (grp >= tiles) {
+            // No tile for this group: the copies are not needed, but each is waited for, so that the counts are
+            // this head's.
+            mbar_wait(&sm.k_full, phase, err, 55);
+            done(work, false);
+            mbar_wait(&sm.v_full, phase, err, 56);
+            done(work, true);
         }
     }
     __syncwarp();
-    if (C > 1) cl.sync();  // no block leaves while another writes to it
+    if (CLUSTER) cl.sync();  // no block leaves while another writes to it
 }
 
 // The clusters of C blocks of a kernel that the current device holds at once.
@@ -1104,7 +1053,7 @@ int max_clusters(const void* kernel, int C, int threads, size_t smem) {
 // By GROUPS - 1 and log2 C, the resident clusters (found when a device is opened; the GPUs of a host are alike).
 int g_bulk_clusters[2][4];
 
-template <int GROUPS, bool NARROW, bool SSHI>
+template <int GROUPS, bool CLUSTER, bool NARROW, bool SSHI>
 cudaError_t launch_bulk(const TreeArgs& a, int C, int num_sms, int* err, cudaStream_t st) {
     const int works = (int)a.n_seq * a.n_kv;
     int lg = 0;
@@ -1113,7 +1062,7 @@ cudaError_t launch_bulk(const TreeArgs& a, int C, int num_sms, int* err, cudaStr
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)((works < clusters ? works : clusters) * C));
     cfg.blockDim = dim3(BTHREADS);
-    cfg.dynamicSmemBytes = bulk_smem<GROUPS>(C);
+    cfg.dynamicSmemBytes = bulk_smem(C, a.rule.reach);
     cfg.stream = st;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;
@@ -1121,32 +1070,29 @@ cudaError_t launch_bulk(const TreeArgs& a, int C, int num_sms, int* err, cudaStr
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_tree_attention_bulk<GROUPS, NARROW, SSHI>, a, works, err);
+    return cudaLaunchKernelEx(&cfg, k_tree_attention_bulk<GROUPS, CLUSTER, NARROW, SSHI>, a, works, err);
 }
 
-template <int GROUPS>
-cudaError_t launch_bulk_rule(const TreeArgs& a, int num_sms, int* err, cudaStream_t st) {
-    int C = 1;
-    while (C * BK < a.max_keys) C *= 2;
+template <int GROUPS, bool CLUSTER>
+cudaError_t launch_bulk_rule(const TreeArgs& a, int C, int num_sms, int* err, cudaStream_t st) {
     const int rule = score_rule(a.rule, 64);
-    if (rule == 2) return launch_bulk<GROUPS, true, true>(a, C, num_sms, err, st);
-    if (rule == 1) return launch_bulk<GROUPS, true, false>(a, C, num_sms, err, st);
-    return launch_bulk<GROUPS, false, false>(a, C, num_sms, err, st);
+    if (rule == 2) return launch_bulk<GROUPS, CLUSTER, true, true>(a, C, num_sms, err, st);
+    if (rule == 1) return launch_bulk<GROUPS, CLUSTER, true, false>(a, C, num_sms, err, st);
+    return launch_bulk<GROUPS, CLUSTER, false, false>(a, C, num_sms, err, st);
 }
 
-template <int GROUPS>
+template <int GROUPS, bool CLUSTER>
 cudaError_t configure_bulk() {
-    const void* fns[3] = {(const void*)k_tree_attention_bulk<GROUPS, true, true>,
-                          (const void*)k_tree_attention_bulk<GROUPS, true, false>,
-                          (const void*)k_tree_attention_bulk<GROUPS, false, false>};
+    const void* fns[3] = {(const void*)k_tree_attention_bulk<GROUPS, CLUSTER, true, true>,
+                          (const void*)k_tree_attention_bulk<GROUPS, CLUSTER, true, false>,
+                          (const void*)k_tree_attention_bulk<GROUPS, CLUSTER, false, false>};
     for (const void* f : fns) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bulk_smem<GROUPS>(TMAXC));
+        const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BLOCK_SMEM);
         if (e != cudaSuccess) return e;
     }
-    for (int lg = 1; lg < 4; lg++) {
+    for (int lg = 1; CLUSTER && lg < 4; lg++) {
         int n = 1 << 30;
-        for (const void* f : fns) n = std::min(n, max_clusters(f, 1 << lg, BTHREADS, bulk_smem<GROUPS>(1 << lg)));
+        for (const void* f : fns) n = std::min(n, max_clusters(f, 1 << lg, BTHREADS, BLOCK_SMEM));
         g_bulk_clusters[GROUPS - 1][lg] = n;
     }
     return cudaSuccess;
@@ -1158,9 +1104,17 @@ cudaError_t launch_tree_attention(const TreeArgs& a, int num_sms, int* err, cuda
     if (a.n_seq == 0 || a.max_count == 0) return cudaSuccess;
     const bool vec = a.cache.vec && reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride % 16 == 0 &&
                      a.rule.tlen <= ATTN_TABLE_MAX;
-    if (vec && a.cache.hd == 64 && a.max_keys > TW * 64)
-        return a.max_count * (a.n_head / a.n_kv) > 16 ? launch_bulk_rule<2>(a, num_sms, err, st)
-                                                      : launch_bulk_rule<1>(a, num_sms, err, st);
+    if (vec && a.cache.hd == 64 && a.max_keys > TW * 64) {
+        int C = 1;
+        while (C * BK < a.max_keys) C *= 2;
+        if (bulk_smem(C, a.rule.reach) <= BLOCK_SMEM) {
+            const bool tile = a.max_count * (a.n_head / a.n_kv) <= 16;  // one tile a head
+            if (C == 1)
+                return tile ? launch_bulk_rule<1, false>(a, C, num_sms, err, st)
+                            : launch_bulk_rule<2, false>(a, C, num_sms, err, st);
+            return tile ? launch_bulk_rule<1, true>(a, C, num_sms, err, st) : launch_bulk_rule<2, true>(a, C, num_sms, err, st);
+        }
+    }
     if (vec && a.cache.hd == 64) return launch_tree_width<64>(a, num_sms, err, st);
     if (vec && a.cache.hd == 128) return launch_tree_width<128>(a, num_sms, err, st);
     const size_t smem = 4 * (size_t)a.max_keys + (size_t)a.cache.hd;
@@ -1175,8 +1129,11 @@ cudaError_t configure_draft_kernels() {
     if (e == cudaSuccess) e = configure_tree<128, 4>();
     if (e == cudaSuccess) e = configure_tree<128, 8>();
     if (e == cudaSuccess) e = configure_tree<128, 16>();
-    if (e == cudaSuccess) e = configure_bulk<1>();
-    if (e == cudaSuccess) e = configure_bulk<2>();
+    if (e == cudaSuccess) e = configure_tree<64, 16>();
+    if (e == cudaSuccess) e = configure_bulk<1, false>();
+    if (e == cudaSuccess) e = configure_bulk<1, true>();
+    if (e == cudaSuccess) e = configure_bulk<2, false>();
+    if (e == cudaSuccess) e = configure_bulk<2, true>();
     if (e == cudaSuccess) e = configure_beam();
     if (e != cudaSuccess) return e;
     return cudaFuncSetAttribute((const void*)k_tree_attention_any, cudaFuncAttributeMaxDynamicSharedMemorySize,

@@ -207,6 +207,27 @@ def test_tree_of_many_keys_and_sequences(dev):
     check_tree(dev, tree_case(16, counts, [min(int(p), 2048 - c) for p, c in zip(pre, counts)], 2048, heads=12, kv=12))
 
 
+@pytest.mark.parametrize("counts,prefixes,n_ctx", [([40, 9], [900, 20], 1024), ([33], [2000], 2048), ([5], [700], 1024)])
+def test_tree_table_that_changes_to_its_end(dev, counts, prefixes, n_ctx):
+    """8,192 different entries: no shared memory is left for the copies of keys and values."""
+    table = (1 << 30) - 100_000 * np.arange(8192, dtype=np.int64)
+    check_tree(dev, tree_case(54, counts, prefixes, n_ctx), dict(RULE, table=table))
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_tree_random_batches(dev, seed):
+    """Ragged batches of every size of context, with empty trees and heads shared or not."""
+    r = np.random.default_rng(1000 + seed)
+    n_ctx = int(r.choice([512, 1024, 1040, 2048, 4096]))
+    kv, group = int(r.integers(1, 4)), int(r.choice([1, 1, 2, 5]))
+    counts = [int(c) for c in r.integers(0, int(r.choice([5, 17, 60, 129])), 9)]
+    counts[0] = max(counts[0], 1)
+    prefixes = [int(r.integers(0, n_ctx - c + 1)) for c in counts]
+    prefixes[0] = n_ctx - counts[0]
+    check_tree(dev, tree_case(2000 + seed, counts, prefixes, n_ctx, kv * group, kv, gap=int(r.integers(0, 2))),
+               pad=int(r.choice([0, 16])))
+
+
 def test_tree_on_a_side_stream_and_in_a_graph(dev):
     c = tree_case(17, [16, 5], [100, 30], 128)
     st = torch.cuda.Stream()
