@@ -132,10 +132,7 @@ __global__ void __launch_bounds__(ANY_THREADS) k_tree_attention_any(const TreeAr
 // as P and V agree: column c of key tile i is key (c / 2) 2 NT + 2 i + c % 2 of the slice, so that the
 // accumulators of thread t hold its 2 NT consecutive keys, which are the bytes of V^T rows it loads.
 
-constexpr int TW = 8;              // warps of a block
-constexpr int TTHREADS = 32 * TW;
 constexpr int TMAXC = 8;           // blocks of a cluster
-constexpr int CH = 64;             // channels of O that the warps' parts hold at a time
 
 __device__ __forceinline__ void mma_s8s8(int32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -178,6 +175,10 @@ __device__ __forceinline__ uint64_t ceil_pow2_div_near(int sh, uint64_t s) {
     if (R <= -(int64_t)s) x -= 1;
     return x;
 }
+
+// The node and the head of row x of a tree and kv head with G query heads (a division only if they are shared).
+__device__ __forceinline__ int node_of(int x, int G) { return G == 1 ? x : x / G; }
+__device__ __forceinline__ int head_of(int x, int G) { return G == 1 ? 0 : x % G; }
 
 // The bits of the keys first .. first + 31 that a row sees: the context (below `prefix`) and the tree's
 // nodes in the mask words (bits from `count` on are none).
@@ -366,7 +367,7 @@ __device__ __forceinline__ void tree_multiply(const int32_t (&c)[NT][4], const u
 template <int N>
 __device__ __forceinline__ void tree_put(const TreeArgs& a, const TreeSeq& s, int kv, int G, int x, int hd, int ch,
                                          const int2 (&o)[N], float fsc, double omsc, bool fast) {
-    int8_t* to = a.out + ((size_t)s.first_row + x / G) * a.out_stride + (size_t)(kv * G + x % G) * hd + ch;
+    int8_t* to = a.out + ((size_t)s.first_row + node_of(x, G)) * a.out_stride + (size_t)(kv * G + head_of(x, G)) * hd + ch;
     uint32_t y[N], word = 0;
 #pragma unroll
     for (int i = 0; i < N; i++) {
@@ -385,40 +386,39 @@ __device__ __forceinline__ void tree_put(const TreeArgs& a, const TreeSeq& s, in
 
 // O of a row and channel in two whole numbers, sum (p >> 8) v and sum (p & 255) v: with sum p <= 2^30 and
 // |v| <= 128 the first is at most 2^29 in magnitude over all keys, the second at most 8192 * 2^15 = 2^28.
-struct TreeSmem {
-    // O of each warp. The channels of odd rows are 8 pairs off (exclusive or), so that the two rows of a
-    // quarter warp's stores take all the banks.
-    __align__(16) int2 part[TW][16][CH];
-    // By slice of the item, the row maxima and sums (each block of a cluster has all of them).
-    uint64_t wsum[TW * TMAXC][16];
-};
+// Odd rows' channels are 8 pairs off (exclusive or), so that the two rows of a quarter warp's stores of a part
+// take all the banks.
 __device__ __forceinline__ int part_at(int row, int ch) { return ch ^ ((row & 1) << 3); }
 
-// (a single block takes TW slices of wsum, then wmax behind them)
-constexpr size_t tree_smem(int C) {
-    return 4 * ATTN_TABLE_MAX + 8 * TW * 16 * CH + (size_t)TW * C * 16 * 12;
+// Shared memory of W warps in clusters of C blocks: the warps' parts of O [W][16][CH] pairs, then by slice of
+// the item the row sums [W C][16] u64 and maxima [W C][16] i32 (each block of a cluster has all of them), the
+// exponent table up to its last change.
+constexpr size_t tree_smem(int W, int CH, int C, int reach) {
+    return 8 * (size_t)W * 16 * CH + (size_t)W * C * 16 * 12 + 4 * (((size_t)reach + 3) & ~(size_t)3);
 }
 
-template <int HD, int NT, bool NARROW, bool SSHI>
-__global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_constant__ TreeArgs a, int tiles, int items,
-                                                                int* err) {
+template <int HD, int TW, int NT, int CH, bool NARROW, bool SSHI>
+__global__ void __launch_bounds__(32 * TW, 2) k_tree_attention(const __grid_constant__ TreeArgs a, int tiles, int items,
+                                                               int* err) {
+    constexpr int TTHREADS = 32 * TW, PER = 16 * CH / TTHREADS;  // sums of a thread
     constexpr int S = 8 * NT;        // keys of a warp
     constexpr int TK = 2 * NT;       // keys of a thread
     constexpr int KB = HD / 64;      // 16-byte pieces of a key's row per thread
     constexpr int VB = TK / 4;       // words of a channel's values per thread
     extern __shared__ __align__(16) uint8_t s_tree[];
-    int32_t* sT = reinterpret_cast<int32_t*>(s_tree);
-    TreeSmem& sm = *reinterpret_cast<TreeSmem*>(s_tree + 4 * ATTN_TABLE_MAX);
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-    int32_t(*wmax)[16] = reinterpret_cast<int32_t(*)[16]>(&sm.wsum[TW * C]);
+    int2(*part)[16][CH] = reinterpret_cast<int2(*)[16][CH]>(s_tree);
+    uint64_t(*wsum)[16] = reinterpret_cast<uint64_t(*)[16]>(part + TW);
+    int32_t(*wmax)[16] = reinterpret_cast<int32_t(*)[16]>(wsum + TW * C);
+    int32_t* sT = reinterpret_cast<int32_t*>(wmax + TW * C);
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
     const int32_t m = a.rule.sm;
-    const int ss = a.rule.ss, last = a.rule.tlen - 1, G = a.n_head / a.n_kv;
+    const int ss = a.rule.ss, last = a.rule.reach - 1, G = a.n_head / a.n_kv;
     const double omsc = (double)a.rule.om * exp2_neg(a.rule.os);
     const float fsc = (float)omsc;
     const bool fast = a.rule.os <= 95 && fabs(omsc) <= 1.9073486328125e-6;
-    for (int i = tid; i < (a.rule.tlen + 3) / 4; i += TTHREADS)
+    for (int i = tid; i < (a.rule.reach + 3) / 4; i += TTHREADS)
         reinterpret_cast<int4*>(sT)[i] = reinterpret_cast<const int4*>(a.rule.table)[i];
     auto meet = [&]() {  // of all the item's warps
         if (C > 1) cl.sync();
@@ -475,8 +475,8 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
 #pragma unroll
             for (int r = 0; r < 2; r++) {
                 const int x = g + 8 * r;
-                const size_t at = (size_t)s.first_row + (16 * tile + x) / G;
-                const int head = kv * G + (16 * tile + x) % G;
+                const size_t at = (size_t)s.first_row + node_of(16 * tile + x, G);
+                const int head = kv * G + head_of(16 * tile + x, G);
                 const uint4* p = reinterpret_cast<const uint4*>(a.q + at * a.q_stride + (size_t)head * HD) + t;
 #pragma unroll
                 for (int b = 0; b < KB; b++) {
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
                     const int x = g + 8 * r;
-                    const size_t at = (size_t)s.first_row + (16 * tile + x) / G;
+                    const size_t at = (size_t)s.first_row + node_of(16 * tile + x, G);
                     seen[r] = x < rows ? seen_word(a.mask + at * a.mask_words, k0 + t * TK, prefix, (int)s.count) : 0;
                 }
             }
@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
             uint64_t sum[2];
             tree_weigh<NT, NARROW, SSHI>(c, whole, seen, e, m, ss, sT, last, sum);
             for (int b = t; b < C; b += 4) {
-                uint64_t* to = C > 1 ? cl.map_shared_rank(&sm.wsum[slice][0], b) : sm.wsum[slice];
+                uint64_t* to = C > 1 ? cl.map_shared_rank(&wsum[slice][0], b) : wsum[slice];
                 to[g] = sum[0];
                 to[g + 8] = sum[1];
             }
@@ -581,15 +581,12 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
         if (on) {
             load_v(0, v[0]);
             uint64_t z = 0;
-            for (int i = 0; i < slices; i++) z += sm.wsum[i][lane & 15];
+            for (int i = 0; i < slices; i++) z += wsum[i][lane & 15];
             tree_planes<NT>(c, z, a.rule.P);
         }
         // O, CH channels at a time: each warp its keys' part, then the sum over the warps.
-        const int row = tid / (CH / 4), ch = tid % (CH / 4) * 4;
-        int2 acc[HD / CH][4] = {};
-        auto put = [&](int r, int at, const int2 (&o)[4]) {
-            tree_put<4>(a, s, kv, G, 16 * tile + r, HD, at, o, fsc, omsc, fast);
-        };
+        const int row = tid / (CH / PER), ch = tid % (CH / PER) * PER;
+        int2 acc[HD / CH][PER];
 #pragma unroll
         for (int ch0 = 0; ch0 < HD; ch0 += CH) {
             if (on) {
@@ -601,19 +598,19 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
                     tree_multiply<NT>(c, v[j & 1], x);
 #pragma unroll
                     for (int r = 0; r < 2; r++)
-                        *reinterpret_cast<int4*>(&sm.part[w][g + 8 * r][part_at(g, 8 * j + 2 * t)]) = x[r];
+                        *reinterpret_cast<int4*>(&part[w][g + 8 * r][part_at(g, 8 * j + 2 * t)]) = x[r];
                 }
             }
             __syncthreads();
-            // Four channels of a row a thread.
+            int2* sums = acc[ch0 / CH];
+#pragma unroll
+            for (int x = 0; x < PER; x++) sums[x] = make_int2(0, 0);
             for (int i = 0; i < live; i++)
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const int4 y = *reinterpret_cast<const int4*>(&sm.part[i][row][part_at(row, ch + 2 * x)]);
-                    acc[ch0 / CH][2 * x].x += y.x;
-                    acc[ch0 / CH][2 * x].y += y.y;
-                    acc[ch0 / CH][2 * x + 1].x += y.z;
-                    acc[ch0 / CH][2 * x + 1].y += y.w;
+                for (int x = 0; x < PER; x++) {
+                    const int2 y = part[i][row][part_at(row, ch + x)];
+                    sums[x].x += y.x;
+                    sums[x].y += y.y;
                 }
             if (HD > CH) __syncthreads();  // the parts are read
         }
@@ -623,48 +620,50 @@ __global__ void __launch_bounds__(TTHREADS, 2) k_tree_attention(const __grid_con
 #pragma unroll
             for (int h = 0; h < HD / CH; h++)
 #pragma unroll
-                for (int x = 0; x < 4; x++) sm.part[h][row][ch + x] = acc[h][x];
+                for (int x = 0; x < PER; x++) part[h][row][CH == HD ? part_at(row, ch + x) : ch + x] = acc[h][x];
             cl.sync();
-            constexpr int QUADS = HD / 4;
+            constexpr int QUADS = HD / PER;
             for (int i = rank * TTHREADS + tid; i < 16 * QUADS; i += C * TTHREADS) {
-                const int r = i / QUADS, c4 = i % QUADS * 4;
-                int2 sum4[4] = {};
-                for (int b = 0; b < C; b++) {
-                    const int2* of = cl.map_shared_rank(&sm.part[c4 / CH][r][c4 % CH], b);
+                const int r = i / QUADS, at = i % QUADS * PER;
+                int2 sums[PER];
 #pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        sum4[x].x += of[x].x;
-                        sum4[x].y += of[x].y;
+                for (int x = 0; x < PER; x++) sums[x] = make_int2(0, 0);
+                for (int b = 0; b < C; b++) {
+                    const int2* of = cl.map_shared_rank(&part[at / CH][r][0], b);
+#pragma unroll
+                    for (int x = 0; x < PER; x++) {
+                        const int2 y = of[CH == HD ? part_at(r, at + x) : at % CH + x];
+                        sums[x].x += y.x;
+                        sums[x].y += y.y;
                     }
                 }
-                if (r < rows) put(r, c4, sum4);
+                if (r < rows) tree_put<PER>(a, s, kv, G, 16 * tile + r, HD, at, sums, fsc, omsc, fast);
             }
-            cl.sync();  // (the parts are written again after two more meetings; this one is for HD > CH)
+            cl.sync();  // the sums are read
         } else if (row < rows) {
 #pragma unroll
-            for (int h = 0; h < HD / CH; h++) put(row, h * CH + ch, acc[h]);
+            for (int h = 0; h < HD / CH; h++)
+                tree_put<PER>(a, s, kv, G, 16 * tile + row, HD, h * CH + ch, acc[h], fsc, omsc, fast);
         }
     }
     if (C > 1) cl.sync();  // no block leaves while another reads its memory
 }
 
-template <int HD, int NT, bool NARROW, bool SSHI>
-cudaError_t launch_tree_mma(const TreeArgs& a, int C, int num_sms, int* err, cudaStream_t st) {
-    const int G = a.n_head / a.n_kv, tiles = (a.max_count * G + 15) / 16;
-    const int items = (int)a.n_seq * a.n_kv * tiles;
+// The clusters of C blocks of a kernel that the current device holds at once.
+int max_clusters(const void* kernel, int C, int threads, size_t smem) {
     cudaLaunchConfig_t cfg{};
-    const int clusters = 2 * num_sms / C;
-    cfg.gridDim = dim3((unsigned)(items < clusters ? items : clusters) * C);
-    cfg.blockDim = dim3(TTHREADS);
-    cfg.dynamicSmemBytes = tree_smem(C);
-    cfg.stream = st;
+    cfg.gridDim = dim3((unsigned)C);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = C;
+    at.val.clusterDim.x = (unsigned)C;
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_tree_attention<HD, NT, NARROW, SSHI>, a, tiles, items, err);
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) cudaGetLastError();
+    return n;
 }
 
 // Which score rule fits: 0 wide; 1 narrow: every |score| is below 2^30, so distances fit in 32 bits and no
@@ -675,52 +674,75 @@ int score_rule(const AttnRuleView& r, int hd) {
     return narrow ? r.ss >= 32 ? 2 : 1 : 0;
 }
 
-template <int HD, int NT>
-cudaError_t launch_tree_rule(const TreeArgs& a, int C, int num_sms, int* err, cudaStream_t st) {
-    const int rule = score_rule(a.rule, HD);
-    if (rule == 2) return launch_tree_mma<HD, NT, true, true>(a, C, num_sms, err, st);
-    if (rule == 1) return launch_tree_mma<HD, NT, true, false>(a, C, num_sms, err, st);
-    return launch_tree_mma<HD, NT, false, false>(a, C, num_sms, err, st);
-}
+// A kernel's shape, and by log2 C the clusters that a device holds at once (found when a device is opened; the
+// GPUs of a host are alike).
+template <int HD, int TW, int NT, int CH>
+struct TreeShape {
+    static constexpr int KEYS = TW * NT * 8;  // of a block
+    static inline int fit[4] = {0, 0, 0, 0};
 
-template <int HD>
-cudaError_t launch_tree_width(const TreeArgs& a, int num_sms, int* err, cudaStream_t st) {
-    // Short contexts: smaller slices, so that all the warps of a block have keys.
-    if (a.max_keys <= TW * 32) return launch_tree_rule<HD, 4>(a, 1, num_sms, err, st);
-    if (a.max_keys <= TW * 64) return launch_tree_rule<HD, 8>(a, 1, num_sms, err, st);
-    int C = 1;
-    while (C * TW * 128 < a.max_keys) C *= 2;
-    return launch_tree_rule<HD, 16>(a, C, num_sms, err, st);
-}
-
-template <int HD, int NT>
-cudaError_t configure_tree() {
-    const void* fns[3] = {(const void*)k_tree_attention<HD, NT, true, true>,
-                          (const void*)k_tree_attention<HD, NT, true, false>,
-                          (const void*)k_tree_attention<HD, NT, false, false>};
-    for (const void* f : fns) {
-        const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tree_smem(TMAXC));
-        if (e != cudaSuccess) return e;
+    static cudaError_t configure() {
+        const void* fns[3] = {(const void*)k_tree_attention<HD, TW, NT, CH, true, true>,
+                              (const void*)k_tree_attention<HD, TW, NT, CH, true, false>,
+                              (const void*)k_tree_attention<HD, TW, NT, CH, false, false>};
+        for (const void* f : fns) {
+            const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                       (int)tree_smem(TW, CH, TMAXC, ATTN_TABLE_MAX));
+            if (e != cudaSuccess) return e;
+        }
+        for (int lg = 0; lg < 4; lg++) {
+            int n = 1 << 30;
+            for (const void* f : fns)
+                n = std::min(n, max_clusters(f, 1 << lg, 32 * TW, tree_smem(TW, CH, 1 << lg, 6144)));
+            fit[lg] = n;
+        }
+        return cudaSuccess;
     }
-    return cudaSuccess;
-}
+
+    template <bool NARROW, bool SSHI>
+    static cudaError_t go(const TreeArgs& a, int* err, cudaStream_t st) {
+        const int G = a.n_head / a.n_kv, tiles = (a.max_count * G + 15) / 16;
+        const int items = (int)a.n_seq * a.n_kv * tiles;
+        int lg = 0;
+        while (KEYS << lg < a.max_keys) lg++;
+        const int C = 1 << lg, clusters = fit[lg] > 0 ? fit[lg] : 1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)((items < clusters ? items : clusters) * C));
+        cfg.blockDim = dim3(32 * TW);
+        cfg.dynamicSmemBytes = tree_smem(TW, CH, C, a.rule.reach);
+        cfg.stream = st;
+        cudaLaunchAttribute at;
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = C;
+        at.val.clusterDim.y = at.val.clusterDim.z = 1;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, k_tree_attention<HD, TW, NT, CH, NARROW, SSHI>, a, tiles, items, err);
+    }
+
+    static cudaError_t launch(const TreeArgs& a, int* err, cudaStream_t st) {
+        const int rule = score_rule(a.rule, HD);
+        if (rule == 2) return go<true, true>(a, err, st);
+        if (rule == 1) return go<true, false>(a, err, st);
+        return go<false, false>(a, err, st);
+    }
+};
 
 // ---- head width 64: keys and values by bulk copies ----
 //
 // The mathematics and the fragments of the kernel above, with the operands ahead of the work: bulk copies
 // bring the keys (up to 1,024 rows) and the transposed values of a tree's kv head into shared memory. The
 // last warp that has made its scores of a head asks for the next head's keys, the last that has multiplied
-// asks for its values; no warp waits to copy. One block per SM, 16 warps:
-//   GROUPS = 2: two groups of 8 warps take the 16-row tiles of the head in turn, 128 keys a warp. The
-//     groups meet only within themselves, so one multiplies while the other weighs.
-//   GROUPS = 1: 16 warps share the only tile, 64 keys a warp.
+// asks for its values; no warp waits to copy. One block per SM, 16 warps in two groups of 8 that take the
+// 16-row tiles of the head in turn, 128 keys a warp. The groups meet only within themselves, so one multiplies
+// while the other weighs.
 // Contexts over 1,024 keys take a cluster, a block for each 1,024 keys; the row maxima and sums go to every
 // block's shared memory, the blocks' O to the block that owns the row, with an mbarrier of the group for
 // each meeting. The exponent table is held up to its last change (table_reach); a table that leaves no room
 // for the rest takes the kernel above.
 
 constexpr int BK = 1024;                 // keys of a block
-constexpr int BWARPS = 16;
+constexpr int BWARPS = 16, GROUPS = 2;
 constexpr int BTHREADS = 32 * BWARPS;
 constexpr int VROW = BK + 16;            // bytes of a channel's values (padded: two rows in a quarter warp's banks)
 
@@ -729,7 +751,7 @@ struct __align__(16) TreeBulk {
     uint8_t v[64 * VROW];
     uint64_t k_full, v_full;
     uint32_t k_done, v_done;             // warps that need this head's keys (values) no more
-    uint64_t met[2][4];                  // of a cluster's groups: maxima, sums, O (three meetings)
+    uint64_t met[GROUPS][3];             // of a cluster's groups: maxima, sums, O (three meetings)
 };
 // Behind it: the warps' O [BWARPS][16][channels] pairs (32 channels at a time, 16 in clusters, for room), the
 // groups' wsum [slices][16] u64 and wmax [slices][16] i32 (slices: the warps of the group in the cluster), in
@@ -737,7 +759,7 @@ struct __align__(16) TreeBulk {
 __host__ __device__ constexpr int bulk_channels(bool cluster) { return cluster ? 16 : 32; }
 constexpr size_t bulk_smem(int C, int reach) {
     return sizeof(TreeBulk) + (size_t)BWARPS * 16 * bulk_channels(C > 1) * 8 + (size_t)BWARPS * C * 16 * 12 +
-           (C > 1 ? 2 * 16 * 64 * 8 : 0) + 4 * (((size_t)reach + 3) & ~(size_t)3);
+           (C > 1 ? GROUPS * 16 * 64 * 8 : 0) + 4 * (((size_t)reach + 3) & ~(size_t)3);
 }
 constexpr size_t BLOCK_SMEM = 227 * 1024;
 static_assert(bulk_smem(1, 7800) <= BLOCK_SMEM && bulk_smem(8, 6200) <= BLOCK_SMEM, "room for the usual tables");
@@ -768,11 +790,11 @@ __device__ __forceinline__ void mbar_wait_cluster(uint64_t* bar, uint32_t phase,
 
 // A wait that gives up sets the error word and lets its thread go on: every barrier still gets its arrivals,
 // every later wait returns at once, and the call's results count for nothing.
-template <int GROUPS, bool CLUSTER, bool NARROW, bool SSHI>
+template <bool CLUSTER, bool NARROW, bool SSHI>
 __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __grid_constant__ TreeArgs a, int works,
                                                                      int* err) {
     constexpr int HD = 64, WPG = BWARPS / GROUPS, NT = BK / WPG / 8, S = 8 * NT, TK = 2 * NT, VB = TK / 4;
-    constexpr int GTHREADS = 32 * WPG, CC = bulk_channels(CLUSTER), PER = 16 * CC < GTHREADS ? 1 : 16 * CC / GTHREADS;
+    constexpr int GTHREADS = 32 * WPG, CC = bulk_channels(CLUSTER), PER = 16 * CC / GTHREADS;
     extern __shared__ __align__(128) uint8_t s_bulk[];
     TreeBulk& sm = *reinterpret_cast<TreeBulk*>(s_bulk);
     cg::cluster_group cl = cg::this_cluster();
@@ -784,7 +806,7 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
     uint64_t(*wsums)[16] = reinterpret_cast<uint64_t(*)[16]>(parts + BWARPS);
     int32_t(*wmaxs)[16] = reinterpret_cast<int32_t(*)[16]>(wsums + BWARPS * C);
     int2(*owns)[16][HD] = reinterpret_cast<int2(*)[16][HD]>(wmaxs + BWARPS * C);
-    int32_t* table = reinterpret_cast<int32_t*>(owns + (CLUSTER ? 2 : 0));
+    int32_t* table = reinterpret_cast<int32_t*>(owns + (CLUSTER ? GROUPS : 0));
     const int slice = rank * WPG + w;
     int2(*part)[16][CC] = parts + grp * WPG;
     uint64_t(*wsum)[16] = wsums + grp * C * WPG;
@@ -804,7 +826,7 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
         fence_barrier_init();
     }
     if (CLUSTER)
-        for (int i = tid; i < 2 * 16 * HD; i += BTHREADS) (&owns[0][0][0])[i] = make_int2(0, 0);
+        for (int i = tid; i < GROUPS * 16 * HD; i += BTHREADS) (&owns[0][0][0])[i] = make_int2(0, 0);
     for (int i = tid; i < (a.rule.reach + 3) / 4; i += BTHREADS)
         reinterpret_cast<int4*>(table)[i] = reinterpret_cast<const int4*>(a.rule.table)[i];
     if (CLUSTER) cl.sync();
@@ -886,7 +908,8 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
         // The rows of a tile: their fragments and what they see of this thread's keys (slices inside the
         // context are whole for every row), loaded a tile ahead.
         const bool whole = k0 + S <= prefix;
-        uint32_t q[2][4], seen[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+        const int node0 = k0 + t * TK - prefix;  // the node of this thread's first key
+        uint32_t q[2][4], words[2][2] = {};
         auto load_rows = [&](int tile) {
             if (!on) return;
 #pragma unroll
@@ -894,22 +917,42 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
                 const int x = 16 * tile + g + 8 * r;
                 uint4 v = make_uint4(0, 0, 0, 0);
                 if (x < total)
-                    v = reinterpret_cast<const uint4*>(a.q + ((size_t)s.first_row + x / G) * a.q_stride +
-                                                       (size_t)(kv * G + x % G) * HD)[t];
+                    v = reinterpret_cast<const uint4*>(a.q + ((size_t)s.first_row + node_of(x, G)) * a.q_stride +
+                                                       (size_t)(kv * G + head_of(x, G)) * HD)[t];
                 q[0][r] = v.x;
                 q[0][2 + r] = v.y;
                 q[1][r] = v.z;
                 q[1][2 + r] = v.w;
-                if (!whole)
-                    seen[r] = x < total ? seen_word(a.mask + ((size_t)s.first_row + x / G) * a.mask_words, k0 + t * TK,
-                                                    prefix, (int)s.count)
-                                        : 0;
+                if (!whole) {
+                    // The mask words that hold the nodes k0 + t TK - prefix .. + 31 (put together at the tile).
+                    const uint32_t* of = a.mask + ((size_t)s.first_row + node_of(x, G)) * a.mask_words;
+                    words[r][0] = words[r][1] = 0;
+                    if (x < total && node0 > -32) {
+                        if (node0 >= 0 && node0 < (int)s.count) words[r][0] = of[node0 >> 5];
+                        const int up = node0 < 0 ? 0 : (node0 >> 5) + 1;
+                        if (32 * up < (int)s.count) words[r][1] = of[up];
+                    }
+                }
             }
         };
         load_rows(grp);
         for (int tile = grp; tile < tiles; tile += GROUPS) {
             const int rows = total - 16 * tile;
             int32_t c[NT][4];
+            uint32_t seen[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+            if (on && !whole) {
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    // Keys before node 0 are the context's; nodes from `count` on are none.
+                    const uint32_t lo = node0 >= 0 ? words[r][0] : 0xFFFFFFFFu;
+                    const uint32_t bits = __funnelshift_r(lo, words[r][1], node0 & 31);
+                    const int left = (int)s.count - node0;
+                    seen[r] = 16 * tile + g + 8 * r >= total || left <= 0 ? 0u
+                              : node0 <= -32                              ? 0xFFFFFFFFu
+                              : left >= 32                                ? bits
+                                                                          : bits & ((1u << left) - 1u);
+                }
+            }
             if (tile == grp) mbar_wait(&sm.k_full, phase, err, 55);
             if (on) {
                 const uint4* kp = reinterpret_cast<const uint4*>(ks + ((g >> 1) * TK + (g & 1)) * HD) + t;
@@ -954,7 +997,6 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
             // a row a thread. (Odd rows' channels are 8 pairs off, so that the two rows of a quarter warp's
             // stores take all the banks.)
             const int row = gtid / (CC / PER), ch = gtid % (CC / PER) * PER;
-            const bool sums = row < 16;  // (a group of 512 threads has more than it needs)
 #pragma unroll 1
             for (int ch0 = 0; ch0 < HD; ch0 += CC) {
                 if (on) {
@@ -981,7 +1023,7 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
                 int2 o[PER];
 #pragma unroll
                 for (int x = 0; x < PER; x++) o[x] = make_int2(0, 0);
-                for (int i = 0; i < live && sums; i++)
+                for (int i = 0; i < live; i++)
 #pragma unroll
                     for (int x = 0; x < PER; x++) {
                         const int2 y = part[i][row][part_at(row, ch + x)];
@@ -990,7 +1032,7 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
                     }
                 if constexpr (CLUSTER) {
                     // To the block that owns the row.
-                    if (live > 0 && sums) {
+                    if (live > 0) {
                         int2* to = cl.map_shared_rank(&own[row][ch0 + ch], row % C);
 #pragma unroll
                         for (int x = 0; x < PER; x++) {
@@ -1033,32 +1075,15 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
     if (CLUSTER) cl.sync();  // no block leaves while another writes to it
 }
 
-// The clusters of C blocks of a kernel that the current device holds at once.
-int max_clusters(const void* kernel, int C, int threads, size_t smem) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)C);
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)C;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) cudaGetLastError();
-    return n;
-}
+// By log2 C, the resident clusters (found when a device is opened; the GPUs of a host are alike).
+int g_bulk_clusters[4];
 
-// By GROUPS - 1 and log2 C, the resident clusters (found when a device is opened; the GPUs of a host are alike).
-int g_bulk_clusters[2][4];
-
-template <int GROUPS, bool CLUSTER, bool NARROW, bool SSHI>
+template <bool CLUSTER, bool NARROW, bool SSHI>
 cudaError_t launch_bulk(const TreeArgs& a, int C, int num_sms, int* err, cudaStream_t st) {
     const int works = (int)a.n_seq * a.n_kv;
     int lg = 0;
     while (1 << lg < C) lg++;
-    const int fit = C == 1 ? num_sms : g_bulk_clusters[GROUPS - 1][lg], clusters = fit > 0 ? fit : 1;
+    const int fit = C == 1 ? num_sms : g_bulk_clusters[lg], clusters = fit > 0 ? fit : 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)((works < clusters ? works : clusters) * C));
     cfg.blockDim = dim3(BTHREADS);
@@ -1070,22 +1095,22 @@ cudaError_t launch_bulk(const TreeArgs& a, int C, int num_sms, int* err, cudaStr
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_tree_attention_bulk<GROUPS, CLUSTER, NARROW, SSHI>, a, works, err);
+    return cudaLaunchKernelEx(&cfg, k_tree_attention_bulk<CLUSTER, NARROW, SSHI>, a, works, err);
 }
 
-template <int GROUPS, bool CLUSTER>
+template <bool CLUSTER>
 cudaError_t launch_bulk_rule(const TreeArgs& a, int C, int num_sms, int* err, cudaStream_t st) {
     const int rule = score_rule(a.rule, 64);
-    if (rule == 2) return launch_bulk<GROUPS, CLUSTER, true, true>(a, C, num_sms, err, st);
-    if (rule == 1) return launch_bulk<GROUPS, CLUSTER, true, false>(a, C, num_sms, err, st);
-    return launch_bulk<GROUPS, CLUSTER, false, false>(a, C, num_sms, err, st);
+    if (rule == 2) return launch_bulk<CLUSTER, true, true>(a, C, num_sms, err, st);
+    if (rule == 1) return launch_bulk<CLUSTER, true, false>(a, C, num_sms, err, st);
+    return launch_bulk<CLUSTER, false, false>(a, C, num_sms, err, st);
 }
 
-template <int GROUPS, bool CLUSTER>
+template <bool CLUSTER>
 cudaError_t configure_bulk() {
-    const void* fns[3] = {(const void*)k_tree_attention_bulk<GROUPS, CLUSTER, true, true>,
-                          (const void*)k_tree_attention_bulk<GROUPS, CLUSTER, true, false>,
-                          (const void*)k_tree_attention_bulk<GROUPS, CLUSTER, false, false>};
+    const void* fns[3] = {(const void*)k_tree_attention_bulk<CLUSTER, true, true>,
+                          (const void*)k_tree_attention_bulk<CLUSTER, true, false>,
+                          (const void*)k_tree_attention_bulk<CLUSTER, false, false>};
     for (const void* f : fns) {
         const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BLOCK_SMEM);
         if (e != cudaSuccess) return e;
@@ -1093,10 +1118,16 @@ cudaError_t configure_bulk() {
     for (int lg = 1; CLUSTER && lg < 4; lg++) {
         int n = 1 << 30;
         for (const void* f : fns) n = std::min(n, max_clusters(f, 1 << lg, BTHREADS, BLOCK_SMEM));
-        g_bulk_clusters[GROUPS - 1][lg] = n;
+        g_bulk_clusters[lg] = n;
     }
     return cudaSuccess;
 }
+
+// Head width, warps, key tiles of a warp, channels of O at a time.
+using Short64 = TreeShape<64, 8, 4, 64>;
+using Long64 = TreeShape<64, 8, 16, 32>;
+using Short128 = TreeShape<128, 8, 8, 64>;
+using Long128 = TreeShape<128, 8, 16, 64>;
 
 }  // namespace
 
@@ -1104,19 +1135,17 @@ cudaError_t launch_tree_attention(const TreeArgs& a, int num_sms, int* err, cuda
     if (a.n_seq == 0 || a.max_count == 0) return cudaSuccess;
     const bool vec = a.cache.vec && reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride % 16 == 0 &&
                      a.rule.tlen <= ATTN_TABLE_MAX;
-    if (vec && a.cache.hd == 64 && a.max_keys > TW * 64) {
+    if (vec && a.cache.hd == 64) {
+        if (a.max_keys <= Short64::KEYS) return Short64::launch(a, err, st);
         int C = 1;
         while (C * BK < a.max_keys) C *= 2;
-        if (bulk_smem(C, a.rule.reach) <= BLOCK_SMEM) {
-            const bool tile = a.max_count * (a.n_head / a.n_kv) <= 16;  // one tile a head
-            if (C == 1)
-                return tile ? launch_bulk_rule<1, false>(a, C, num_sms, err, st)
-                            : launch_bulk_rule<2, false>(a, C, num_sms, err, st);
-            return tile ? launch_bulk_rule<1, true>(a, C, num_sms, err, st) : launch_bulk_rule<2, true>(a, C, num_sms, err, st);
-        }
+        // More than one tile a head: K and V are worth keeping in shared memory.
+        if (a.max_count * (a.n_head / a.n_kv) > 16 && bulk_smem(C, a.rule.reach) <= BLOCK_SMEM)
+            return C == 1 ? launch_bulk_rule<false>(a, C, num_sms, err, st) : launch_bulk_rule<true>(a, C, num_sms, err, st);
+        return Long64::launch(a, err, st);
     }
-    if (vec && a.cache.hd == 64) return launch_tree_width<64>(a, num_sms, err, st);
-    if (vec && a.cache.hd == 128) return launch_tree_width<128>(a, num_sms, err, st);
+    if (vec && a.cache.hd == 128)
+        return a.max_keys <= Short128::KEYS ? Short128::launch(a, err, st) : Long128::launch(a, err, st);
     const size_t smem = 4 * (size_t)a.max_keys + (size_t)a.cache.hd;
     const dim3 grid(a.n_seq * (uint32_t)a.max_count, (uint32_t)a.n_head);
     k_tree_attention_any<<<grid, ANY_THREADS, smem, st>>>(a, err);
@@ -1124,16 +1153,12 @@ cudaError_t launch_tree_attention(const TreeArgs& a, int num_sms, int* err, cuda
 }
 
 cudaError_t configure_draft_kernels() {
-    cudaError_t e = configure_tree<64, 4>();
-    if (e == cudaSuccess) e = configure_tree<64, 8>();
-    if (e == cudaSuccess) e = configure_tree<128, 4>();
-    if (e == cudaSuccess) e = configure_tree<128, 8>();
-    if (e == cudaSuccess) e = configure_tree<128, 16>();
-    if (e == cudaSuccess) e = configure_tree<64, 16>();
-    if (e == cudaSuccess) e = configure_bulk<1, false>();
-    if (e == cudaSuccess) e = configure_bulk<1, true>();
-    if (e == cudaSuccess) e = configure_bulk<2, false>();
-    if (e == cudaSuccess) e = configure_bulk<2, true>();
+    cudaError_t e = Short64::configure();
+    if (e == cudaSuccess) e = Long64::configure();
+    if (e == cudaSuccess) e = Short128::configure();
+    if (e == cudaSuccess) e = Long128::configure();
+    if (e == cudaSuccess) e = configure_bulk<false>();
+    if (e == cudaSuccess) e = configure_bulk<true>();
     if (e == cudaSuccess) e = configure_beam();
     if (e != cudaSuccess) return e;
     return cudaFuncSetAttribute((const void*)k_tree_attention_any, cudaFuncAttributeMaxDynamicSharedMemorySize,
