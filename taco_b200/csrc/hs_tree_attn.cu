@@ -363,44 +363,77 @@ __device__ __forceinline__ void tree_multiply(const int32_t (&c)[NT][4], const u
     }
 }
 
-// N outputs (1, 2 or 4 channels from `ch` on) of row x of a tree's kv head, in one store where they are aligned.
-template <int N>
-__device__ __forceinline__ void tree_put(const TreeArgs& a, const TreeSeq& s, int kv, int G, int x, int hd, int ch,
-                                         const int2 (&o)[N], float fsc, double omsc, bool fast) {
-    int8_t* to = a.out + ((size_t)s.first_row + node_of(x, G)) * a.out_stride + (size_t)(kv * G + head_of(x, G)) * hd + ch;
-    uint32_t y[N], word = 0;
+// O of a tile and 16 HD channels in shared memory: two whole numbers a row and channel, sum (p >> 8) v and
+// sum (p & 255) v. With sum p <= 2^30 and |v| <= 128 the first is at most 2^29 in magnitude over all keys, the
+// second at most 8192 * 2^15 = 2^28. The word of lane l's number x (of tree_multiply) for row g + 8 r and the 8
+// channels j: each of a warp's additions takes all the banks, and so do the reads of the 16 quads of a row.
+__device__ __forceinline__ int o_at(int j, int r, int x, int l) { return ((j * 2 + r) * 4 + x) * 32 + ((l + 4 * j) & 31); }
+
+__device__ __forceinline__ void o_add(int32_t* o, int j, const int4 (&x)[2]) {
+    const int l = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
+    for (int r = 0; r < 2; r++) {
+        atomicAdd(o + o_at(j, r, 0, l), x[r].x);
+        atomicAdd(o + o_at(j, r, 1, l), x[r].y);
+        atomicAdd(o + o_at(j, r, 2, l), x[r].z);
+        atomicAdd(o + o_at(j, r, 3, l), x[r].w);
+    }
+}
+
+// The numbers of four channels, 4 quad .. 4 quad + 3, of a row.
+__device__ __forceinline__ void o_get(const int32_t* o, int row, int quad, int2 (&y)[4]) {
+    const int l = 4 * (row & 7) + 2 * (quad & 1);
+    int2 c[4];
+#pragma unroll
+    for (int x = 0; x < 4; x++) c[x] = *reinterpret_cast<const int2*>(o + o_at(quad >> 1, row >> 3, x, l));
+    y[0] = make_int2(c[0].x, c[1].x);
+    y[1] = make_int2(c[2].x, c[3].x);
+    y[2] = make_int2(c[0].y, c[1].y);
+    y[3] = make_int2(c[2].y, c[3].y);
+}
+__device__ __forceinline__ void o_clear(int32_t* o, int row, int quad) {
+#pragma unroll
+    for (int x = 0; x < 4; x++)
+        *reinterpret_cast<int2*>(o + o_at(quad >> 1, row >> 3, x, 4 * (row & 7) + 2 * (quad & 1))) = make_int2(0, 0);
+}
+
+// The tile whose O waits to be written: the tree's first row, the kv head, the tile's first row and its rows.
+struct Pending {
+    uint32_t first_row;
+    int kv, x0, rows;
+};
+
+// The outputs of four channels of a row, in one store where they are aligned.
+__device__ __forceinline__ void tree_put(const TreeArgs& a, const Pending& p, int G, int row, int hd, int quad,
+                                         const int2 (&o)[4], float fsc, double omsc, bool fast) {
+    const int x = p.x0 + row;
+    int8_t* to = a.out + ((size_t)p.first_row + node_of(x, G)) * a.out_stride +
+                 (size_t)(p.kv * G + head_of(x, G)) * hd + 4 * quad;
+    uint32_t y[4], word = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
         y[i] = (uint32_t)output_of(o[i], a.rule.om, a.rule.os, fsc, omsc, fast) & 0xFFu;
         word |= y[i] << (8 * i);
     }
-    if (reinterpret_cast<uintptr_t>(to) % N == 0) {
-        if constexpr (N == 4) *reinterpret_cast<uint32_t*>(to) = word;
-        else if constexpr (N == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)word;
-        else *to = (int8_t)word;
+    if (reinterpret_cast<uintptr_t>(to) % 4 == 0) {
+        *reinterpret_cast<uint32_t*>(to) = word;
     } else {
 #pragma unroll
-        for (int i = 0; i < N; i++) to[i] = (int8_t)y[i];
+        for (int i = 0; i < 4; i++) to[i] = (int8_t)y[i];
     }
 }
 
-// O of a row and channel in two whole numbers, sum (p >> 8) v and sum (p & 255) v: with sum p <= 2^30 and
-// |v| <= 128 the first is at most 2^29 in magnitude over all keys, the second at most 8192 * 2^15 = 2^28.
-// Odd rows' channels are 8 pairs off (exclusive or), so that the two rows of a quarter warp's stores of a part
-// take all the banks.
-__device__ __forceinline__ int part_at(int row, int ch) { return ch ^ ((row & 1) << 3); }
-
-// Shared memory of W warps in clusters of C blocks: the warps' parts of O [W][16][CH] pairs, then by slice of
-// the item the row sums [W C][16] u64 and maxima [W C][16] i32 (each block of a cluster has all of them), the
+// Shared memory of W warps in clusters of C blocks: O of this item and the last [2][16 HD][2] i32, then by slice
+// of the item the row sums [W C][16] u64 and maxima [W C][16] i32 (each block of a cluster has all of them), the
 // exponent table up to its last change.
-constexpr size_t tree_smem(int W, int CH, int C, int reach) {
-    return 8 * (size_t)W * 16 * CH + (size_t)W * C * 16 * 12 + 4 * (((size_t)reach + 3) & ~(size_t)3);
+constexpr size_t tree_smem(int W, int HD, int C, int reach) {
+    return 16 * (size_t)16 * HD + (size_t)W * C * 16 * 12 + 4 * (((size_t)reach + 3) & ~(size_t)3);
 }
 
-template <int HD, int TW, int NT, int CH, bool NARROW, bool SSHI>
+template <int HD, int TW, int NT, bool NARROW, bool SSHI>
 __global__ void __launch_bounds__(32 * TW, 2) k_tree_attention(const __grid_constant__ TreeArgs a, int tiles, int items,
                                                                int* err) {
-    constexpr int TTHREADS = 32 * TW, PER = 16 * CH / TTHREADS;  // sums of a thread
+    constexpr int TTHREADS = 32 * TW, QUADS = HD / 4;
     constexpr int S = 8 * NT;        // keys of a warp
     constexpr int TK = 2 * NT;       // keys of a thread
     constexpr int KB = HD / 64;      // 16-byte pieces of a key's row per thread
@@ -408,8 +441,8 @@ __global__ void __launch_bounds__(32 * TW, 2) k_tree_attention(const __grid_cons
     extern __shared__ __align__(16) uint8_t s_tree[];
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-    int2(*part)[16][CH] = reinterpret_cast<int2(*)[16][CH]>(s_tree);
-    uint64_t(*wsum)[16] = reinterpret_cast<uint64_t(*)[16]>(part + TW);
+    int32_t(*o)[32 * HD] = reinterpret_cast<int32_t(*)[32 * HD]>(s_tree);
+    uint64_t(*wsum)[16] = reinterpret_cast<uint64_t(*)[16]>(o + 2);
     int32_t(*wmax)[16] = reinterpret_cast<int32_t(*)[16]>(wsum + TW * C);
     int32_t* sT = reinterpret_cast<int32_t*>(wmax + TW * C);
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -420,12 +453,34 @@ __global__ void __launch_bounds__(32 * TW, 2) k_tree_attention(const __grid_cons
     const bool fast = a.rule.os <= 95 && fabs(omsc) <= 1.9073486328125e-6;
     for (int i = tid; i < (a.rule.reach + 3) / 4; i += TTHREADS)
         reinterpret_cast<int4*>(sT)[i] = reinterpret_cast<const int4*>(a.rule.table)[i];
+    for (int i = tid; i < 2 * 32 * HD; i += TTHREADS) o[0][i] = 0;
     auto meet = [&]() {  // of all the item's warps
         if (C > 1) cl.sync();
         else __syncthreads();
     };
     // No block of the cluster writes to another before that one runs.
     meet();
+    // O of the last item out: the cluster's sum, each block some rows.
+    Pending last_item{0, 0, 0, 0};
+    uint32_t count = 0;  // of the items so far: item i adds to o[i & 1]
+    auto put = [&]() {
+        for (int i = rank * TTHREADS + tid; i < 16 * QUADS; i += C * TTHREADS) {
+            const int row = i / QUADS, quad = i % QUADS;
+            if (row >= last_item.rows) break;
+            int2 y[4];
+            o_get(o[~count & 1], row, quad, y);
+            for (int b = 1; b < C; b++) {
+                int2 z[4];
+                o_get(cl.map_shared_rank(o[~count & 1], (rank + b) % C), row, quad, z);
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    y[x].x += z[x].x;
+                    y[x].y += z[x].y;
+                }
+            }
+            tree_put(a, last_item, G, row, HD, quad, y, fsc, omsc, fast);
+        }
+    };
 
     // The keys and values of an item's slice of this warp, on their way into L2.
     auto ask = [&](const TreeSeq& s, int kv, int tile, bool keys) {
@@ -541,6 +596,8 @@ __global__ void __launch_bounds__(32 * TW, 2) k_tree_attention(const __grid_cons
         }
         meet();
         if (item + stride < items) ask(next, (item + stride) / tiles % a.n_kv, (item + stride) % tiles, true);
+        // Every block has added to the last item's O; it is read before the next meeting and cleared after it.
+        put();
         if (on) {
             // Lane l has row l % 16.
             int32_t e = m >= 0 ? INT32_MIN : INT32_MAX;
@@ -584,68 +641,22 @@ __global__ void __launch_bounds__(32 * TW, 2) k_tree_attention(const __grid_cons
             for (int i = 0; i < slices; i++) z += wsum[i][lane & 15];
             tree_planes<NT>(c, z, a.rule.P);
         }
-        // O, CH channels at a time: each warp its keys' part, then the sum over the warps.
-        const int row = tid / (CH / PER), ch = tid % (CH / PER) * PER;
-        int2 acc[HD / CH][PER];
+        for (int i = tid; i < 16 * QUADS; i += TTHREADS) o_clear(o[~count & 1], i / QUADS, i % QUADS);
+        if (on) {
 #pragma unroll
-        for (int ch0 = 0; ch0 < HD; ch0 += CH) {
-            if (on) {
-#pragma unroll
-                for (int j = 0; j < CH / 8; j++) {
-                    // The next 8 channels' values while these are multiplied.
-                    if (ch0 + 8 * j + 8 < HD) load_v(ch0 + 8 * j + 8, v[(j + 1) & 1]);
-                    int4 x[2];
-                    tree_multiply<NT>(c, v[j & 1], x);
-#pragma unroll
-                    for (int r = 0; r < 2; r++)
-                        *reinterpret_cast<int4*>(&part[w][g + 8 * r][part_at(g, 8 * j + 2 * t)]) = x[r];
-                }
+            for (int j = 0; j < HD / 8; j++) {
+                // The next 8 channels' values while these are multiplied.
+                if (j + 1 < HD / 8) load_v(8 * j + 8, v[(j + 1) & 1]);
+                int4 x[2];
+                tree_multiply<NT>(c, v[j & 1], x);
+                o_add(o[count & 1], j, x);
             }
-            __syncthreads();
-            int2* sums = acc[ch0 / CH];
-#pragma unroll
-            for (int x = 0; x < PER; x++) sums[x] = make_int2(0, 0);
-            for (int i = 0; i < live; i++)
-#pragma unroll
-                for (int x = 0; x < PER; x++) {
-                    const int2 y = part[i][row][part_at(row, ch + x)];
-                    sums[x].x += y.x;
-                    sums[x].y += y.y;
-                }
-            if (HD > CH) __syncthreads();  // the parts are read
         }
-        if (C > 1) {
-            // The block's sums in the place of its warps' parts (with one round of channels a thread writes
-            // where it alone has read), then each block sums some rows over the cluster.
-#pragma unroll
-            for (int h = 0; h < HD / CH; h++)
-#pragma unroll
-                for (int x = 0; x < PER; x++) part[h][row][CH == HD ? part_at(row, ch + x) : ch + x] = acc[h][x];
-            cl.sync();
-            constexpr int QUADS = HD / PER;
-            for (int i = rank * TTHREADS + tid; i < 16 * QUADS; i += C * TTHREADS) {
-                const int r = i / QUADS, at = i % QUADS * PER;
-                int2 sums[PER];
-#pragma unroll
-                for (int x = 0; x < PER; x++) sums[x] = make_int2(0, 0);
-                for (int b = 0; b < C; b++) {
-                    const int2* of = cl.map_shared_rank(&part[at / CH][r][0], b);
-#pragma unroll
-                    for (int x = 0; x < PER; x++) {
-                        const int2 y = of[CH == HD ? part_at(r, at + x) : at % CH + x];
-                        sums[x].x += y.x;
-                        sums[x].y += y.y;
-                    }
-                }
-                if (r < rows) tree_put<PER>(a, s, kv, G, 16 * tile + r, HD, at, sums, fsc, omsc, fast);
-            }
-            cl.sync();  // the sums are read
-        } else if (row < rows) {
-#pragma unroll
-            for (int h = 0; h < HD / CH; h++)
-                tree_put<PER>(a, s, kv, G, 16 * tile + row, HD, h * CH + ch, acc[h], fsc, omsc, fast);
-        }
+        last_item = Pending{s.first_row, kv, 16 * tile, min(rows, 16)};
+        count++;
     }
+    meet();
+    put();
     if (C > 1) cl.sync();  // no block leaves while another reads its memory
 }
 
@@ -676,24 +687,24 @@ int score_rule(const AttnRuleView& r, int hd) {
 
 // A kernel's shape, and by log2 C the clusters that a device holds at once (found when a device is opened; the
 // GPUs of a host are alike).
-template <int HD, int TW, int NT, int CH>
+template <int HD, int TW, int NT>
 struct TreeShape {
     static constexpr int KEYS = TW * NT * 8;  // of a block
     static inline int fit[4] = {0, 0, 0, 0};
 
     static cudaError_t configure() {
-        const void* fns[3] = {(const void*)k_tree_attention<HD, TW, NT, CH, true, true>,
-                              (const void*)k_tree_attention<HD, TW, NT, CH, true, false>,
-                              (const void*)k_tree_attention<HD, TW, NT, CH, false, false>};
+        const void* fns[3] = {(const void*)k_tree_attention<HD, TW, NT, true, true>,
+                              (const void*)k_tree_attention<HD, TW, NT, true, false>,
+                              (const void*)k_tree_attention<HD, TW, NT, false, false>};
         for (const void* f : fns) {
             const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                       (int)tree_smem(TW, CH, TMAXC, ATTN_TABLE_MAX));
+                                                       (int)tree_smem(TW, HD, TMAXC, ATTN_TABLE_MAX));
             if (e != cudaSuccess) return e;
         }
         for (int lg = 0; lg < 4; lg++) {
             int n = 1 << 30;
             for (const void* f : fns)
-                n = std::min(n, max_clusters(f, 1 << lg, 32 * TW, tree_smem(TW, CH, 1 << lg, 6144)));
+                n = std::min(n, max_clusters(f, 1 << lg, 32 * TW, tree_smem(TW, HD, 1 << lg, 6144)));
             fit[lg] = n;
         }
         return cudaSuccess;
@@ -709,7 +720,7 @@ struct TreeShape {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)((items < clusters ? items : clusters) * C));
         cfg.blockDim = dim3(32 * TW);
-        cfg.dynamicSmemBytes = tree_smem(TW, CH, C, a.rule.reach);
+        cfg.dynamicSmemBytes = tree_smem(TW, HD, C, a.rule.reach);
         cfg.stream = st;
         cudaLaunchAttribute at;
         at.id = cudaLaunchAttributeClusterDimension;
@@ -717,7 +728,7 @@ struct TreeShape {
         at.val.clusterDim.y = at.val.clusterDim.z = 1;
         cfg.attrs = &at;
         cfg.numAttrs = 1;
-        return cudaLaunchKernelEx(&cfg, k_tree_attention<HD, TW, NT, CH, NARROW, SSHI>, a, tiles, items, err);
+        return cudaLaunchKernelEx(&cfg, k_tree_attention<HD, TW, NT, NARROW, SSHI>, a, tiles, items, err);
     }
 
     static cudaError_t launch(const TreeArgs& a, int* err, cudaStream_t st) {
@@ -736,10 +747,8 @@ struct TreeShape {
 // asks for its values; no warp waits to copy. One block per SM, 16 warps in two groups of 8 that take the
 // 16-row tiles of the head in turn, 128 keys a warp. The groups meet only within themselves, so one multiplies
 // while the other weighs.
-// Contexts over 1,024 keys take a cluster, a block for each 1,024 keys; the row maxima and sums go to every
-// block's shared memory, the blocks' O to the block that owns the row, with an mbarrier of the group for
-// each meeting. The exponent table is held up to its last change (table_reach); a table that leaves no room
-// for the rest takes the kernel above.
+// The exponent table is held up to its last change (table_reach); a table that leaves no room for the rest
+// takes the kernel above, as do longer contexts.
 
 constexpr int BK = 1024;                 // keys of a block
 constexpr int BWARPS = 16, GROUPS = 2;
@@ -751,67 +760,35 @@ struct __align__(16) TreeBulk {
     uint8_t v[64 * VROW];
     uint64_t k_full, v_full;
     uint32_t k_done, v_done;             // warps that need this head's keys (values) no more
-    uint64_t met[GROUPS][3];             // of a cluster's groups: maxima, sums, O (three meetings)
 };
-// Behind it: the warps' O [BWARPS][16][channels] pairs (32 channels at a time, 16 in clusters, for room), the
-// groups' wsum [slices][16] u64 and wmax [slices][16] i32 (slices: the warps of the group in the cluster), in
-// clusters the owned rows' O [groups][16][64] pairs, and the table.
-__host__ __device__ constexpr int bulk_channels(bool cluster) { return cluster ? 16 : 32; }
-constexpr size_t bulk_smem(int C, int reach) {
-    return sizeof(TreeBulk) + (size_t)BWARPS * 16 * bulk_channels(C > 1) * 8 + (size_t)BWARPS * C * 16 * 12 +
-           (C > 1 ? GROUPS * 16 * 64 * 8 : 0) + 4 * (((size_t)reach + 3) & ~(size_t)3);
+// Behind it: the groups' O [GROUPS][16 * 64][2] i32, the warps' wsum [BWARPS][16] u64 and wmax [BWARPS][16] i32,
+// and the table.
+constexpr size_t bulk_smem(int reach) {
+    return sizeof(TreeBulk) + 8 * (size_t)GROUPS * 16 * 64 + (size_t)BWARPS * 16 * 12 + 4 * (((size_t)reach + 3) & ~(size_t)3);
 }
 constexpr size_t BLOCK_SMEM = 227 * 1024;
-static_assert(bulk_smem(1, 7800) <= BLOCK_SMEM && bulk_smem(8, 6200) <= BLOCK_SMEM, "room for the usual tables");
-
-// Arrives on the mbarrier at the same place of block `rank` of the cluster, after this thread's writes.
-__device__ __forceinline__ void mbar_arrive_cluster(uint64_t* bar, int rank) {
-    asm volatile(
-        "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, %1;\n\t"
-        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n\t}" ::"r"(smem_u32(bar)),
-        "r"(rank)
-        : "memory");
-}
-__device__ __forceinline__ void mbar_wait_cluster(uint64_t* bar, uint32_t phase, int* err, int code) {
-    for (uint32_t i = 0; i < (1u << 26); i++) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(phase)
-            : "memory");
-        if (ok) return;
-        if (i > 64) __nanosleep(32);
-        if ((i & 1023) == 0 && *(volatile int*)err != 0) return;
-    }
-    atomicCAS(err, 0, code);
-}
+static_assert(bulk_smem(ATTN_TABLE_MAX) <= BLOCK_SMEM, "room for every table");
 
 // A wait that gives up sets the error word and lets its thread go on: every barrier still gets its arrivals,
 // every later wait returns at once, and the call's results count for nothing.
-template <bool CLUSTER, bool NARROW, bool SSHI>
+template <bool NARROW, bool SSHI>
 __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __grid_constant__ TreeArgs a, int works,
                                                                      int* err) {
     constexpr int HD = 64, WPG = BWARPS / GROUPS, NT = BK / WPG / 8, S = 8 * NT, TK = 2 * NT, VB = TK / 4;
-    constexpr int GTHREADS = 32 * WPG, CC = bulk_channels(CLUSTER), PER = 16 * CC / GTHREADS;
+    constexpr int GTHREADS = 32 * WPG;
+    static_assert(GTHREADS == 16 * HD / 4, "a thread of a group for each four channels of a tile's row");
     extern __shared__ __align__(128) uint8_t s_bulk[];
     TreeBulk& sm = *reinterpret_cast<TreeBulk*>(s_bulk);
-    cg::cluster_group cl = cg::this_cluster();
-    const int C = CLUSTER ? (int)cl.num_blocks() : 1, rank = CLUSTER ? (int)cl.block_rank() : 0;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int grp = warp / WPG, w = warp % WPG, gtid = tid - grp * GTHREADS, g = lane >> 2, t = lane & 3;
-    const int G = a.n_head / a.n_kv, first = blockIdx.x / C, stride = gridDim.x / C;
-    int2(*parts)[16][CC] = reinterpret_cast<int2(*)[16][CC]>(&sm + 1);
-    uint64_t(*wsums)[16] = reinterpret_cast<uint64_t(*)[16]>(parts + BWARPS);
-    int32_t(*wmaxs)[16] = reinterpret_cast<int32_t(*)[16]>(wsums + BWARPS * C);
-    int2(*owns)[16][HD] = reinterpret_cast<int2(*)[16][HD]>(wmaxs + BWARPS * C);
-    int32_t* table = reinterpret_cast<int32_t*>(owns + (CLUSTER ? GROUPS : 0));
-    const int slice = rank * WPG + w;
-    int2(*part)[16][CC] = parts + grp * WPG;
-    uint64_t(*wsum)[16] = wsums + grp * C * WPG;
-    int32_t(*wmax)[16] = wmaxs + grp * C * WPG;
-    int2(*own)[HD] = owns[CLUSTER ? grp : 0];
+    const int G = a.n_head / a.n_kv, first = blockIdx.x, stride = gridDim.x;
+    int32_t(*os)[32 * HD] = reinterpret_cast<int32_t(*)[32 * HD]>(&sm + 1);
+    uint64_t(*wsums)[16] = reinterpret_cast<uint64_t(*)[16]>(os + GROUPS);
+    int32_t(*wmaxs)[16] = reinterpret_cast<int32_t(*)[16]>(wsums + BWARPS);
+    int32_t* table = reinterpret_cast<int32_t*>(wmaxs + BWARPS);
+    int32_t* o = os[grp];
+    uint64_t(*wsum)[16] = wsums + grp * WPG;
+    int32_t(*wmax)[16] = wmaxs + grp * WPG;
     const int32_t m = a.rule.sm;
     const int ss = a.rule.ss, last = a.rule.reach - 1;
     const double omsc = (double)a.rule.om * exp2_neg(a.rule.os);
@@ -821,35 +798,30 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
         mbar_init(&sm.k_full, 1);
         mbar_init(&sm.v_full, 1);
         sm.k_done = sm.v_done = 0;
-        for (int i = 0; i < GROUPS; i++)
-            for (int k = 0; k < 3; k++) mbar_init(&sm.met[i][k], WPG * C);
         fence_barrier_init();
     }
-    if (CLUSTER)
-        for (int i = tid; i < GROUPS * 16 * HD; i += BTHREADS) (&owns[0][0][0])[i] = make_int2(0, 0);
     for (int i = tid; i < (a.rule.reach + 3) / 4; i += BTHREADS)
         reinterpret_cast<int4*>(table)[i] = reinterpret_cast<const int4*>(a.rule.table)[i];
-    if (CLUSTER) cl.sync();
-    else __syncthreads();
+    for (int i = gtid; i < 32 * HD; i += GTHREADS) o[i] = 0;
+    __syncthreads();
 
     // The copies of the keys (values) of the first work from `work` on that has rows, by one warp.
     auto copy = [&](int work, bool values) {
         for (; work < works; work += stride) {
             const TreeSeq s = a.seqs[work / a.n_kv];
             if (!tree_seq_ok(s, a.n_rows, a.cache.slots, a.max_count, a.max_keys) || s.count == 0) continue;
-            const int n = (int)(s.prefix + s.count), k0 = rank * BK, kn = max(0, min(BK, n - k0));
+            const int n = (int)(s.prefix + s.count);
             const size_t plane = (size_t)s.slot * a.cache.slot_stride +
                                  (size_t)(a.plane0 + work % a.n_kv) * ((size_t)a.cache.n_ctx * HD);
             if (values) {
-                const uint32_t bytes = (uint32_t)(kn + 15) & ~15u;  // (n_ctx % 16 == 0)
+                const uint32_t bytes = (uint32_t)(n + 15) & ~15u;  // (n_ctx % 16 == 0)
                 if (lane == 0) mbar_arrive_expect_tx(&sm.v_full, bytes * HD);
                 __syncwarp();
-                if (kn)
-                    for (int ch = lane; ch < HD; ch += 32)
-                        bulk_load(sm.v + ch * VROW, a.cache.v + plane + (size_t)ch * a.cache.n_ctx + k0, bytes, &sm.v_full);
+                for (int ch = lane; ch < HD; ch += 32)
+                    bulk_load(sm.v + ch * VROW, a.cache.v + plane + (size_t)ch * a.cache.n_ctx, bytes, &sm.v_full);
             } else if (lane == 0) {
-                mbar_arrive_expect_tx(&sm.k_full, (uint32_t)kn * HD);
-                if (kn) bulk_load(sm.k, a.cache.k + plane + (size_t)k0 * HD, (uint32_t)kn * HD, &sm.k_full);
+                mbar_arrive_expect_tx(&sm.k_full, (uint32_t)n * HD);
+                bulk_load(sm.k, a.cache.k + plane, (uint32_t)n * HD, &sm.k_full);
             }
             break;
         }
@@ -876,17 +848,14 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
         __syncwarp();
         named_bar(1 + grp, GTHREADS);
     };
-    // The group's warps, of all blocks of the cluster, at meeting k of this round.
-    uint32_t round = 0;
-    auto meet = [&](int k) {
-        if (CLUSTER) {
-            __syncwarp();
-            if (lane < C) mbar_arrive_cluster(&sm.met[grp][k], lane);
-            mbar_wait_cluster(&sm.met[grp][k], round & 1, err, 52 + k);
-            __syncwarp();
-        } else {
-            group_bar();
-        }
+    // O of the group's last tile out, between two meetings: every warp has added to it, none adds yet.
+    Pending last_tile{0, 0, 0, 0};
+    auto put = [&]() {
+        const int row = gtid / (HD / 4), quad = gtid % (HD / 4);
+        int2 y[4];
+        o_get(o, row, quad, y);
+        o_clear(o, row, quad);
+        if (row < last_tile.rows) tree_put(a, last_tile, G, row, HD, quad, y, fsc, omsc, fast);
     };
     uint32_t count = 0;
     for (int work = first; work < works; work += stride) {
@@ -898,13 +867,12 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
         if (s.count == 0) continue;
         const int kv = work % a.n_kv, prefix = (int)s.prefix, n = prefix + (int)s.count;
         const int total = (int)s.count * G, tiles = (total + 15) / 16, slices = (n + S - 1) / S;
-        const int live = CLUSTER ? min(max(slices - rank * WPG, 0), WPG) : slices;  // this block's warps with keys
-        const bool on = slice < slices;
-        const int k0 = slice * S;  // of the context; the block's copy starts at rank * BK
+        const bool on = w < slices;
+        const int k0 = w * S;
         const uint32_t phase = count & 1;
         count++;
-        const uint8_t* ks = sm.k + (size_t)(w * S) * HD;
-        const uint8_t* vs = sm.v + w * S + t * TK;
+        const uint8_t* ks = sm.k + (size_t)k0 * HD;
+        const uint8_t* vs = sm.v + k0 + t * TK;
         // The rows of a tile: their fragments and what they see of this thread's keys (slices inside the
         // context are whole for every row), loaded a tile ahead.
         const bool whole = k0 + S <= prefix;
@@ -964,28 +932,26 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
                 }
                 int32_t ext[2];
                 tree_extremes<NT>(c, whole, seen, m, ext);
-                // Lane t of a quad gives them to the blocks t, t + 4.
-                for (int b = t; b < C; b += 4) {
-                    int32_t* to = CLUSTER ? cl.map_shared_rank(&wmax[slice][0], b) : wmax[slice];
-                    to[g] = ext[0];
-                    to[g + 8] = ext[1];
+                if (t == 0) {
+                    wmax[w][g] = ext[0];
+                    wmax[w][g + 8] = ext[1];
                 }
             }
             if (tile + GROUPS >= tiles) done(work, false);  // the group's last scores of this head
-            meet(0);
+            group_bar();
+            put();
             if (on) {
                 // Lane l has row l % 16.
                 int32_t e = m >= 0 ? INT32_MIN : INT32_MAX;
                 for (int i = 0; i < slices; i++) e = m >= 0 ? max(e, wmax[i][lane & 15]) : min(e, wmax[i][lane & 15]);
                 uint64_t sum[2];
                 tree_weigh<NT, NARROW, SSHI>(c, whole, seen, e, m, ss, table, last, sum);
-                for (int b = t; b < C; b += 4) {
-                    uint64_t* to = CLUSTER ? cl.map_shared_rank(&wsum[slice][0], b) : wsum[slice];
-                    to[g] = sum[0];
-                    to[g + 8] = sum[1];
+                if (t == 0) {
+                    wsum[w][g] = sum[0];
+                    wsum[w][g + 8] = sum[1];
                 }
             }
-            meet(1);
+            group_bar();
             if (tile + GROUPS < tiles) load_rows(tile + GROUPS);
             if (on) {
                 uint64_t z = 0;
@@ -993,74 +959,25 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
                 tree_planes<NT>(c, z, a.rule.P);
             }
             if (tile == grp) mbar_wait(&sm.v_full, phase, err, 56);
-            // O, CC channels at a time: each warp its keys' part, then the sum over the warps, PER channels of
-            // a row a thread. (Odd rows' channels are 8 pairs off, so that the two rows of a quarter warp's
-            // stores take all the banks.)
-            const int row = gtid / (CC / PER), ch = gtid % (CC / PER) * PER;
-#pragma unroll 1
-            for (int ch0 = 0; ch0 < HD; ch0 += CC) {
-                if (on) {
+            if (on) {
 #pragma unroll
-                    for (int j = 0; j < CC / 8; j++) {
-                        uint32_t v[VB];
+                for (int j = 0; j < HD / 8; j++) {
+                    uint32_t v[VB];
 #pragma unroll
-                        for (int b = 0; b < TK / 16; b++) {
-                            const uint4 x = *reinterpret_cast<const uint4*>(vs + (ch0 + 8 * j + g) * VROW + 16 * b);
-                            v[4 * b] = x.x;
-                            v[4 * b + 1] = x.y;
-                            v[4 * b + 2] = x.z;
-                            v[4 * b + 3] = x.w;
-                        }
-                        int4 x[2];
-                        tree_multiply<NT>(c, v, x);
-#pragma unroll
-                        for (int r = 0; r < 2; r++)
-                            *reinterpret_cast<int4*>(&part[w][g + 8 * r][part_at(g, 8 * j + 2 * t)]) = x[r];
+                    for (int b = 0; b < TK / 16; b++) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(vs + (8 * j + g) * VROW + 16 * b);
+                        v[4 * b] = x.x;
+                        v[4 * b + 1] = x.y;
+                        v[4 * b + 2] = x.z;
+                        v[4 * b + 3] = x.w;
                     }
+                    int4 x[2];
+                    tree_multiply<NT>(c, v, x);
+                    o_add(o, j, x);
                 }
-                if (ch0 + CC == HD && tile + GROUPS >= tiles) done(work, true);  // the last product of this head
-                group_bar();
-                int2 o[PER];
-#pragma unroll
-                for (int x = 0; x < PER; x++) o[x] = make_int2(0, 0);
-                for (int i = 0; i < live; i++)
-#pragma unroll
-                    for (int x = 0; x < PER; x++) {
-                        const int2 y = part[i][row][part_at(row, ch + x)];
-                        o[x].x += y.x;
-                        o[x].y += y.y;
-                    }
-                if constexpr (CLUSTER) {
-                    // To the block that owns the row.
-                    if (live > 0) {
-                        int2* to = cl.map_shared_rank(&own[row][ch0 + ch], row % C);
-#pragma unroll
-                        for (int x = 0; x < PER; x++) {
-                            atomicAdd(&to[x].x, o[x].x);
-                            atomicAdd(&to[x].y, o[x].y);
-                        }
-                    }
-                } else if (row < rows) {
-                    tree_put<PER>(a, s, kv, G, 16 * tile + row, HD, ch0 + ch, o, fsc, omsc, fast);
-                }
-                if (ch0 + CC < HD) group_bar();  // the parts are read
             }
-            if (CLUSTER) {
-                meet(2);
-                round++;
-                for (int i = gtid; i < 16 * HD / 4; i += GTHREADS) {
-                    const int r = i / (HD / 4), c4 = i % (HD / 4) * 4;
-                    if (r % C != rank) continue;
-                    int2 o[4];
-#pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        o[x] = own[r][c4 + x];
-                        own[r][c4 + x] = make_int2(0, 0);  // for the next tile
-                    }
-                    if (r < rows) tree_put<4>(a, s, kv, G, 16 * tile + r, HD, c4, o, fsc, omsc, fast);
-                }
-                __syncwarp();
-            }
+            if (tile + GROUPS >= tiles) done(work, true);  // the group's last product of this head
+            last_tile = Pending{s.first_row, kv, 16 * tile, min(rows, 16)};
         }
         if (grp >= tiles) {
             // No tile for this group: the copies are not needed, but each is waited for, so that the counts are
@@ -1071,63 +988,32 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
             done(work, true);
         }
     }
-    __syncwarp();
-    if (CLUSTER) cl.sync();  // no block leaves while another writes to it
+    group_bar();
+    put();
 }
 
-// By log2 C, the resident clusters (found when a device is opened; the GPUs of a host are alike).
-int g_bulk_clusters[4];
-
-template <bool CLUSTER, bool NARROW, bool SSHI>
-cudaError_t launch_bulk(const TreeArgs& a, int C, int num_sms, int* err, cudaStream_t st) {
+template <bool NARROW, bool SSHI>
+cudaError_t launch_bulk(const TreeArgs& a, int num_sms, int* err, cudaStream_t st) {
     const int works = (int)a.n_seq * a.n_kv;
-    int lg = 0;
-    while (1 << lg < C) lg++;
-    const int fit = C == 1 ? num_sms : g_bulk_clusters[lg], clusters = fit > 0 ? fit : 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)((works < clusters ? works : clusters) * C));
-    cfg.blockDim = dim3(BTHREADS);
-    cfg.dynamicSmemBytes = bulk_smem(C, a.rule.reach);
-    cfg.stream = st;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)C;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_tree_attention_bulk<CLUSTER, NARROW, SSHI>, a, works, err);
+    k_tree_attention_bulk<NARROW, SSHI>
+        <<<works < num_sms ? works : num_sms, BTHREADS, bulk_smem(a.rule.reach), st>>>(a, works, err);
+    return cudaGetLastError();
 }
 
-template <bool CLUSTER>
-cudaError_t launch_bulk_rule(const TreeArgs& a, int C, int num_sms, int* err, cudaStream_t st) {
-    const int rule = score_rule(a.rule, 64);
-    if (rule == 2) return launch_bulk<CLUSTER, true, true>(a, C, num_sms, err, st);
-    if (rule == 1) return launch_bulk<CLUSTER, true, false>(a, C, num_sms, err, st);
-    return launch_bulk<CLUSTER, false, false>(a, C, num_sms, err, st);
-}
-
-template <bool CLUSTER>
 cudaError_t configure_bulk() {
-    const void* fns[3] = {(const void*)k_tree_attention_bulk<CLUSTER, true, true>,
-                          (const void*)k_tree_attention_bulk<CLUSTER, true, false>,
-                          (const void*)k_tree_attention_bulk<CLUSTER, false, false>};
-    for (const void* f : fns) {
+    for (const void* f : {(const void*)k_tree_attention_bulk<true, true>, (const void*)k_tree_attention_bulk<true, false>,
+                          (const void*)k_tree_attention_bulk<false, false>}) {
         const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BLOCK_SMEM);
         if (e != cudaSuccess) return e;
-    }
-    for (int lg = 1; CLUSTER && lg < 4; lg++) {
-        int n = 1 << 30;
-        for (const void* f : fns) n = std::min(n, max_clusters(f, 1 << lg, BTHREADS, BLOCK_SMEM));
-        g_bulk_clusters[lg] = n;
     }
     return cudaSuccess;
 }
 
-// Head width, warps, key tiles of a warp, channels of O at a time.
-using Short64 = TreeShape<64, 8, 4, 64>;
-using Long64 = TreeShape<64, 8, 16, 32>;
-using Short128 = TreeShape<128, 8, 8, 64>;
-using Long128 = TreeShape<128, 8, 16, 64>;
+// Head width, warps, key tiles of a warp.
+using Short64 = TreeShape<64, 8, 4>;
+using Long64 = TreeShape<64, 8, 16>;
+using Short128 = TreeShape<128, 8, 8>;
+using Long128 = TreeShape<128, 8, 16>;
 
 }  // namespace
 
@@ -1137,11 +1023,13 @@ cudaError_t launch_tree_attention(const TreeArgs& a, int num_sms, int* err, cuda
                      a.rule.tlen <= ATTN_TABLE_MAX;
     if (vec && a.cache.hd == 64) {
         if (a.max_keys <= Short64::KEYS) return Short64::launch(a, err, st);
-        int C = 1;
-        while (C * BK < a.max_keys) C *= 2;
-        // More than one tile a head: K and V are worth keeping in shared memory.
-        if (a.max_count * (a.n_head / a.n_kv) > 16 && bulk_smem(C, a.rule.reach) <= BLOCK_SMEM)
-            return C == 1 ? launch_bulk_rule<false>(a, C, num_sms, err, st) : launch_bulk_rule<true>(a, C, num_sms, err, st);
+        // More than one tile a head, and K and V fit in a block.
+        if (a.max_keys <= BK && a.max_count * (a.n_head / a.n_kv) > 16 && bulk_smem(a.rule.reach) <= BLOCK_SMEM) {
+            const int rule = score_rule(a.rule, 64);
+            return rule == 2   ? launch_bulk<true, true>(a, num_sms, err, st)
+                   : rule == 1 ? launch_bulk<true, false>(a, num_sms, err, st)
+                               : launch_bulk<false, false>(a, num_sms, err, st);
+        }
         return Long64::launch(a, err, st);
     }
     if (vec && a.cache.hd == 128)
@@ -1157,8 +1045,7 @@ cudaError_t configure_draft_kernels() {
     if (e == cudaSuccess) e = Long64::configure();
     if (e == cudaSuccess) e = Short128::configure();
     if (e == cudaSuccess) e = Long128::configure();
-    if (e == cudaSuccess) e = configure_bulk<false>();
-    if (e == cudaSuccess) e = configure_bulk<true>();
+    if (e == cudaSuccess) e = configure_bulk();
     if (e == cudaSuccess) e = configure_beam();
     if (e != cudaSuccess) return e;
     return cudaFuncSetAttribute((const void*)k_tree_attention_any, cudaFuncAttributeMaxDynamicSharedMemorySize,
