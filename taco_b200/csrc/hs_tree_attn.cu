@@ -283,7 +283,8 @@ __device__ __forceinline__ void tree_weigh(int32_t (&c)[NT][4], bool whole, cons
                 if constexpr (!decltype(all)::value)
                     if (((seen[x >> 1] >> (2 * i + (x & 1))) & 1) == 0) e = 0;
                 c[i][x] = (int32_t)e;
-                sum[x >> 1] = add_wide(sum[x >> 1], e);
+                // (weights are below 2^31: two fit in 32 bits)
+                if (x & 1) sum[x >> 1] = add_wide(sum[x >> 1], (uint32_t)c[i][x - 1] + e);
             }
     };
     if (whole) weigh(std::true_type{});
@@ -596,8 +597,8 @@ __global__ void __launch_bounds__(32 * TW, 2) k_tree_attention(const __grid_cons
         }
         meet();
         if (item + stride < items) ask(next, (item + stride) / tiles % a.n_kv, (item + stride) % tiles, true);
-        // Every block has added to the last item's O; it is read before the next meeting and cleared after it.
-        put();
+        // Every block has read O of the item before the last, whose place this item takes.
+        for (int i = tid; i < 16 * QUADS; i += TTHREADS) o_clear(o[count & 1], i / QUADS, i % QUADS);
         if (on) {
             // Lane l has row l % 16.
             int32_t e = m >= 0 ? INT32_MIN : INT32_MAX;
@@ -641,7 +642,6 @@ __global__ void __launch_bounds__(32 * TW, 2) k_tree_attention(const __grid_cons
             for (int i = 0; i < slices; i++) z += wsum[i][lane & 15];
             tree_planes<NT>(c, z, a.rule.P);
         }
-        for (int i = tid; i < 16 * QUADS; i += TTHREADS) o_clear(o[~count & 1], i / QUADS, i % QUADS);
         if (on) {
 #pragma unroll
             for (int j = 0; j < HD / 8; j++) {
@@ -652,6 +652,7 @@ __global__ void __launch_bounds__(32 * TW, 2) k_tree_attention(const __grid_cons
                 o_add(o[count & 1], j, x);
             }
         }
+        put();  // (all have added to the last item's O since this item's first meeting)
         last_item = Pending{s.first_row, kv, 16 * tile, min(rows, 16)};
         count++;
     }
