@@ -471,7 +471,8 @@ uint64_t hs_launch_count(void);
 
 /* Waits for `stream` and reports the first error that the device-resident operators of this handle
  * met on the device since the last check (HS_BAD_ARGUMENT for an entry that is not valid, HS_CUDA
- * for a failed launch), and clears it. */
+ * for a failed launch), and clears it. A stream that is being captured is refused (HS_BAD_ARGUMENT);
+ * its capture goes on. */
 int hs_dev_check(hs_dev* dev, void* stream);
 
 /* A KV cache as a batch keeps it: k [slots][planes][n_ctx][head_dim] and v, transposed,

@@ -147,7 +147,12 @@ int hs_dev_check(hs_dev* dev, void* stream) {
         DeviceScope on(d.ordinal);
         if (on.e != cudaSuccess) return cuda_fail("cudaSetDevice", on.e);
         cudaStream_t st = (cudaStream_t)stream;
-        cudaError_t e = cudaStreamSynchronize(st);
+        // A wait would end the capture with an error (the legacy stream is never one that captures).
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        cudaError_t e = st && st != cudaStreamLegacy ? cudaStreamIsCapturing(st, &cap) : cudaSuccess;
+        if (e != cudaSuccess) return cuda_fail("cudaStreamIsCapturing", e);
+        if (cap != cudaStreamCaptureStatusNone) return host_fail(HS_BAD_ARGUMENT, "the stream is being captured");
+        e = cudaStreamSynchronize(st);
         if (e != cudaSuccess) return cuda_fail("cudaStreamSynchronize", e);
         int code = 0;
         if ((e = cudaMemcpyAsync(&code, d.op_err, sizeof(int), cudaMemcpyDeviceToHost, st)) != cudaSuccess ||
@@ -226,6 +231,9 @@ int hs_op_tree_attention(hs_attn_rule* rule, const hs_tree_attention* a, void* s
         if (a->mask_words > 1024 || (uint64_t)a->mask_words * 32 < a->max_count)
             return host_fail(HS_BAD_ARGUMENT, "the mask has too few words for max_count nodes");
         if (a->n_seq > (1u << 20) || a->n_rows > (1u << 27)) return host_fail(HS_UNSUPPORTED, "too many trees or rows");
+        const uint64_t tiles = ((uint64_t)a->max_count * (a->n_head / a->n_kv_head) + 15) / 16;
+        if (a->n_seq * (uint64_t)a->n_kv_head * tiles > (1u << 30))
+            return host_fail(HS_UNSUPPORTED, "too many trees times heads");
         const uint64_t width = (uint64_t)a->n_head * a->cache.head_dim;
         t.q_stride = a->q_stride ? a->q_stride : width;
         t.out_stride = a->out_stride ? a->out_stride : width;

@@ -10,6 +10,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -691,7 +692,7 @@ int score_rule(const AttnRuleView& r, int hd) {
 template <int HD, int TW, int NT>
 struct TreeShape {
     static constexpr int KEYS = TW * NT * 8;  // of a block
-    static inline int fit[4] = {0, 0, 0, 0};
+    static inline std::atomic<int> fit[4];  // (host threads open their devices at once)
 
     static cudaError_t configure() {
         const void* fns[3] = {(const void*)k_tree_attention<HD, TW, NT, true, true>,
@@ -717,7 +718,7 @@ struct TreeShape {
         const int items = (int)a.n_seq * a.n_kv * tiles;
         int lg = 0;
         while (KEYS << lg < a.max_keys) lg++;
-        const int C = 1 << lg, clusters = fit[lg] > 0 ? fit[lg] : 1;
+        const int C = 1 << lg, found = fit[lg], clusters = found > 0 ? found : 1;
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)((items < clusters ? items : clusters) * C));
         cfg.blockDim = dim3(32 * TW);
@@ -748,8 +749,7 @@ struct TreeShape {
 // asks for its values; no warp waits to copy. One block per SM, 16 warps in two groups of 8 that take the
 // 16-row tiles of the head in turn, 128 keys a warp. The groups meet only within themselves, so one multiplies
 // while the other weighs.
-// The exponent table is held up to its last change (table_reach); a table that leaves no room for the rest
-// takes the kernel above, as do longer contexts.
+// The exponent table is held up to its last change (table_reach).
 
 constexpr int BK = 1024;                 // keys of a block
 constexpr int BWARPS = 16, GROUPS = 2;
@@ -1025,7 +1025,7 @@ cudaError_t launch_tree_attention(const TreeArgs& a, int num_sms, int* err, cuda
     if (vec && a.cache.hd == 64) {
         if (a.max_keys <= Short64::KEYS) return Short64::launch(a, err, st);
         // More than one tile a head, and K and V fit in a block.
-        if (a.max_keys <= BK && a.max_count * (a.n_head / a.n_kv) > 16 && bulk_smem(a.rule.reach) <= BLOCK_SMEM) {
+        if (a.max_keys <= BK && a.max_count * (a.n_head / a.n_kv) > 16) {
             const int rule = score_rule(a.rule, 64);
             return rule == 2   ? launch_bulk<true, true>(a, num_sms, err, st)
                    : rule == 1 ? launch_bulk<true, false>(a, num_sms, err, st)

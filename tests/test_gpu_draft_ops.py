@@ -699,3 +699,133 @@ def test_beam_weights_below_the_looked_up_bits(dev):
     check_beam(dev, c, 20)
     c["finished"] = np.array([1, 0])
     check_beam(dev, c, 20)
+
+
+# ---- the calls at the edges of what the documentation allows ----
+
+
+def tree_op(dev, c):
+    """The op of a case on new buffers, its outputs and the rule to close."""
+    rows, heads, hd = c["q"].shape
+    slots, planes = c["k"].shape[:2]
+    out = torch.full(c["q"].shape, 99, dtype=torch.int8, device="cuda")
+    h = B.AttnRule(dev, *(RULE[n] for n in ("score_m", "score_s", "out_m", "out_s", "P", "table")))
+    op = B.TreeAttention(h, B.KvCache(gpu(c["k"]), gpu(c["v"]), slots, planes, c["n_ctx"], hd), heads, c["kv"], gpu(c["q"]),
+                         out, rows, gpu(c["seqs"]), len(c["seqs"]), c["max_count"], c["max_keys"], gpu(c["mask"]),
+                         c["mask"].shape[1], c["plane0"])
+    torch.cuda.synchronize()
+    return op, out, h
+
+
+@pytest.mark.parametrize("counts,prefixes,n_ctx", [
+    ([33, 20, 40], [500, 900, 12], 1024),      # several tiles a head, one block
+    ([16, 9, 12], [500, 900, 300], 1024),      # one tile a head
+    ([40, 16, 20], [3000, 100, 1500], 4096)])  # clusters
+@pytest.mark.parametrize("bad", [0, 1, 2])
+@pytest.mark.parametrize("at,value", [(0, 1 << 20), (1, 41), (2, 3), (3, -1)])
+def test_tree_bad_record_keeps_its_rows_and_the_others_theirs(dev, counts, prefixes, n_ctx, bad, at, value):
+    c = tree_case(60, counts, prefixes, n_ctx, gap=1)
+    want = want_tree(c)
+    first, count = c["seqs"][bad, :2]
+    want[first:first + count] = 99
+    c["seqs"][bad, at] = value
+    op, out, h = tree_op(dev, c)
+    op.run(0)
+    with pytest.raises(B.HardShellError, match="a tree's rows"):
+        dev.check(0)
+    dev.check(0)
+    assert np.array_equal(out.cpu().numpy(), want)
+    h.close()
+
+
+@pytest.mark.parametrize("n_ctx,most", [(512, 40), (512, 16), (1040, 40)])
+def test_tree_works_that_follow_one_another(dev, n_ctx, most):
+    """More heads than the GPU has blocks: empty trees, heads of one tile and of several in every block's turn."""
+    r = np.random.default_rng(61)
+    counts = [0 if i % 5 == 4 else int(r.integers(1, most + 1)) for i in range(160)]
+    prefixes = [int(r.integers(0, n_ctx - most + 1)) for _ in counts]
+    prefixes[0], counts[0] = n_ctx - most, most
+    check_tree(dev, tree_case(61, counts, prefixes, n_ctx, heads=4, kv=4))
+
+
+def test_trees_of_one_slot(dev):
+    """Two drafts of one context: their records name one slot, and each sees its own nodes' cache rows."""
+    c = tree_case(62, [20, 20], [300, 300], 512, slots=2)
+    c["seqs"][:, 2] = 1
+    check_tree(dev, c)
+
+
+@pytest.mark.parametrize("counts,prefixes,n_ctx", [([40, 33], [500, 900], 1024), ([9, 16], [900, 20], 1024),
+                                                   ([31, 5], [3000, 10], 4096)])
+def test_two_tree_calls_at_once_and_replayed(dev, counts, prefixes, n_ctx):
+    """Two streams and two graphs run the operator at once: no state of one reaches the other."""
+    cases = [tree_case(63 + i, counts, prefixes, n_ctx) for i in range(2)]
+    ops = [tree_op(dev, c) for c in cases]
+    wants = [want_tree(c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in ops]
+    for _ in range(20):
+        for (op, _, _), st in zip(ops, streams):
+            op.run(st.cuda_stream)
+    for st in streams:
+        dev.check(st.cuda_stream)
+    graphs = []
+    for op, out, _ in ops:
+        assert np.array_equal(out.cpu().numpy(), wants[len(graphs)])
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            op.run(torch.cuda.current_stream().cuda_stream)
+        out.fill_(99)
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for (_, out, h), want in zip(ops, wants):
+        assert np.array_equal(out.cpu().numpy(), want)
+        h.close()
+    dev.check(0)
+
+
+def test_check_of_a_captured_stream_is_refused(dev):
+    c = tree_case(65, [5], [30], 64)
+    op, out, h = tree_op(dev, c)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        st = torch.cuda.current_stream().cuda_stream
+        op.run(st)
+        with pytest.raises(B.HardShellError, match="captured") as e:
+            dev.check(st)
+        assert e.value.code == B.HS_BAD_ARGUMENT
+    g.replay()
+    dev.check(0)
+    assert np.array_equal(out.cpu().numpy(), want_tree(c))
+    h.close()
+
+
+def test_tree_refuses_more_items_than_it_counts(dev):
+    buf = torch.zeros(64, dtype=torch.int32, device="cuda")
+    h = B.AttnRule(dev, *(RULE[n] for n in ("score_m", "score_s", "out_m", "out_s", "P", "table")))
+    op = B.TreeAttention(h, B.KvCache(buf, buf, 1, 4096, 16, 16), 4096, 4096, buf, buf, 1, buf, 1 << 20, 1, 16, buf, 1)
+    with pytest.raises(B.HardShellError, match="too many trees") as e:
+        op.run(0)
+    assert e.value.code == B.HS_UNSUPPORTED
+    h.close()
+
+
+def test_reorder_where_all_beams_take_one(dev):
+    """The same parent for every beam, its own among them."""
+    r = np.random.default_rng(66)
+    k = r.integers(-128, 128, (8, 3, 32, 64)).astype(np.int8)
+    v = r.integers(-128, 128, (8, 3, 64, 32)).astype(np.int8)
+    rows = np.full(8, 29, np.uint32)
+    parent = np.full(8, 5, np.uint32)
+    gk, gv = gpu(k), gpu(v)
+    op = B.CacheReorder(dev, B.KvCache(gk, gv, 8, 3, 32, 64), 1, 8, gpu(parent), gpu(rows))
+    op.run(0)
+    dev.check(0)
+    wk, wv = k.copy(), v.copy()
+    wk[:, :, :29] = k[5, :, :29]
+    wv[:, :, :, :29] = v[5, :, :, :29]
+    assert np.array_equal(gk.cpu().numpy(), wk) and np.array_equal(gv.cpu().numpy(), wv)
