@@ -18,6 +18,9 @@
 // look-ups take 32 bits, floor(table[j] / 2^s), so the sum is known to lie in [L 2^s, L 2^s + vocab (2^s -
 // 1)]. N does not decrease with W, so where both ends give one N it is exact; where they differ (W next to
 // a border) the low bits are summed as well.
+//
+// Measured (vocabulary 50257): 256 groups of 8 beams 99 us, a third of HBM's rate (212 MB of distances); 64
+// groups 31 us from L2, 39 us cold; one group of 4 beams 12 to 15 us, the latency of its six phases.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -458,7 +461,9 @@ cudaError_t launch_beam_select(const BeamArgs& a, int num_sms, cudaStream_t st) 
     if (a.groups == 0) return cudaSuccess;
     // The split: `segs` segments a row and clusters of C blocks, by the time of the segments of the busiest
     // block (a fixed part each, and one that grows with their symbols and with the blocks that share an SM)
-    // and of the end of a group.
+    // and of the end of a group. Measured: 256 groups of 8, one segment, C = 1, 2, 4, 8: 118, 99, 101, 101 us (two
+    // segments 134 at best); 64 groups of 8: 81, 46, 33, 31 us (42); one group of 4: 43, 25, 17, 17 us, two
+    // segments and C = 8 15 us, four 19 us. The rule takes the best of each, or one within 1 %.
     int C = 1;
     BeamShape sh = beam_shape(a, 1);
     double best = 1e300;

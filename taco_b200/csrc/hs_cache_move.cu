@@ -1,7 +1,7 @@
 // The moves of KV-cache rows: the reordering of the beams' states after a selection and the commit of
 // an accepted path of a draft tree. Both are in place: a thread owns the same bytes of every slot (or
 // row) that takes part, reads all of them before it writes any, so no order of threads matters.
-// Bytes in and out are the only cost.
+// Bytes in and out are the only cost (times: B200, 144 planes of 1,024 rows of 64).
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -19,7 +19,10 @@ constexpr int MOVE_THREADS = 256;
 // T: the unit of a move (16 bytes where n_ctx and head_dim are multiples of 16, else a byte). B: the
 // most beams of a group. blockIdx.y is the group, blockIdx.x a plane's keys (rows * hd bytes from row 0)
 // or values (the first `rows` bytes of each channel's row): a unit of values may pass the last row, and
-// then goes byte by byte.
+// then goes byte by byte. A thread's B loads in flight and the SM's room for them decide: 32 groups of 4
+// beams of 700 rows take 0.61 ms with B = 4 (5.4 TB/s in and out) and 1.24 ms with B = 32, one group of 8 at
+// 300 rows 29 and 35 us with B = 8 and 32; for 8 groups of 16 beams of 700 rows B = 16 took 1.87 ms (four
+// 64-register sets of loads an SM), B = 32 1.30 ms, so there is no kernel between 8 and 32.
 template <typename T, int B>
 __global__ void __launch_bounds__(MOVE_THREADS) k_cache_reorder(const CacheView c, const uint32_t* slots,
                                                                 const uint32_t* parents, const uint32_t* rows,
@@ -93,16 +96,16 @@ __global__ void __launch_bounds__(MOVE_THREADS) k_cache_reorder(const CacheView 
 // A warp moves parts of planes of one tree: a plane's keys (part 0) or some channels of its values.
 // path is strictly increasing, so path[j] >= j: taken in ascending runs, all of a run's rows read before
 // any is written, no row is written before it is read. The bytes of a path lie in a few 32-byte sectors of
-// each channel's row of values: that traffic is the cost (a lane takes a path's byte).
-constexpr int COMMIT_DEEP = 16, COMMIT_WARPS = 8, COMMIT_BLOCKS = 5;
-
-// The lanes that a channel of a path of m rows takes.
-__host__ __device__ inline int commit_width(uint32_t m) { return m <= 4 ? 4 : m <= 8 ? 8 : m <= 16 ? 16 : 32; }
+// each channel's row of values: that traffic is the cost. A lane takes a path's byte of COMMIT_DEEP channels,
+// all in flight: 64 trees with a path of 8 take 28 us with 32 channels and three blocks an SM, 32 with 16
+// channels and 36 with 64 (paths of 24 of 128 nodes 54, 58, 55 us); the sectors alone would be about 15 us. A
+// warp shared by several channels of short paths is no faster (35 us).
+constexpr int COMMIT_DEEP = 32, COMMIT_WARPS = 8, COMMIT_BLOCKS = 3;
 
 template <bool VEC>
 __global__ void __launch_bounds__(32 * COMMIT_WARPS, COMMIT_BLOCKS) k_cache_commit(const CacheView c, const TreeSeq* seqs,
                                                                    const uint32_t* path, const uint32_t* lengths,
-                                                                   uint32_t path_stride, int unit_ch, int parts, uint32_t units,
+                                                                   uint32_t path_stride, int parts, uint32_t units,
                                                                    int* err) {
     const int lane = threadIdx.x & 31;
     const uint32_t first = blockIdx.y * (uint32_t)COMMIT_WARPS + (threadIdx.x >> 5);  // unit of the tree
@@ -159,29 +162,21 @@ __global__ void __launch_bounds__(32 * COMMIT_WARPS, COMMIT_BLOCKS) k_cache_comm
             }
             continue;
         }
-        // Short paths share the warp between channels: `width` lanes of a channel.
-        const int ch0 = (int)(part - 1) * unit_ch, width = commit_width(m);
-        const int step = 32 / width, end = min(ch0 + unit_ch, c.hd);
+        const int ch0 = (int)(part - 1) * COMMIT_DEEP, n = min(COMMIT_DEEP, c.hd - ch0);
+        int8_t* V = c.v + base + (size_t)ch0 * c.n_ctx + s.prefix;
         for (uint32_t k0 = 0; k0 * 32 < m; k0++) {
-            const uint32_t pk = k0 == 0 ? p[0] : k0 == 1 ? p[1] : k0 == 2 ? p[2] : p[3];
-            const uint32_t j = 32 * k0 + lane % width, from = __shfl_sync(0xffffffffu, pk, lane % width);
-            const bool move = j < m && from != j;
-            const size_t next = (size_t)step * c.n_ctx;
-            for (int ch = ch0; ch < end; ch += COMMIT_DEEP * step) {
-                // This lane's channels ch + lane / width + q step.
-                const int mine = move ? (end - ch - lane / width + step - 1) / step : 0;
-                int8_t* V = c.v + base + (size_t)(ch + lane / width) * c.n_ctx + s.prefix;
-                const int8_t* of = V + from;
-                int8_t* to = V + j;
-                int8_t val[COMMIT_DEEP];
+            const uint32_t j = 32 * k0 + lane, from = k0 == 0 ? p[0] : k0 == 1 ? p[1] : k0 == 2 ? p[2] : p[3];
+            const int mine = j < m && from != j ? n : 0;
+            const int8_t* of = V + from;
+            int8_t* to = V + j;
+            int8_t val[COMMIT_DEEP];
 #pragma unroll
-                for (int q = 0; q < COMMIT_DEEP; q++, of += next)
-                    if (q < mine) val[q] = *of;
-                __syncwarp();
+            for (int q = 0; q < COMMIT_DEEP; q++, of += c.n_ctx)
+                if (q < mine) val[q] = *of;
+            __syncwarp();
 #pragma unroll
-                for (int q = 0; q < COMMIT_DEEP; q++, to += next)
-                    if (q < mine) *to = val[q];
-            }
+            for (int q = 0; q < COMMIT_DEEP; q++, to += c.n_ctx)
+                if (q < mine) *to = val[q];
             __syncwarp();
         }
     }
@@ -192,7 +187,6 @@ void reorder(const CacheView& c, const uint32_t* slots, const uint32_t* parents,
              uint32_t beams, dim3 grid, int* err, cudaStream_t st) {
     if (beams <= 4) k_cache_reorder<T, 4><<<grid, MOVE_THREADS, 0, st>>>(c, slots, parents, rows, groups, beams, err);
     else if (beams <= 8) k_cache_reorder<T, 8><<<grid, MOVE_THREADS, 0, st>>>(c, slots, parents, rows, groups, beams, err);
-    else if (beams <= 16) k_cache_reorder<T, 16><<<grid, MOVE_THREADS, 0, st>>>(c, slots, parents, rows, groups, beams, err);
     else k_cache_reorder<T, 32><<<grid, MOVE_THREADS, 0, st>>>(c, slots, parents, rows, groups, beams, err);
 }
 
@@ -203,7 +197,8 @@ cudaError_t launch_cache_reorder(const CacheView& c, const uint32_t* slots, cons
                                  cudaStream_t st) {
     if (groups == 0 || beams < 2) return cudaSuccess;
     // Blocks beyond one for each group and plane's keys or values: up to 16 for an SM, so that few groups
-    // have many loads in flight, each with at least two units a thread at a full context.
+    // have many loads in flight, each with at least two units a thread at a full context. One group of 8 beams
+    // of 300 rows: 29 us, 41 us without the parts.
     const uint64_t blocks = 2ull * c.planes * groups, full = (uint64_t)c.n_ctx * c.hd / (c.vec ? 16 : 1);
     uint64_t parts = (16ull * num_sms + blocks - 1) / blocks;
     const uint64_t most = (full + 2 * MOVE_THREADS - 1) / (2 * MOVE_THREADS);
@@ -215,17 +210,16 @@ cudaError_t launch_cache_reorder(const CacheView& c, const uint32_t* slots, cons
 }
 
 cudaError_t launch_cache_commit(const CacheView& c, const TreeSeq* seqs, const uint32_t* path, const uint32_t* lengths,
-                                uint32_t n_seq, uint32_t path_stride, int num_sms, int* err, cudaStream_t st) {
-    (void)num_sms;
+                                uint32_t n_seq, uint32_t path_stride, int* err, cudaStream_t st) {
     if (n_seq == 0) return cudaSuccess;
-    const int unit_ch = COMMIT_DEEP * (32 / commit_width(path_stride)), parts = 1 + (c.hd + unit_ch - 1) / unit_ch;
+    const int parts = 1 + (c.hd + COMMIT_DEEP - 1) / COMMIT_DEEP;
     const uint32_t units = c.planes * (uint32_t)parts;
     const uint32_t blocks = (units + COMMIT_WARPS - 1) / COMMIT_WARPS;
     const dim3 grid(n_seq, blocks < 65535u ? blocks : 65535u);
     if (c.vec)
-        k_cache_commit<true><<<grid, 32 * COMMIT_WARPS, 0, st>>>(c, seqs, path, lengths, path_stride, unit_ch, parts, units, err);
+        k_cache_commit<true><<<grid, 32 * COMMIT_WARPS, 0, st>>>(c, seqs, path, lengths, path_stride, parts, units, err);
     else
-        k_cache_commit<false><<<grid, 32 * COMMIT_WARPS, 0, st>>>(c, seqs, path, lengths, path_stride, unit_ch, parts, units, err);
+        k_cache_commit<false><<<grid, 32 * COMMIT_WARPS, 0, st>>>(c, seqs, path, lengths, path_stride, parts, units, err);
     return cudaGetLastError();
 }
 

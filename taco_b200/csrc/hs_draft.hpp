@@ -98,6 +98,6 @@ cudaError_t launch_cache_reorder(const CacheView& c, const uint32_t* slots, cons
                                  const uint32_t* rows, uint32_t groups, uint32_t beams, int num_sms, int* err,
                                  cudaStream_t st);
 cudaError_t launch_cache_commit(const CacheView& c, const TreeSeq* seqs, const uint32_t* path, const uint32_t* lengths,
-                                uint32_t n_seq, uint32_t path_stride, int num_sms, int* err, cudaStream_t st);
+                                uint32_t n_seq, uint32_t path_stride, int* err, cudaStream_t st);
 
 }  // namespace hs

@@ -377,7 +377,7 @@ int hs_op_cache_commit(hs_dev* dev, const hs_cache_commit* a, void* stream) {
         if (a->n_seq > a->cache.slots) return host_fail(HS_BAD_ARGUMENT, "more trees than the cache has slots");
         return launch(d.ordinal, stream, "the cache commit", [&](cudaStream_t st) {
             return launch_cache_commit(c, reinterpret_cast<const TreeSeq*>(a->seqs), a->path, a->lengths, a->n_seq,
-                                       a->path_stride, d.num_sms, d.op_err, st);
+                                       a->path_stride, d.op_err, st);
         });
     });
 }

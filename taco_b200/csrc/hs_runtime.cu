@@ -1587,7 +1587,7 @@ int tree_commit(hs_batch* b, uint32_t n, const uint32_t* nodes) {
         CK(cudaMemcpyAsync(d_len, lens.data(), sizeof(uint32_t) * lens.size(), cudaMemcpyHostToDevice, b->stream));
         ProfScope p(b, OP_CACHE_MOVE, 0);
         CK(launch_cache_commit(cache_of(b), b->d_tree_seqs, b->d_path, d_len, (uint32_t)seqs.size(), MAX_TREE,
-                               m->dev->num_sms, m->dev->d_err, b->stream));
+                               m->dev->d_err, b->stream));
     }
     for (const Accept& a : acc) {
         const uint32_t s = a.tree->slot;

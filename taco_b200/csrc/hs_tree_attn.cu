@@ -40,7 +40,8 @@ constexpr int ANY_THREADS = 128;
 
 // The kernel of every head width and alignment: one block per (row, head). Thread j takes the keys
 // j, j + 128, ... for the dots and the weights (kept in shared memory), then a warp takes a channel at
-// a time for the sum over the keys (V^T rows are contiguous).
+// a time for the sum over the keys (V^T rows are contiguous). Each row reads its keys again (from L2) and
+// multiplies byte by byte: it is bounded by that, not by HBM.
 __global__ void __launch_bounds__(ANY_THREADS) k_tree_attention_any(const TreeArgs a, int* err) {
     extern __shared__ __align__(16) uint32_t s_any[];  // [max_keys] dots, then e, then p; then q
     __shared__ int64_t red[ANY_THREADS / 32];
@@ -125,7 +126,14 @@ __global__ void __launch_bounds__(ANY_THREADS) k_tree_attention_any(const TreeAr
 //   S = Q K^T (mma m16n8k32, s8 x s8), the row maxima over the cluster, e and the row sums over the
 //   cluster, p = floor(e 2^P / sum) by an exact multiply-shift, p cut into four unsigned bytes, O += P V
 //   (u8 x s8) for each byte plane, the planes joined in 64 bits, O summed over warps and blocks.
-// Whole-number sums in any order: the split changes nothing.
+// Whole-number sums in any order: the split changes nothing. O is summed over a block's warps by additions in
+// shared memory (one word a lane and bank; parts of each warp, added up behind two more barriers, took 466 us
+// where this takes 405), and over a cluster's blocks when it is written, while the next item is under way.
+//
+// Bound: not HBM (23 % of it at 64 trees of 16 nodes and 1,024 keys, 51 us) but the integer work of a score (about
+// 25 instructions from the product to the probability's planes, one of them a table look-up in shared memory at
+// random banks) and the three latencies of an item that its warps meet at. 16 warps an SM are what 64 scores a
+// thread leave room for; 32 warps of 64 registers took 785 us where 16 of 128 took 560.
 //
 // Operands come straight from global memory in the layout of the fragments. The order of the channels in
 // a dot product is free, so thread t of a quad takes bytes 16 t .. 16 t + 15 of a key's row (and of the
@@ -748,7 +756,9 @@ struct TreeShape {
 // last warp that has made its scores of a head asks for the next head's keys, the last that has multiplied
 // asks for its values; no warp waits to copy. One block per SM, 16 warps in two groups of 8 that take the
 // 16-row tiles of the head in turn, 128 keys a warp. The groups meet only within themselves, so one multiplies
-// while the other weighs.
+// while the other weighs. At 256 trees of 64 nodes and 1,024 keys, 12 heads, 405 us: an SM issues 1.35
+// instructions a cycle (33 %), the tensor pipe is busy 19 %, the integer pipes 21 and 25 %; the warps wait for
+// one another's rows (22 %), for the next instruction's operands (20 %) and for first rows and masks (16 %).
 // The exponent table is held up to its last change (table_reach).
 
 constexpr int BK = 1024;                 // keys of a block
@@ -1010,7 +1020,11 @@ cudaError_t configure_bulk() {
     return cudaSuccess;
 }
 
-// Head width, warps, key tiles of a warp.
+// Head width, warps, key tiles of a warp. A warp that holds few keys leaves a short context to more warps: 256 keys a
+// block of 64-wide heads take 9.4 us (one tree of 8 at 200 keys, 12 heads) and 22.9 us (64 trees of 16 at 256),
+// 1,024 a block 12.9 and 31.2 us. Above that the longer slices win: 64 trees of 16 at 1,024 keys 50 us, 89 us in
+// clusters of four short blocks. Heads of 128, 512 or 1,024 keys a block: one tree of 8 at 512 keys 14.4 and 15.7
+// us, 64 of 16 at 512 keys 47 and 60 us, at 1,024 keys 95 (two blocks) and 85 us.
 using Short64 = TreeShape<64, 8, 4>;
 using Long64 = TreeShape<64, 8, 16>;
 using Short128 = TreeShape<128, 8, 8>;
@@ -1024,7 +1038,10 @@ cudaError_t launch_tree_attention(const TreeArgs& a, int num_sms, int* err, cuda
                      a.rule.tlen <= ATTN_TABLE_MAX;
     if (vec && a.cache.hd == 64) {
         if (a.max_keys <= Short64::KEYS) return Short64::launch(a, err, st);
-        // More than one tile a head, and K and V fit in a block.
+        // More than one tile a head, and K and V fit in a block: 64 trees of 31 nodes at 1,024 keys take 74 us, 84 by
+        // the kernel without copies, 256 trees of 64 nodes 405 and 558 us. One tile reads K and V once anyway: 64
+        // trees of 16 nodes 60 us with the copies, 50 without. (In clusters, for longer contexts, they lose: 8 trees
+        // of 31 at 8,192 keys 138 us, 111 without.)
         if (a.max_keys <= BK && a.max_count * (a.n_head / a.n_kv) > 16) {
             const int rule = score_rule(a.rule, 64);
             return rule == 2   ? launch_bulk<true, true>(a, num_sms, err, st)
