@@ -463,7 +463,7 @@ cudaError_t launch_beam_select(const BeamArgs& a, int num_sms, cudaStream_t st) 
     // block (a fixed part each, and one that grows with their symbols and with the blocks that share an SM)
     // and of the end of a group. Measured: 256 groups of 8, one segment, C = 1, 2, 4, 8: 118, 99, 101, 101 us (two
     // segments 134 at best); 64 groups of 8: 81, 46, 33, 31 us (42); one group of 4: 43, 25, 17, 17 us, two
-    // segments and C = 8 15 us, four 19 us. The rule takes the best of each, or one within 1 %.
+    // segments and C = 8 15 us, four 19 us; one lone beam 17 us whole, 11 us in eight segments. The rule takes the best of each, or one within 1 %.
     int C = 1;
     BeamShape sh = beam_shape(a, 1);
     double best = 1e300;

@@ -4,6 +4,7 @@
 // Bytes in and out are the only cost (times: B200, 144 planes of 1,024 rows of 64).
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <type_traits>
 
@@ -14,22 +15,48 @@ namespace hs {
 
 namespace {
 
-constexpr int MOVE_THREADS = 256;
+// Threads of a block of the kernel for B beams: 32 loads of 16 bytes a thread want more registers than 256
+// threads have (8 groups of 16 beams of 700 rows by the kernel for 32: 1.17 ms, 0.66 with 128 threads; the
+// kernel for 16 0.59, and with 128 threads 0.60, that for 4 0.58 against 0.56).
+__host__ __device__ constexpr int move_threads(int B) { return B > 16 ? 128 : 256; }
+
+// The first n bytes (1 to 15) of a unit, in a store for each bit of n.
+__device__ __forceinline__ void put_head(int8_t* to, uint4 v, uint32_t n) {
+    uint32_t a = v.x, b = v.y;
+    if (n & 8) {
+        *reinterpret_cast<uint2*>(to) = make_uint2(v.x, v.y);
+        to += 8;
+        a = v.z;
+        b = v.w;
+    }
+    if (n & 4) {
+        *reinterpret_cast<uint32_t*>(to) = a;
+        to += 4;
+        a = b;
+    }
+    if (n & 2) {
+        *reinterpret_cast<uint16_t*>(to) = (uint16_t)a;
+        to += 2;
+        a >>= 16;
+    }
+    if (n & 1) *to = (int8_t)a;
+}
 
 // T: the unit of a move (16 bytes where n_ctx and head_dim are multiples of 16, else a byte). B: the
 // most beams of a group. blockIdx.y is the group, blockIdx.x a plane's keys (rows * hd bytes from row 0)
 // or values (the first `rows` bytes of each channel's row): a unit of values may pass the last row, and
-// then goes byte by byte. A thread's B loads in flight and the SM's room for them decide: 32 groups of 4
-// beams of 700 rows take 0.61 ms with B = 4 (5.4 TB/s in and out) and 1.24 ms with B = 32, one group of 8 at
-// 300 rows 29 and 35 us with B = 8 and 32; for 8 groups of 16 beams of 700 rows B = 16 took 1.87 ms (four
-// 64-register sets of loads an SM), B = 32 1.30 ms, so there is no kernel between 8 and 32.
+// then goes by parts (byte by byte one group of 8 beams of 300 rows took 30 us, by parts 20).
+//
+// Bound by HBM: 32 groups of 4 beams of 700 rows take 0.56 ms (5.9 TB/s in and out, 90 % of a copy's rate), 16 of
+// 8 0.57, 8 of 16 0.59. The loads of beams that a group does not have cost: the kernel for 32 takes 1.2 ms with
+// groups of 4, so there is one for 4, 8, 16 and 32.
 template <typename T, int B>
-__global__ void __launch_bounds__(MOVE_THREADS) k_cache_reorder(const CacheView c, const uint32_t* slots,
+__global__ void __launch_bounds__(move_threads(B)) k_cache_reorder(const CacheView c, const uint32_t* slots,
                                                                 const uint32_t* parents, const uint32_t* rows,
                                                                 uint32_t groups, uint32_t beams, int* err) {
     __shared__ uint32_t s_dst[B], s_src[B], s_rows[B];  // the moves of the group: slots, and the rows moved
     __shared__ uint32_t s_n, s_most, s_bad;
-    constexpr int W = (int)sizeof(T);
+    constexpr int W = (int)sizeof(T), MOVE_THREADS = move_threads(B);
     for (uint32_t g = blockIdx.y; g < groups; g += gridDim.y) {
         __syncthreads();
         if (threadIdx.x < 32) {
@@ -85,8 +112,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) k_cache_reorder(const CacheView 
                     *reinterpret_cast<T*>(to) = val[j];
                 } else {
                     // The last rows of a channel's values end inside the unit.
-                    const int8_t* bytes = reinterpret_cast<const int8_t*>(&val[j]);
-                    for (uint32_t i = 0; i < s_rows[j] - x; i++) to[i] = bytes[i];
+                    if constexpr (W == 16) put_head(to, val[j], s_rows[j] - x);
                 }
             }
         }
@@ -182,12 +208,26 @@ __global__ void __launch_bounds__(32 * COMMIT_WARPS, COMMIT_BLOCKS) k_cache_comm
     }
 }
 
-template <typename T>
+template <typename T, int B>
 void reorder(const CacheView& c, const uint32_t* slots, const uint32_t* parents, const uint32_t* rows, uint32_t groups,
-             uint32_t beams, dim3 grid, int* err, cudaStream_t st) {
-    if (beams <= 4) k_cache_reorder<T, 4><<<grid, MOVE_THREADS, 0, st>>>(c, slots, parents, rows, groups, beams, err);
-    else if (beams <= 8) k_cache_reorder<T, 8><<<grid, MOVE_THREADS, 0, st>>>(c, slots, parents, rows, groups, beams, err);
-    else k_cache_reorder<T, 32><<<grid, MOVE_THREADS, 0, st>>>(c, slots, parents, rows, groups, beams, err);
+             uint32_t beams, int num_sms, int* err, cudaStream_t st) {
+    // Blocks beyond one for each group and plane's keys or values: up to 6 for an SM, so that few groups have
+    // many loads in flight, each with at least two units a thread at a full context. One group of 4 beams of 300
+    // rows in L2: 9.1 us; 10.2 without the parts, 10.5 with up to 16 for an SM (8: 14.8, 14.7, 16.7).
+    const uint64_t blocks = 2ull * c.planes * groups, full = (uint64_t)c.n_ctx * c.hd / sizeof(T);
+    const uint64_t most = (full + 2 * move_threads(B) - 1) / (2 * move_threads(B));
+    const uint64_t parts = std::min<uint64_t>({(6ull * num_sms + blocks - 1) / blocks, most, 64});
+    const dim3 grid(2 * c.planes, groups < 65535u ? groups : 65535u, (unsigned)parts);
+    k_cache_reorder<T, B><<<grid, move_threads(B), 0, st>>>(c, slots, parents, rows, groups, beams, err);
+}
+
+template <typename T>
+void reorder_any(const CacheView& c, const uint32_t* slots, const uint32_t* parents, const uint32_t* rows, uint32_t groups,
+                 uint32_t beams, int num_sms, int* err, cudaStream_t st) {
+    if (beams <= 4) reorder<T, 4>(c, slots, parents, rows, groups, beams, num_sms, err, st);
+    else if (beams <= 8) reorder<T, 8>(c, slots, parents, rows, groups, beams, num_sms, err, st);
+    else if (beams <= 16) reorder<T, 16>(c, slots, parents, rows, groups, beams, num_sms, err, st);
+    else reorder<T, 32>(c, slots, parents, rows, groups, beams, num_sms, err, st);
 }
 
 }  // namespace
@@ -196,16 +236,8 @@ cudaError_t launch_cache_reorder(const CacheView& c, const uint32_t* slots, cons
                                  const uint32_t* rows, uint32_t groups, uint32_t beams, int num_sms, int* err,
                                  cudaStream_t st) {
     if (groups == 0 || beams < 2) return cudaSuccess;
-    // Blocks beyond one for each group and plane's keys or values: up to 16 for an SM, so that few groups
-    // have many loads in flight, each with at least two units a thread at a full context. One group of 8 beams
-    // of 300 rows: 29 us, 41 us without the parts.
-    const uint64_t blocks = 2ull * c.planes * groups, full = (uint64_t)c.n_ctx * c.hd / (c.vec ? 16 : 1);
-    uint64_t parts = (16ull * num_sms + blocks - 1) / blocks;
-    const uint64_t most = (full + 2 * MOVE_THREADS - 1) / (2 * MOVE_THREADS);
-    parts = parts < most ? parts : most;
-    const dim3 grid(2 * c.planes, groups < 65535u ? groups : 65535u, (unsigned)(parts < 64 ? parts : 64));
-    if (c.vec) reorder<uint4>(c, slots, parents, rows, groups, beams, grid, err, st);
-    else reorder<uint8_t>(c, slots, parents, rows, groups, beams, grid, err, st);
+    if (c.vec) reorder_any<uint4>(c, slots, parents, rows, groups, beams, num_sms, err, st);
+    else reorder_any<uint8_t>(c, slots, parents, rows, groups, beams, num_sms, err, st);
     return cudaGetLastError();
 }
 

@@ -829,3 +829,22 @@ def test_reorder_where_all_beams_take_one(dev):
     wk[:, :, :29] = k[5, :, :29]
     wv[:, :, :, :29] = v[5, :, :, :29]
     assert np.array_equal(gk.cpu().numpy(), wk) and np.array_equal(gv.cpu().numpy(), wv)
+
+
+def test_reorder_of_every_length(dev):
+    """Rows that end at every byte of a 16-byte unit; the bytes behind them stay."""
+    n, beams = 48, 3
+    r = np.random.default_rng(67)
+    k = r.integers(-128, 128, (n * beams, 2, 48, 16)).astype(np.int8)
+    v = r.integers(-128, 128, (n * beams, 2, 16, 48)).astype(np.int8)
+    rows = np.repeat(np.arange(1, n + 1), beams).astype(np.uint32)
+    parent = np.tile([1, 2, 1], n).astype(np.uint32)
+    gk, gv = gpu(k), gpu(v)
+    B.CacheReorder(dev, B.KvCache(gk, gv, n * beams, 2, 48, 16), n, beams, gpu(parent), gpu(rows)).run(0)
+    dev.check(0)
+    wk, wv = k.copy(), v.copy()
+    for g in range(n):
+        for j in range(beams):
+            to, of, m = g * beams + j, g * beams + parent[g * beams + j], g + 1
+            wk[to, :, :m], wv[to, :, :, :m] = k[of, :, :m], v[of, :, :, :m]
+    assert np.array_equal(gk.cpu().numpy(), wk) and np.array_equal(gv.cpu().numpy(), wv)
