@@ -85,6 +85,11 @@ __device__ __forceinline__ int64_t warp_max8(int64_t v) {  // over lanes 0..7 (a
     return v;
 }
 
+// The cluster barrier in two halves, each by all threads of all blocks. Nothing written before it is read behind
+// it, so the arrival orders no memory.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
+
 // VEC: rows of 16-byte vectors; else symbol by symbol. One cluster per group.
 template <bool VEC>
 __global__ void __launch_bounds__(BT, BEAM_BLOCKS) k_beam_select(const __grid_constant__ BeamArgs a,
@@ -92,6 +97,9 @@ __global__ void __launch_bounds__(BT, BEAM_BLOCKS) k_beam_select(const __grid_co
     extern __shared__ __align__(16) uint8_t s_beam[];
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    // No block writes to the first one's shared memory before that one runs: all arrive here and wait behind
+    // the loads below (the cluster's other meeting is the one before the merge).
+    if (C > 1) cluster_arrive();
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
     const int last = a.tlen - 1, tiles = (a.vocab + (1 << a.tsh) - 1) >> a.tsh;
     const uint32_t keep = (uint32_t)a.keep, no_symbol = (uint32_t)a.tlen;
@@ -136,6 +144,7 @@ __global__ void __launch_bounds__(BT, BEAM_BLOCKS) k_beam_select(const __grid_co
     ahead(rank);
     for (int i = tid; i <= a.tlen / 4; i += BT)
         reinterpret_cast<uint4*>(sT)[i] = __ldg(reinterpret_cast<const uint4*>(a.high) + i);
+    if (C > 1) cluster_wait();
 
     for (int item = rank; item < items; item += C) {
         const int b = item / sh.segs, seg = item % sh.segs;
