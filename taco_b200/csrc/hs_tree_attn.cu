@@ -771,6 +771,8 @@ struct __align__(16) TreeBulk {
     uint8_t v[64 * VROW];
     uint64_t k_full, v_full;
     uint32_t k_done, v_done;             // warps that need this head's keys (values) no more
+    uint32_t k_asked, v_asked;           // copies asked for so far
+    uint32_t gave_up;                    // the code of a wait of this block that ran out
 };
 // Behind it: the groups' O [GROUPS][16 * 64][2] i32, the warps' wsum [BWARPS][16] u64 and wmax [BWARPS][16] i32,
 // and the table.
@@ -780,8 +782,21 @@ constexpr size_t bulk_smem(int reach) {
 constexpr size_t BLOCK_SMEM = 227 * 1024;
 static_assert(bulk_smem(ATTN_TABLE_MAX) <= BLOCK_SMEM, "room for every table");
 
-// A wait that gives up sets the error word and lets its thread go on: every barrier still gets its arrivals,
-// every later wait returns at once, and the call's results count for nothing.
+// A wait for a block's copy, of at most `polls` tries. It ends early only after another wait of the block ran out
+// (gave_up is then not 0; null: it does not): the error word may hold a refused record, of this call or of an
+// earlier one, which is no reason to read keys that have not arrived.
+__device__ __forceinline__ bool copy_wait(uint64_t* bar, uint32_t phase, const uint32_t* gave_up, uint32_t polls) {
+    for (uint32_t i = 0; i < polls; i++) {
+        if (mbar_try_wait(bar, phase)) return true;
+        if (i > 64) __nanosleep(32);
+        if (gave_up && *(const volatile uint32_t*)gave_up) break;
+    }
+    return false;
+}
+
+// A wait that gives up notes its code and lets its thread go on: every barrier still gets its arrivals, every later
+// wait returns at once, no further copy is asked for, and the call's results count for nothing. The block then sets
+// the error word and waits (again with a limit) for the copies under way before it ends.
 template <bool NARROW, bool SSHI>
 __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __grid_constant__ TreeArgs a, int works,
                                                                      int* err) {
@@ -808,7 +823,7 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
     if (tid == 0) {
         mbar_init(&sm.k_full, 1);
         mbar_init(&sm.v_full, 1);
-        sm.k_done = sm.v_done = 0;
+        sm.k_done = sm.v_done = sm.k_asked = sm.v_asked = sm.gave_up = 0;
         fence_barrier_init();
     }
     for (int i = tid; i < (a.rule.reach + 3) / 4; i += BTHREADS)
@@ -818,6 +833,7 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
 
     // The copies of the keys (values) of the first work from `work` on that has rows, by one warp.
     auto copy = [&](int work, bool values) {
+        if (*(volatile uint32_t*)&sm.gave_up) return;
         for (; work < works; work += stride) {
             const TreeSeq s = a.seqs[work / a.n_kv];
             if (!tree_seq_ok(s, a.n_rows, a.cache.slots, a.max_count, a.max_keys) || s.count == 0) continue;
@@ -826,11 +842,15 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
                                  (size_t)(a.plane0 + work % a.n_kv) * ((size_t)a.cache.n_ctx * HD);
             if (values) {
                 const uint32_t bytes = (uint32_t)(n + 15) & ~15u;  // (n_ctx % 16 == 0)
-                if (lane == 0) mbar_arrive_expect_tx(&sm.v_full, bytes * HD);
+                if (lane == 0) {
+                    sm.v_asked++;
+                    mbar_arrive_expect_tx(&sm.v_full, bytes * HD);
+                }
                 __syncwarp();
                 for (int ch = lane; ch < HD; ch += 32)
                     bulk_load(sm.v + ch * VROW, a.cache.v + plane + (size_t)ch * a.cache.n_ctx, bytes, &sm.v_full);
             } else if (lane == 0) {
+                sm.k_asked++;
                 mbar_arrive_expect_tx(&sm.k_full, (uint32_t)n * HD);
                 bulk_load(sm.k, a.cache.k + plane, (uint32_t)n * HD, &sm.k_full);
             }
@@ -839,6 +859,9 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
     };
     if (warp == 0) copy(first, false);
     if (warp == 1) copy(first, true);
+    auto wait = [&](uint64_t* bar, uint32_t phase, uint32_t code) {
+        if (!copy_wait(bar, phase, &sm.gave_up, 1u << 26)) *(volatile uint32_t*)&sm.gave_up = code;
+    };
     // This warp has read the keys (values) of `work`: the last one asks for the next.
     auto done = [&](int work, bool values) {
         __syncwarp();
@@ -932,7 +955,7 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
                                                                           : bits & ((1u << left) - 1u);
                 }
             }
-            if (tile == grp) mbar_wait(&sm.k_full, phase, err, 55);
+            if (tile == grp) wait(&sm.k_full, phase, 55);
             if (on) {
                 const uint4* kp = reinterpret_cast<const uint4*>(ks + ((g >> 1) * TK + (g & 1)) * HD) + t;
 #pragma unroll
@@ -969,7 +992,7 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
                 for (int i = 0; i < slices; i++) z += wsum[i][lane & 15];
                 tree_planes<NT>(c, z, a.rule.P);
             }
-            if (tile == grp) mbar_wait(&sm.v_full, phase, err, 56);
+            if (tile == grp) wait(&sm.v_full, phase, 56);
             if (on) {
 #pragma unroll
                 for (int j = 0; j < HD / 8; j++) {
@@ -993,14 +1016,21 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
         if (grp >= tiles) {
             // No tile for this group: the copies are not needed, but each is waited for, so that the counts are
             // this head's.
-            mbar_wait(&sm.k_full, phase, err, 55);
+            wait(&sm.k_full, phase, 55);
             done(work, false);
-            mbar_wait(&sm.v_full, phase, err, 56);
+            wait(&sm.v_full, phase, 56);
             done(work, true);
         }
     }
     group_bar();
     put();
+    __syncthreads();
+    if (tid == 0 && sm.gave_up) {
+        atomicCAS(err, 0, (int)sm.gave_up);
+        // (else every copy has been waited for; copy n completes phase n - 1 of its barrier)
+        if (sm.k_asked) copy_wait(&sm.k_full, (sm.k_asked - 1) & 1, nullptr, 1u << 22);
+        if (sm.v_asked) copy_wait(&sm.v_full, (sm.v_asked - 1) & 1, nullptr, 1u << 22);
+    }
 }
 
 template <bool NARROW, bool SSHI>

@@ -9,10 +9,69 @@ import pytest
 
 import tests.draft_ref as R
 from taco_b200 import backend as B
-from tests.test_gpu_draft_ops import beam_case, dev, gpu  # noqa: F401  (dev: the fixture)
+from tests.test_gpu_draft_ops import beam_case, dev, gpu, tree_case, tree_op, want_tree  # noqa: F401  (dev: the fixture)
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
+
+
+# ---- tree attention ----
+
+
+def bad_reorder(dev):
+    """A call whose parent is out of range: it sets the handle's error word and moves nothing."""
+    z = torch.zeros((2, 1, 16, 16), dtype=torch.int8, device="cuda")
+    ids = torch.tensor([1, 9], dtype=torch.int32, device="cuda")
+    B.CacheReorder(dev, B.KvCache(z, z.clone(), 2, 1, 16, 16), 1, 2, ids, torch.zeros_like(ids)).run()
+
+
+def many_trees(seed, n, most, n_ctx, heads):
+    """More (tree, head) pairs than the GPU has blocks."""
+    r = np.random.default_rng(seed)
+    counts = [int(x) for x in r.integers(1, most + 1, n)]
+    counts[0] = most
+    prefixes = [int(r.integers(n_ctx // 2, n_ctx - most + 1)) for _ in counts]
+    prefixes[0] = n_ctx - most
+    return tree_case(seed, counts, prefixes, n_ctx, heads=heads, kv=heads)
+
+
+@pytest.mark.parametrize("n,most,n_ctx,heads", [(45, 20, 512, 4), (15, 20, 1024, 12), (15, 20, 1040, 12), (45, 16, 512, 4)])
+def test_trees_beside_an_unreported_error(dev, n, most, n_ctx, heads):
+    """An error that nobody has asked about yet changes nothing for later calls on the handle."""
+    c = many_trees(71, n, most, n_ctx, heads)
+    op, out, h = tree_op(dev, c)
+    bad_reorder(dev)
+    want = want_tree(c)
+    for _ in range(5):
+        out.fill_(99)
+        op.run(0)
+        torch.cuda.synchronize()
+        assert np.array_equal(out.cpu().numpy(), want)
+    with pytest.raises(B.HardShellError, match="a beam's parent"):
+        dev.check()
+    dev.check()
+    h.close()
+
+
+@pytest.mark.parametrize("n,most,n_ctx,heads", [(45, 20, 512, 4), (15, 20, 1024, 12), (45, 16, 512, 4)])
+def test_bad_records_among_more_trees_than_blocks(dev, n, most, n_ctx, heads):
+    """Records that are not valid, the first among them: every other tree has its outputs."""
+    c = many_trees(72, n, most, n_ctx, heads)
+    want = want_tree(c)
+    for i in (0, n // 3, n - 1):
+        first, count = c["seqs"][i, :2]
+        want[first:first + count] = 99
+        c["seqs"][i, 2] = n  # no such slot
+    op, out, h = tree_op(dev, c)
+    for _ in range(5):
+        out.fill_(99)
+        op.run(0)
+        torch.cuda.synchronize()
+        assert np.array_equal(out.cpu().numpy(), want)
+    with pytest.raises(B.HardShellError, match="a tree's rows"):
+        dev.check()
+    dev.check()
+    h.close()
 
 
 # ---- beam selection ----
