@@ -543,11 +543,11 @@ void hs_weight_rule_free(hs_weight_rule* rule);
  * then the lower symbol first among equal costs: parent (the beam), token and cost of
  * [groups][keep]. finished (may be NULL): a beam whose byte is not 0 keeps its place as one
  * candidate of cost base and token HS_NO_TOKEN, and its logits are not read. A beam whose base is
- * negative or at least 2^62 has no candidates. With fewer than `keep` candidates the rest of
- * parent and token is HS_NO_TOKEN, of cost -1. The strides count elements (0: dense rows of vocab
- * symbols and of its tiles); dist must be 16-byte aligned and dist_stride a multiple of 8 for the
- * vector loads, else it is read by symbols. vocab * table[0] < 2^64, vocab 2 to 65536, beams at
- * most HS_MAX_BEAMS, keep at most HS_MAX_KEEP. */
+ * negative or at least 2^62 has no candidates, and its logits are not read either. With fewer than
+ * `keep` candidates the rest of parent and token is HS_NO_TOKEN, of cost -1. The strides count
+ * elements (0: dense rows of vocab symbols and of its tiles); dist must be 16-byte aligned and
+ * dist_stride a multiple of 8 for the vector loads, else it is read by symbols. vocab * table[0] <
+ * 2^64, vocab 2 to 65536, beams at most HS_MAX_BEAMS, keep at most HS_MAX_KEEP. */
 typedef struct hs_beam_select {
     const uint16_t* dist;
     const int64_t* tops;

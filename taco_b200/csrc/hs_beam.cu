@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(BT, BEAM_BLOCKS) k_beam_select(const __grid_co
         const uint16_t* dist = a.dist + lrow * a.dist_stride;
         const int64_t* tops = a.tops + lrow * a.tops_stride;
         const int v0 = seg * sh.seg_vecs, v1 = min(v0 + sh.seg_vecs, vecs);
+        const bool fetch = VEC && tid == 0 && item + C < items && state_of((item + C) / sh.segs) == 1;
         for (int o = 16; o > 0; o >>= 1) {
             const int64_t x = __shfl_xor_sync(0xffffffffu, part, o);
             part = x > part ? x : part;
@@ -179,8 +180,8 @@ __global__ void __launch_bounds__(BT, BEAM_BLOCKS) k_beam_select(const __grid_co
             if (seg == 0) *cl.map_shared_rank(&sm.top[b], 0) = mx;
         }
         __syncthreads();
-        // The next segment on its way into L2.
-        if (VEC && tid == 0 && item + C < items) {
+        // The next segment on its way into L2, if its beam has logits (those of the others may not be there).
+        if (fetch) {
             const int f0 = (item + C) % sh.segs * sh.seg_vecs, f1 = min(f0 + sh.seg_vecs, whole);
             if (f1 > f0)
                 asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(

@@ -102,3 +102,31 @@ def test_beams_that_take_no_time(dev, alive, groups, vocab):
         for got, x in zip(o, want):
             assert np.array_equal(got.cpu().numpy(), x)
     rule.close()
+
+
+@pytest.mark.parametrize("ended", [0, 1])
+@pytest.mark.parametrize("vocab,beams,alive", [(50257, 16, 8), (3000, 32, 5), (1024, 20, 1)])
+def test_the_logits_of_dead_and_finished_beams_need_not_be_there(dev, ended, vocab, beams, alive):
+    """The last beams of the last group have ended (or are dead), and the distances end, with their allocation,
+    at the last living beam's."""
+    c = beam_case(73, 1, beams, vocab)
+    c["finished"] = np.where(np.arange(beams) < alive, 0, 1) if ended else None
+    c["base"][alive:] = 77 if ended else -1
+    want = R.beam_select(c["dist"], c["tops"], 7, vocab, beams, beams, c["base"], c["finished"], c["table"])
+    ld = c["dist"].shape[1]
+    whole = torch.zeros(16 << 20, dtype=torch.int16, device="cuda")  # an allocation of its own
+    dist = whole[whole.numel() - alive * ld:].view(alive, ld)
+    dist.copy_(gpu(c["dist"][:alive]))
+    rule = B.WeightRule(dev, c["table"])
+    parent, token = (torch.zeros((1, beams), dtype=torch.int32, device="cuda") for _ in range(2))
+    cost = torch.zeros((1, beams), dtype=torch.int64, device="cuda")
+    fin = None if c["finished"] is None else gpu(c["finished"], np.uint8)
+    op = B.BeamSelect(rule, dist.data_ptr(), gpu(c["tops"]), vocab, 1, beams, beams, gpu(c["base"]), parent, token, cost,
+                      fin, ld, c["tops"].shape[1])
+    torch.cuda.synchronize()
+    for _ in range(3):
+        op.run(0)
+    dev.check()
+    for got, x in zip((parent, token, cost), want):
+        assert np.array_equal(got.cpu().numpy(), x)
+    rule.close()
