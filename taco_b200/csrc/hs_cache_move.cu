@@ -136,23 +136,22 @@ __global__ void __launch_bounds__(32 * COMMIT_WARPS, COMMIT_BLOCKS) k_cache_comm
     const int lane = threadIdx.x & 31;
     const uint32_t first = blockIdx.y * (uint32_t)COMMIT_WARPS + (threadIdx.x >> 5);  // unit of the tree
     const uint32_t i = blockIdx.x;
-    // Lane l holds the path's entries l, l + 32, ...; the ones past its end stay where they are.
-    uint32_t p[MAX_TREE / 32];
-#pragma unroll
-    for (int k = 0; k < MAX_TREE / 32; k++) {
-        const uint32_t j = 32 * k + lane;
-        p[k] = j < path_stride ? path[(size_t)i * path_stride + j] : j;  // with the record and the length
-    }
     const TreeSeq s = seqs[i];
     const uint32_t m = lengths[i];
     bool bad = m > path_stride || m > s.count || s.count > (uint32_t)MAX_TREE || s.slot >= c.slots ||
                s.prefix > (uint32_t)c.n_ctx || s.count > (uint32_t)c.n_ctx - s.prefix;
+    // Lane l holds the path's entries l, l + 32, ...; the ones past its end are not read, and stay where they are.
+    uint32_t p[MAX_TREE / 32];
     uint32_t before = 0;  // the last entry of the run before, plus one
     if (!bad) {
 #pragma unroll
         for (int k = 0; k < MAX_TREE / 32; k++) {
             const uint32_t j = 32 * k + lane;
-            p[k] = j < m ? p[k] : j;
+            p[k] = j < m ? path[(size_t)i * path_stride + j] : j;
+        }
+#pragma unroll
+        for (int k = 0; k < MAX_TREE / 32; k++) {
+            const uint32_t j = 32 * k + lane;
             uint32_t up = __shfl_up_sync(0xffffffffu, p[k], 1);
             if (lane == 0) up = before - 1;
             bad = bad || (j < m && (p[k] >= s.count || (j > 0 && p[k] <= up)));

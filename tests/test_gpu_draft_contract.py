@@ -130,3 +130,31 @@ def test_the_logits_of_dead_and_finished_beams_need_not_be_there(dev, ended, voc
     for got, x in zip((parent, token, cost), want):
         assert np.array_equal(got.cpu().numpy(), x)
     rule.close()
+
+
+# ---- moves of cache rows ----
+
+
+@pytest.mark.parametrize("length", [3, 1, 40])
+@pytest.mark.parametrize("n_ctx,hd", [(64, 16), (50, 20)])
+def test_a_path_is_read_to_its_length(dev, length, n_ctx, hd):
+    """path[i * path_stride + 0 .. lengths[i] - 1] is all there is: the last path's row, and with it the
+    allocation, ends at its last entry."""
+    r = np.random.default_rng(length)
+    n, stride = 3, 128
+    k = r.integers(-128, 128, (n, 2, n_ctx, hd)).astype(np.int8)
+    v = r.integers(-128, 128, (n, 2, hd, n_ctx)).astype(np.int8)
+    seqs = np.array([[0, 20, 2, 4], [20, 44, 0, 5], [64, 44, 1, 0]])
+    lengths = np.array([0, 30, length])
+    path = np.zeros((n, stride), np.int64)
+    for i in range(n):
+        path[i, :lengths[i]] = np.sort(r.permutation(seqs[i, 1])[:lengths[i]])
+    want = R.commit(k, v, seqs, path, lengths)
+    size = (n - 1) * stride + length
+    whole = torch.zeros(8 << 20, dtype=torch.int32, device="cuda")
+    whole[whole.numel() - size:] = gpu(path, np.int32).view(-1)[:size]
+    dk, dv = gpu(k), gpu(v)
+    B.CacheCommit(dev, B.KvCache(dk, dv, n, 2, n_ctx, hd), gpu(seqs, np.int32), n,
+                  whole.data_ptr() + 4 * (whole.numel() - size), stride, gpu(lengths, np.int32)).run()
+    dev.check()
+    assert np.array_equal(dk.cpu().numpy(), want[0]) and np.array_equal(dv.cpu().numpy(), want[1])
