@@ -76,6 +76,13 @@ int need_device(const void* p, int ordinal, const char* name) {
     return HS_OK;
 }
 
+// A table into device memory. The copy from pageable memory may return before its last part has arrived, so the
+// call waits: the caller's stream may use the rule at once.
+cudaError_t put_table(void* to, const void* of, size_t bytes) {
+    const cudaError_t e = cudaMemcpy(to, of, bytes, cudaMemcpyHostToDevice);
+    return e != cudaSuccess ? e : cudaStreamSynchronize(cudaStreamLegacy);
+}
+
 int need_aligned(const void* p, size_t to, const char* name) {
     if (reinterpret_cast<uintptr_t>(p) % to != 0)
         return host_fail(HS_BAD_ARGUMENT, std::string(name) + " is not aligned to " + std::to_string(to) + " bytes");
@@ -191,10 +198,10 @@ int hs_attn_rule_new(hs_dev* dev, int32_t score_m, uint32_t score_s, int32_t out
         t.resize((t.size() + 3) & ~(size_t)3, 0);
         cudaError_t e = cudaMalloc(&r->table, 4 * t.size());
         if (e != cudaSuccess) return cuda_fail("cudaMalloc", e);
-        e = cudaMemcpy(r->table, t.data(), 4 * t.size(), cudaMemcpyHostToDevice);
+        e = put_table(r->table, t.data(), 4 * t.size());
         if (e != cudaSuccess) {
             cudaFree(r->table);
-            return cuda_fail("cudaMemcpy", e);
+            return cuda_fail("the copy of the table", e);
         }
         r->view = AttnRuleView{score_m, out_m, (int)score_s, (int)out_s, (int)softmax_p, (int)table_len, r->table,
                                table_reach(exp_table, (int)table_len)};
@@ -279,10 +286,10 @@ int hs_weight_rule_new(hs_dev* dev, const uint64_t* table, uint32_t table_len, h
         cudaError_t e = cudaMalloc(&r->table, bytes + 4 * high.size());
         if (e != cudaSuccess) return cuda_fail("cudaMalloc", e);
         r->high = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(r->table) + bytes);
-        if ((e = cudaMemcpy(r->table, table, 8 * (size_t)table_len, cudaMemcpyHostToDevice)) != cudaSuccess ||
-            (e = cudaMemcpy(r->high, high.data(), 4 * high.size(), cudaMemcpyHostToDevice)) != cudaSuccess) {
+        if ((e = put_table(r->table, table, 8 * (size_t)table_len)) != cudaSuccess ||
+            (e = put_table(r->high, high.data(), 4 * high.size())) != cudaSuccess) {
             cudaFree(r->table);
-            return cuda_fail("cudaMemcpy", e);
+            return cuda_fail("the copy of the table", e);
         }
         *out = r.release();
         return HS_OK;

@@ -127,13 +127,22 @@ int make_store_tmap(hs_dev* dev, CUtensorMap* tm, const void* base, CUtensorMapD
     return HS_OK;
 }
 
+// Waits for the legacy stream: a memset there, or the last part of a copy from pageable memory, may still run when
+// its call returns, and the batches' and the callers' streams do not wait for it.
+int settle() {
+    CK(cudaStreamSynchronize(cudaStreamLegacy));
+    return HS_OK;
+}
+
 template <typename T>
 int dalloc(T** p, size_t count, std::vector<void*>& owned) {
     void* q = nullptr;
     size_t bytes = std::max<size_t>(count * sizeof(T), 16);
     CK(cudaMalloc(&q, bytes));
-    CK(cudaMemset(q, 0, bytes));
     owned.push_back(q);
+    CK(cudaMemset(q, 0, bytes));
+    int rc = settle();
+    if (rc) return rc;
     *p = (T*)q;
     return HS_OK;
 }
@@ -141,9 +150,9 @@ int dalloc(T** p, size_t count, std::vector<void*>& owned) {
 template <typename T>
 int upload(T** p, const T* src, size_t count, std::vector<void*>& owned) {
     int rc = dalloc(p, count, owned);
-    if (rc) return rc;
-    if (count) CK(cudaMemcpy(*p, src, count * sizeof(T), cudaMemcpyHostToDevice));
-    return HS_OK;
+    if (rc || count == 0) return rc;
+    CK(cudaMemcpy(*p, src, count * sizeof(T), cudaMemcpyHostToDevice));
+    return settle();
 }
 
 struct DevLinear {
@@ -1839,6 +1848,8 @@ int hs_open(int ordinal, hs_dev** out) {
     d->encode = (EncodeTiledFn)fn;
     CK(cudaMalloc(&d->d_err, 2 * sizeof(int)));
     CK(cudaMemset(d->d_err, 0, 2 * sizeof(int)));
+    int rc = settle();
+    if (rc) return rc;
     d->d_op_err = d->d_err + 1;
     CK(configure_core_kernels());
     CK(configure_tc_kernels());
