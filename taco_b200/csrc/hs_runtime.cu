@@ -1628,6 +1628,7 @@ int beam_step(hs_batch* b, uint32_t groups, uint32_t beams, uint32_t* slots, uin
     std::vector<char> seen(b->slots, 0);
     std::vector<uint32_t> row_of(n, 0);
     uint32_t R = 0;
+    auto ran = [&](uint32_t i) { return costs[i] >= 0 && !(finished && finished[i]); };
     for (uint32_t i = 0; i < n; i++) {
         const uint32_t s = slots[i];
         if (s >= (uint32_t)b->slots)
@@ -1636,7 +1637,7 @@ int beam_step(hs_batch* b, uint32_t groups, uint32_t beams, uint32_t* slots, uin
         if (seen[s]) return fail(HS_BAD_ARGUMENT, "two beams in one slot");
         seen[s] = 1;
         if (costs[i] >= (1LL << 62)) return fail(HS_BAD_ARGUMENT, "a beam's cost is 2^62 or more");
-        if (costs[i] < 0 || (finished && finished[i])) continue;
+        if (!ran(i)) continue;
         if (tokens[i] >= (uint32_t)c.V)
             return fail(HS_TOKEN_RANGE, "token " + std::to_string(tokens[i]) + " is not in the vocabulary of " +
                                             std::to_string(c.V) + " tokens");
@@ -1659,10 +1660,9 @@ int beam_step(hs_batch* b, uint32_t groups, uint32_t beams, uint32_t* slots, uin
     b->tree.clear();
     uint32_t *d_row_of = b->d_beam_u32, *d_slots = d_row_of + Rc, *d_parent = d_slots + Rc, *d_token = d_parent + Rc,
              *d_held = d_token + Rc;
-    std::vector<uint32_t> row_pos(n, 0);
     if (R) {
         for (uint32_t i = 0; i < n; i++) {
-            if (costs[i] < 0 || (finished && finished[i])) continue;
+            if (!ran(i)) continue;
             StreamSt& ss = b->streams[slots[i]];
             ss.written = std::max(ss.written, (uint32_t)b->pos[slots[i]] + 1);
             b->h_rows[row_of[i]] = RowInfo{slots[i], tokens[i], (uint32_t)b->pos[slots[i]], 0, 0};
@@ -1712,14 +1712,6 @@ int beam_step(hs_batch* b, uint32_t groups, uint32_t beams, uint32_t* slots, uin
     CK(cudaMemcpyAsync(cost.data(), a.cost, sizeof(int64_t) * n, cudaMemcpyDeviceToHost, b->stream));
     if ((rc = check_device_error(b))) return rc;
     if (b->profiling) prof_collect(b);
-    // The inputs of this step, in the slots that ran.
-    for (uint32_t i = 0; i < n; i++) {
-        if (costs[i] < 0 || (finished && finished[i])) continue;
-        const uint32_t s = slots[i];
-        b->hist[(size_t)s * c.n_ctx + b->pos[s]] = tokens[i];
-        b->pos[s]++;
-        b->streams[s].len++;
-    }
     // The slots of the new beams, and the copies (moves[p]: the place whose state place p takes).
     std::vector<uint32_t> new_slots(n), moves(n), held(n);
     bool any = false;
@@ -1729,7 +1721,7 @@ int beam_step(hs_batch* b, uint32_t groups, uint32_t beams, uint32_t* slots, uin
         std::vector<char> kept(beams, 0);
         for (uint32_t j = 0; j < beams; j++) {
             moves[o + j] = j;
-            held[o + j] = (uint32_t)b->pos[slots[o + j]];
+            held[o + j] = (uint32_t)b->pos[slots[o + j]] + (ran(o + j) ? 1 : 0);
             const uint32_t p = par[o + j];
             if (p < beams && !kept[p]) {
                 kept[p] = 1;
@@ -1757,6 +1749,14 @@ int beam_step(hs_batch* b, uint32_t groups, uint32_t beams, uint32_t* slots, uin
         ProfScope p(b, OP_CACHE_MOVE, 0);
         CK(launch_cache_reorder(cache_of(b), d_slots, d_parent, d_held, groups, beams, m->dev->num_sms,
                                 m->dev->d_err, b->stream));
+    }
+    // Nothing fails from here on. The inputs of this step, in the slots that ran, then the states that follow.
+    for (uint32_t i = 0; i < n; i++) {
+        if (!ran(i)) continue;
+        const uint32_t s = slots[i];
+        b->hist[(size_t)s * c.n_ctx + b->pos[s]] = tokens[i];
+        b->pos[s]++;
+        b->streams[s].len++;
     }
     for (uint32_t i = 0; i < n; i++) {
         const uint32_t dst = slots[i], src = slots[i / beams * beams + moves[i]];

@@ -63,3 +63,83 @@ def test_a_batch_uses_no_buffer_that_is_being_cleared(fake):
     """Buffers are cleared on the legacy stream and used on the batch's own, the ones made by a first tree pass or beam
     step too."""
     there(fake, batches_whose_buffers_are_ready)
+
+
+# ---- errors of a batch ----
+
+
+def beam_steps_that_fail():
+    rt = fake_cuda.Runtime()
+    batch = B.CudaBatch(B.CudaModel(B.CudaDevice(0), tiny_bytes()), 6, 64)
+
+    def step():
+        return batch.beam_step(1, 3, [4, 0, 2], [5, 6, 7], [3, -1, 9], [0, 0, 1])
+
+    def state():
+        return [(batch.position(s), batch.stream_len(s)) for s in range(6)]
+
+    batch.run_coded([4, 4, 2], [1, 2, 3], [0] * 3, [1, 2, 3])
+    batch.run_coded([4] * 4, [1] * 4, [0] * 4, [1] * 4)
+    # (all new beams come from the first one, as kernels that do nothing leave it: the others get copies)
+    rt.clear()
+    before = state()
+    assert before[4] == (6, 6) and before[2] == (1, 1)
+    whole = step()
+    after = state()
+    assert after == [(7, 7), (0, 0), (7, 7), (0, 0), (7, 7), (0, 0)] and whole[0].tolist() == [4, 0, 2]
+    calls = rt.calls()
+    reorder = next(c for c in calls if "cache_reorder" in c)
+    for s in range(6):
+        batch.reset(s)
+    batch.run_coded([4, 4, 2], [1, 2, 3], [0] * 3, [1, 2, 3])
+    batch.run_coded([4] * 4, [1] * 4, [0] * 4, [1] * 4)
+    assert state() == before
+    for name in ("cudaMemcpyAsync", "cudaMemcpy", "cudaStreamSynchronize", reorder):
+        for at in range(calls.count(name) if name != "cudaStreamSynchronize" else 1):
+            rt.clear()
+            rt.fail(name, at)
+            with pytest.raises(B.HardShellError) as e:
+                step()
+            assert e.value.code == B.HS_CUDA, (name, at)
+            rt.clear()
+            assert state() == before, (name, at)
+    assert [x.tolist() for x in step()] == [x.tolist() for x in whole] and state() == after
+
+
+def test_a_beam_step_that_fails_changes_nothing(fake):
+    """Every copy, wait and the cache move of a step fail once: the positions, streams, slots and tokens stay, and the
+    step can be made again."""
+    there(fake, beam_steps_that_fail)
+
+
+def tree_commits_that_fail():
+    rt = fake_cuda.Runtime()
+    batch = B.CudaBatch(B.CudaModel(B.CudaDevice(0), tiny_bytes()), 3, 64)
+    path = [0, 2, 3, 5, 6]
+
+    def trees():
+        for s in range(3):
+            batch.reset(s)
+        batch.run_coded([0] * 5, [1] * 5, [0] * 5, [1] * 5)
+        batch.run_tree([0] * 4 + [2] * 3, [1] * 7, [-1, 0, 0, 2, -1, -1, 5])
+        rt.clear()
+
+    trees()
+    batch.tree_commit(path)
+    calls = rt.calls()
+    assert (batch.position(0), batch.position(2)) == (8, 2)
+    trees()
+    for name in {c for c in calls if c.startswith(("cudaMemcpy", "launch"))}:
+        for at in range(calls.count(name)):
+            rt.clear()
+            rt.fail(name, at)
+            with pytest.raises(B.HardShellError):
+                batch.tree_commit(path)
+            assert (batch.position(0), batch.position(2)) == (5, 0) == (batch.stream_len(0), batch.stream_len(2))
+    rt.clear()
+    batch.tree_commit(path)
+    assert (batch.position(0), batch.position(2)) == (8, 2)
+
+
+def test_a_tree_commit_that_fails_changes_nothing(fake):
+    there(fake, tree_commits_that_fail)
