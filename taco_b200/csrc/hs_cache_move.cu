@@ -234,7 +234,7 @@ void reorder_any(const CacheView& c, const uint32_t* slots, const uint32_t* pare
 cudaError_t launch_cache_reorder(const CacheView& c, const uint32_t* slots, const uint32_t* parents,
                                  const uint32_t* rows, uint32_t groups, uint32_t beams, int num_sms, int* err,
                                  cudaStream_t st) {
-    if (groups == 0 || beams < 2) return cudaSuccess;
+    if (groups == 0 || beams == 0) return cudaSuccess;  // (one beam: nothing moves, but its parent is checked)
     if (c.vec) reorder_any<uint4>(c, slots, parents, rows, groups, beams, num_sms, err, st);
     else reorder_any<uint8_t>(c, slots, parents, rows, groups, beams, num_sms, err, st);
     return cudaGetLastError();

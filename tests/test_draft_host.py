@@ -143,3 +143,24 @@ def tree_commits_that_fail():
 
 def test_a_tree_commit_that_fails_changes_nothing(fake):
     there(fake, tree_commits_that_fail)
+
+
+# ---- launches of the device-resident operators ----
+
+
+def reorders_of_one_beam():
+    rt = fake_cuda.Runtime()
+    dev = B.CudaDevice(0)
+    k, v = (fake_cuda.Tensor(rt, (2, 1, 16, 16), "int8") for _ in range(2))
+    ids = fake_cuda.Tensor(rt, (2,), "int32")
+    for groups, beams in ((2, 1), (1, 2)):
+        rt.clear()
+        before = B.launch_count()
+        B.CacheReorder(dev, B.KvCache(k, v, 2, 1, 16, 16), groups, beams, ids, ids).run()
+        assert len(rt.launches()) == 1 == B.launch_count() - before
+
+
+def test_a_reorder_of_one_beam_is_checked_by_its_kernel(fake):
+    """Groups of one beam have nothing to move, but a parent out of range is reported: the launch is made, as it is
+    counted."""
+    there(fake, reorders_of_one_beam)

@@ -158,3 +158,21 @@ def test_a_path_is_read_to_its_length(dev, length, n_ctx, hd):
                   whole.data_ptr() + 4 * (whole.numel() - size), stride, gpu(lengths, np.int32)).run()
     dev.check()
     assert np.array_equal(dk.cpu().numpy(), want[0]) and np.array_equal(dv.cpu().numpy(), want[1])
+
+
+@pytest.mark.parametrize("parents,fault", [([0, -1, 0], False), ([0, 5, 0], True), ([1, 0, 0], True)])
+def test_reorder_of_lone_beams(dev, parents, fault):
+    """Groups of one beam: nothing moves, and a parent out of range is an error as in any group."""
+    r = np.random.default_rng(74)
+    k = r.integers(-128, 128, (3, 2, 32, 16)).astype(np.int8)
+    v = r.integers(-128, 128, (3, 2, 16, 32)).astype(np.int8)
+    dk, dv = gpu(k), gpu(v)
+    before = B.launch_count()
+    B.CacheReorder(dev, B.KvCache(dk, dv, 3, 2, 32, 16), 3, 1, gpu(np.array(parents), np.int32),
+                   gpu(np.array([4, 5, 6]), np.int32)).run()
+    assert B.launch_count() == before + 1
+    if fault:
+        with pytest.raises(B.HardShellError, match="a beam's parent"):
+            dev.check()
+    dev.check()
+    assert np.array_equal(dk.cpu().numpy(), k) and np.array_equal(dv.cpu().numpy(), v)
