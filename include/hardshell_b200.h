@@ -467,7 +467,9 @@ uint64_t hs_launch_count(void);
  *
  * What only the device knows (sequence records, parents, paths) is checked by the kernels: an
  * entry that is not valid is left out, its outputs as they were, and sets an error word that
- * hs_dev_check reports. All results are whole numbers, the same for every split of the work. */
+ * hs_dev_check reports. All results are whole numbers, the same for every split of the work.
+ *
+ * hs_op_..._check makes the host's checks of a call alone: what the call would refuse, and no launch. */
 
 /* Waits for `stream` and reports the first error that the device-resident operators of this handle
  * met on the device since the last check (HS_BAD_ARGUMENT for an entry that is not valid, HS_CUDA
@@ -522,6 +524,7 @@ typedef struct hs_tree_attention {
     uint32_t plane0, n_head, n_kv_head, n_rows, n_seq, max_count, max_keys, mask_words;
 } hs_tree_attention;
 int hs_op_tree_attention(hs_attn_rule* rule, const hs_tree_attention* args, void* stream);
+int hs_op_tree_attention_check(const hs_attn_rule* rule, const hs_tree_attention* args);
 
 /* The logits-to-weights table of a model (crates/hardshell/src/logits.rs:62-72): 1 to 16384 weights
  * by distance from the row's largest logit, not increasing, the first not 0; copied. */
@@ -560,6 +563,7 @@ typedef struct hs_beam_select {
     uint32_t tile_shift, vocab, groups, beams, keep, reserved;
 } hs_beam_select;
 int hs_op_beam_select(hs_weight_rule* rule, const hs_beam_select* args, void* stream);
+int hs_op_beam_select_check(const hs_weight_rule* rule, const hs_beam_select* args);
 
 /* The reordering of the beams' states after a selection, in place: beam j of group g has the cache
  * slot slots[g * beams + j] (NULL: slot g * beams + j; the slots of a call must be distinct) and
@@ -574,6 +578,7 @@ typedef struct hs_cache_reorder {
     uint32_t groups, beams;
 } hs_cache_reorder;
 int hs_op_cache_reorder(hs_dev* dev, const hs_cache_reorder* args, void* stream);
+int hs_op_cache_reorder_check(hs_dev* dev, const hs_cache_reorder* args);
 
 /* The commit of an accepted path, in place: with the nodes path[i * path_stride + 0 ..
  * lengths[i] - 1] of tree seqs[i], strictly increasing and below its count, cache row prefix +
@@ -587,6 +592,7 @@ typedef struct hs_cache_commit {
     uint32_t n_seq, path_stride;
 } hs_cache_commit;
 int hs_op_cache_commit(hs_dev* dev, const hs_cache_commit* args, void* stream);
+int hs_op_cache_commit_check(hs_dev* dev, const hs_cache_commit* args);
 
 /* ---- op-level entry points: the kernels alone, for tests and measurements ----
  * (the reference's op-level path, crates/hardshell-cuda/src/batch/record.rs, and its GEMM tests,

@@ -218,6 +218,10 @@ def lib() -> ctypes.CDLL:
     L.hs_op_beam_select.argtypes = [vp, ctypes.POINTER(BeamSelectArgs), vp]
     L.hs_op_cache_reorder.argtypes = [vp, ctypes.POINTER(CacheReorderArgs), vp]
     L.hs_op_cache_commit.argtypes = [vp, ctypes.POINTER(CacheCommitArgs), vp]
+    L.hs_op_tree_attention_check.argtypes = [vp, ctypes.POINTER(TreeAttentionArgs)]
+    L.hs_op_beam_select_check.argtypes = [vp, ctypes.POINTER(BeamSelectArgs)]
+    L.hs_op_cache_reorder_check.argtypes = [vp, ctypes.POINTER(CacheReorderArgs)]
+    L.hs_op_cache_commit_check.argtypes = [vp, ctypes.POINTER(CacheCommitArgs)]
     L.hs_batch_set_profiling.argtypes = [vp, i32]
     L.hs_batch_profile.argtypes = [vp, vp, i32]
     L.hs_launch_count.argtypes = []
@@ -890,7 +894,9 @@ class CudaBatch:
 # Arguments are device addresses or tensors of the device (anything with data_ptr()); an operator
 # object holds them, and run(stream) launches it on a CUDA stream (its address; 0 is the legacy
 # default stream). The objects keep their tensors alive. CudaDevice.check(stream) waits and raises the
-# errors that the kernels met.
+# errors that the kernels met. The first run() looks the tensors over: their type, and whether the
+# elements that the call may touch are in them, laid out as it takes them (a view of a larger tensor may
+# be, with its stride given). An address is taken as it is.
 
 NO_TOKEN = 0xFFFFFFFF
 MAX_TREE, MAX_BEAMS, MAX_KEEP = 128, 32, 64
@@ -939,6 +945,52 @@ class WeightRule(_Rule):
         device._children.add(self)
 
 
+def _runs(x):
+    """The memory of a tensor as [elements, stride] from the innermost run outwards, axes that follow one another
+    joined."""
+    out = []
+    for n, s in zip(reversed(tuple(x.shape)), reversed(tuple(x.stride()))):
+        if n == 1:
+            continue
+        if out and s == out[-1][0] * out[-1][1]:
+            out[-1][0] *= n
+        else:
+            out.append([int(n), int(s)])
+    return out or [[int(x.numel()), 1]]
+
+
+def _row_stride(x) -> int:
+    """The elements from a row of a tensor to the next, along its last axis but one (0: an address or a lone row)."""
+    if not hasattr(x, "stride") or len(x.shape) < 2:
+        return 0
+    runs = _runs(x)
+    return runs[1][1] if len(runs) > 1 else int(x.shape[-1])
+
+
+I8, U8, U16, U32, I64 = ("int8",), ("uint8", "int8", "bool"), ("uint16", "int16"), ("uint32", "int32"), ("int64",)
+
+
+def _look(name: str, x, dtypes, rows: int, width: int, stride: int = 0, tail=None):
+    """Raises unless tensor x has `rows` runs of `width` elements, `stride` apart (0: `width`), of one of `dtypes`.
+    tail: its last axes, if it has all of them (four)."""
+    if not (hasattr(x, "dtype") and hasattr(x, "stride")) or rows <= 0 or width <= 0:
+        return
+    stride = stride or width
+    dtype = str(x.dtype).rsplit(".", 1)[-1]
+    if dtype not in dtypes:
+        raise HardShellError(HS_BAD_ARGUMENT, f"{name} is of {dtype}, the call takes {dtypes[0]}")
+    if tail and len(x.shape) == 4 and tuple(x.shape[2:]) != tail:
+        raise HardShellError(HS_BAD_ARGUMENT, f"{name} has rows of {tuple(x.shape[2:])}, the call takes {tail}")
+    runs = _runs(x)
+    n, s = runs[0]
+    if s == 1 and n >= (rows - 1) * stride + width:
+        return
+    if s == 1 and len(runs) == 2 and n >= width and runs[1][0] >= rows and runs[1][1] == stride:
+        return
+    raise HardShellError(HS_BAD_ARGUMENT, f"{name} of shape {tuple(x.shape)} and strides {tuple(x.stride())} does not hold "
+                                          f"{rows} rows of {width} elements, {stride} apart")
+
+
 class KvCache:
     """hs_kv_cache: keys [slots, planes, n_ctx, head_dim] and values [slots, planes, head_dim, n_ctx]."""
 
@@ -946,59 +998,93 @@ class KvCache:
         self.keep = (k, v)
         self.args = KvCacheArgs(_ptr(k), _ptr(v), slot_stride, slots, planes, n_ctx, head_dim)
 
+    def looks(self):
+        a, (k, v) = self.args, self.keep
+        size = a.planes * a.n_ctx * a.head_dim
+        return [("cache.k", k, I8, a.slots, size, a.slot_stride, (a.n_ctx, a.head_dim)),
+                ("cache.v", v, I8, a.slots, size, a.slot_stride, (a.head_dim, a.n_ctx))]
+
 
 class _DeviceOp:
-    """One bound call of a device-resident operator."""
+    """One bound call of a device-resident operator. looks: the _look arguments of its tensors."""
 
-    def __init__(self, name: str, handle, args, keep):
+    def __init__(self, name: str, handle, args, keep, looks):
         self._fn, self._handle, self._args, self._keep = getattr(lib(), name), handle, args, keep
+        self._check_fn, self._looks = getattr(lib(), name + "_check"), looks
         self._ref = ctypes.byref(args)
+
+    def _first(self):
+        """The library's checks, then the tensors'."""
+        _check(self._check_fn(self._handle.h, self._ref))
+        for look in self._looks:
+            _look(*look)
+        self._looks = None
 
     def run(self, stream: int = 0):
         if not self._handle.h:
             raise HardShellError(HS_BAD_ARGUMENT, "the handle is closed")
+        if self._looks is not None:
+            self._first()
         rc = self._fn(self._handle.h, self._ref, stream)
         if rc:
             _check(rc)
 
 
 class TreeAttention(_DeviceOp):
-    """hs_op_tree_attention."""
+    """hs_op_tree_attention. q and out [rows, heads, head_dim], seqs [n_seq, 4], mask [rows, mask_words]."""
 
     def __init__(self, rule: AttnRule, cache: KvCache, heads: int, kv_heads: int, q, out, rows: int, seqs, n_seq: int,
                  max_count: int, max_keys: int, mask, mask_words: int, plane0: int = 0, q_stride: int = 0,
                  out_stride: int = 0):
         args = TreeAttentionArgs(cache.args, _ptr(q), _ptr(out), q_stride, out_stride, _ptr(seqs), _ptr(mask), plane0,
                                  heads, kv_heads, rows, n_seq, max_count, max_keys, mask_words)
-        super().__init__("hs_op_tree_attention", rule, args, (cache, q, out, seqs, mask))
+        width = heads * cache.args.head_dim
+        super().__init__("hs_op_tree_attention", rule, args, (cache, q, out, seqs, mask),
+                         [] if 0 in (n_seq, rows, max_count) else
+                         cache.looks() + [("q", q, I8, rows, width, q_stride), ("out", out, I8, rows, width, out_stride),
+                                          ("seqs", seqs, U32, n_seq, 4), ("mask", mask, U32, rows, mask_words)])
 
 
 class BeamSelect(_DeviceOp):
-    """hs_op_beam_select."""
+    """hs_op_beam_select. dist [groups * beams, >= vocab] and tops [groups * beams, >= tiles] (their strides are the
+    tensors' own), base and finished [groups * beams], parent, token and cost [groups, keep]."""
 
     def __init__(self, rule: WeightRule, dist, tops, vocab: int, groups: int, beams: int, keep: int, base, parent,
                  token, cost, finished=None, dist_stride: int | None = None, tops_stride: int | None = None,
                  tile_shift: int = 7):
         if dist_stride is None:
-            dist_stride = dist.stride(0) if hasattr(dist, "stride") else 0
+            dist_stride = _row_stride(dist)
         if tops_stride is None:
-            tops_stride = tops.stride(0) if hasattr(tops, "stride") else 0
+            tops_stride = _row_stride(tops)
         args = BeamSelectArgs(_ptr(dist), _ptr(tops), dist_stride, tops_stride, _ptr(base), _ptr(finished),
                               _ptr(parent), _ptr(token), _ptr(cost), tile_shift, vocab, groups, beams, keep, 0)
-        super().__init__("hs_op_beam_select", rule, args, (dist, tops, base, finished, parent, token, cost))
+        n, out = groups * beams, groups * keep
+        super().__init__("hs_op_beam_select", rule, args, (dist, tops, base, finished, parent, token, cost),
+                         [] if out == 0 else
+                         [("dist", dist, U16, n, vocab, dist_stride),
+                          ("tops", tops, I64, n, -(-vocab >> tile_shift) if tile_shift >= 0 else 0, tops_stride),
+                          ("base", base, I64, 1, n), ("finished", finished, U8, 1, n), ("parent", parent, U32, 1, out),
+                          ("token", token, U32, 1, out), ("cost", cost, I64, 1, out)])
 
 
 class CacheReorder(_DeviceOp):
-    """hs_op_cache_reorder."""
+    """hs_op_cache_reorder. parent, rows and slots [groups, beams]."""
 
     def __init__(self, device: CudaDevice, cache: KvCache, groups: int, beams: int, parent, rows, slots=None):
         args = CacheReorderArgs(cache.args, _ptr(slots), _ptr(parent), _ptr(rows), groups, beams)
-        super().__init__("hs_op_cache_reorder", device, args, (cache, slots, parent, rows))
+        n = groups * beams
+        super().__init__("hs_op_cache_reorder", device, args, (cache, slots, parent, rows),
+                         [] if n == 0 else
+                         cache.looks() + [("parent", parent, U32, 1, n), ("rows", rows, U32, 1, n),
+                                          ("slots", slots, U32, 1, n)])
 
 
 class CacheCommit(_DeviceOp):
-    """hs_op_cache_commit."""
+    """hs_op_cache_commit. seqs [n_seq, 4], path [n_seq, path_ld], length [n_seq]."""
 
     def __init__(self, device: CudaDevice, cache: KvCache, seqs, n_seq: int, path, path_ld: int, length):
         args = CacheCommitArgs(cache.args, _ptr(seqs), _ptr(path), _ptr(length), n_seq, path_ld)
-        super().__init__("hs_op_cache_commit", device, args, (cache, seqs, path, length))
+        super().__init__("hs_op_cache_commit", device, args, (cache, seqs, path, length),
+                         [] if n_seq == 0 else
+                         cache.looks() + [("seqs", seqs, U32, n_seq, 4), ("path", path, U32, n_seq, path_ld),
+                                          ("length", length, U32, 1, n_seq)])

@@ -141,6 +141,124 @@ int launch(int ordinal, void* stream, const char* what, F&& f) {
     return HS_OK;
 }
 
+// The checks of a call and the arguments of its launch. A call with nothing to do leaves `out` as it is: without
+// trees, groups or beams.
+int tree_args(const hs_attn_rule* rule, const hs_tree_attention* a, TreeArgs* out) {
+    const int o = rule->dev.ordinal;
+    if (a->n_seq == 0 || a->n_rows == 0 || a->max_count == 0) return HS_OK;
+    TreeArgs t{};
+    int rc;
+    if ((rc = cache_view(a->cache, o, &t.cache)) || (rc = need_array(a->q, o, "q")) ||
+        (rc = need_array(a->out, o, "out")) || (rc = need_array(a->seqs, o, "seqs")) ||
+        (rc = need_array(a->mask, o, "mask")))
+        return rc;
+    if (a->n_head == 0 || a->n_head > 65535 || a->n_kv_head == 0 || a->n_head % a->n_kv_head != 0)
+        return host_fail(HS_UNSUPPORTED, "n_head must be a multiple of n_kv_head");
+    if (a->plane0 > a->cache.planes || a->n_kv_head > a->cache.planes - a->plane0)
+        return host_fail(HS_BAD_ARGUMENT, "the layer's planes lie outside the cache");
+    if (a->max_count > HS_MAX_TREE) return host_fail(HS_UNSUPPORTED, "a tree has at most 128 nodes");
+    if (a->max_keys == 0 || a->max_keys > a->cache.n_ctx || a->max_count > a->max_keys)
+        return host_fail(HS_BAD_ARGUMENT, "max_keys must be max_count to n_ctx");
+    if (a->mask_words > 1024 || (uint64_t)a->mask_words * 32 < a->max_count)
+        return host_fail(HS_BAD_ARGUMENT, "the mask has too few words for max_count nodes");
+    if (a->n_seq > (1u << 20) || a->n_rows > (1u << 27)) return host_fail(HS_UNSUPPORTED, "too many trees or rows");
+    const uint64_t tiles = ((uint64_t)a->max_count * (a->n_head / a->n_kv_head) + 15) / 16;
+    if (a->n_seq * (uint64_t)a->n_kv_head * tiles > (1u << 30))
+        return host_fail(HS_UNSUPPORTED, "too many trees times heads");
+    const uint64_t width = (uint64_t)a->n_head * a->cache.head_dim;
+    t.q_stride = a->q_stride ? a->q_stride : width;
+    t.out_stride = a->out_stride ? a->out_stride : width;
+    if (t.q_stride < width || t.out_stride < width)
+        return host_fail(HS_BAD_ARGUMENT, "q_stride or out_stride is less than a row");
+    t.rule = rule->view;
+    t.q = a->q;
+    t.out = a->out;
+    t.seqs = reinterpret_cast<const TreeSeq*>(a->seqs);
+    t.mask = a->mask;
+    t.plane0 = a->plane0;
+    t.n_rows = a->n_rows;
+    t.n_seq = a->n_seq;
+    t.n_head = (int)a->n_head;
+    t.n_kv = (int)a->n_kv_head;
+    t.max_count = (int)a->max_count;
+    t.max_keys = (int)a->max_keys;
+    t.mask_words = (int)a->mask_words;
+    *out = t;
+    return HS_OK;
+}
+
+int beam_args(const hs_weight_rule* rule, const hs_beam_select* a, BeamArgs* out) {
+    const int o = rule->dev.ordinal;
+    if (a->groups == 0 || a->keep == 0) return HS_OK;
+    int rc;
+    if ((rc = need_array(a->dist, o, "dist")) || (rc = need_array(a->tops, o, "tops")) ||
+        (rc = need_array(a->base, o, "base")) || (rc = need_array(a->parent, o, "parent")) ||
+        (rc = need_array(a->token, o, "token")) || (rc = need_array(a->cost, o, "cost")) ||
+        (a->finished && (rc = need_array(a->finished, o, "finished"))))
+        return rc;
+    if (a->tile_shift != 6 && a->tile_shift != 7) return host_fail(HS_UNSUPPORTED, "tile_shift must be 6 or 7");
+    if (a->vocab < 2 || a->vocab > (uint32_t)MAX_CODER_VOCAB)
+        return host_fail(HS_UNSUPPORTED, "the vocabulary needs 2 to 65536 symbols");
+    if (a->beams == 0 || a->beams > HS_MAX_BEAMS) return host_fail(HS_UNSUPPORTED, "a group has 1 to 32 beams");
+    if (a->keep > HS_MAX_KEEP) return host_fail(HS_UNSUPPORTED, "keep is more than 64");
+    if (a->groups > (1u << 24)) return host_fail(HS_UNSUPPORTED, "too many groups");
+    if (rule->first > UINT64_MAX / a->vocab)
+        return host_fail(HS_UNSUPPORTED, "vocab times the largest weight does not fit in 64 bits");
+    const uint64_t tiles = (a->vocab + (1u << a->tile_shift) - 1) >> a->tile_shift;
+    BeamArgs b{};
+    b.dist_stride = a->dist_stride ? a->dist_stride : a->vocab;
+    b.tops_stride = a->tops_stride ? a->tops_stride : tiles;
+    if (b.dist_stride < a->vocab || b.tops_stride < tiles)
+        return host_fail(HS_BAD_ARGUMENT, "dist_stride or tops_stride is less than a row");
+    b.dist = a->dist;
+    b.tops = a->tops;
+    b.base = a->base;
+    b.finished = a->finished;
+    b.parent = a->parent;
+    b.token = a->token;
+    b.cost = a->cost;
+    b.table = rule->table;
+    b.high = rule->high;
+    b.tlen = rule->len;
+    b.last_weight = rule->last_weight;
+    b.cut_bits = weight_cut_bits(rule->first);
+    b.first = rule->first;
+    b.tsh = (int)a->tile_shift;
+    b.vocab = (int)a->vocab;
+    b.groups = (int)a->groups;
+    b.beams = (int)a->beams;
+    b.keep = (int)a->keep;
+    *out = b;
+    return HS_OK;
+}
+
+int reorder_args(const DevInfo& d, const hs_cache_reorder* a, CacheView* out) {
+    if (a->groups == 0 || a->beams == 0) return HS_OK;
+    CacheView c;
+    int rc;
+    if ((rc = cache_view(a->cache, d.ordinal, &c)) || (rc = need_array(a->parents, d.ordinal, "parents")) ||
+        (rc = need_array(a->rows, d.ordinal, "rows")) ||
+        (a->slots && (rc = need_array(a->slots, d.ordinal, "slots"))))
+        return rc;
+    if (a->beams > HS_MAX_BEAMS) return host_fail(HS_UNSUPPORTED, "a group has 1 to 32 beams");
+    if ((uint64_t)a->groups * a->beams > a->cache.slots)
+        return host_fail(HS_BAD_ARGUMENT, "more beams than the cache has slots");
+    *out = c;
+    return HS_OK;
+}
+
+int commit_args(const DevInfo& d, const hs_cache_commit* a, CacheView* out) {
+    if (a->n_seq == 0) return HS_OK;
+    CacheView c;
+    int rc;
+    if ((rc = cache_view(a->cache, d.ordinal, &c)) || (rc = need_array(a->seqs, d.ordinal, "seqs")) ||
+        (rc = need_array(a->path, d.ordinal, "path")) || (rc = need_array(a->lengths, d.ordinal, "lengths")))
+        return rc;
+    if (a->n_seq > a->cache.slots) return host_fail(HS_BAD_ARGUMENT, "more trees than the cache has slots");
+    *out = c;
+    return HS_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -217,49 +335,19 @@ void hs_attn_rule_free(hs_attn_rule* rule) {
     delete rule;
 }
 
+int hs_op_tree_attention_check(const hs_attn_rule* rule, const hs_tree_attention* a) {
+    if (!rule || !a) return host_fail(HS_BAD_ARGUMENT, "null argument");
+    TreeArgs t{};
+    return guarded([&]() -> int { return tree_args(rule, a, &t); });
+}
+
 int hs_op_tree_attention(hs_attn_rule* rule, const hs_tree_attention* a, void* stream) {
     if (!rule || !a) return host_fail(HS_BAD_ARGUMENT, "null argument");
     return guarded([&]() -> int {
-        const int o = rule->dev.ordinal;
-        if (a->n_seq == 0 || a->n_rows == 0 || a->max_count == 0) return HS_OK;
         TreeArgs t{};
-        int rc;
-        if ((rc = cache_view(a->cache, o, &t.cache)) || (rc = need_array(a->q, o, "q")) ||
-            (rc = need_array(a->out, o, "out")) || (rc = need_array(a->seqs, o, "seqs")) ||
-            (rc = need_array(a->mask, o, "mask")))
-            return rc;
-        if (a->n_head == 0 || a->n_head > 65535 || a->n_kv_head == 0 || a->n_head % a->n_kv_head != 0)
-            return host_fail(HS_UNSUPPORTED, "n_head must be a multiple of n_kv_head");
-        if (a->plane0 > a->cache.planes || a->n_kv_head > a->cache.planes - a->plane0)
-            return host_fail(HS_BAD_ARGUMENT, "the layer's planes lie outside the cache");
-        if (a->max_count > HS_MAX_TREE) return host_fail(HS_UNSUPPORTED, "a tree has at most 128 nodes");
-        if (a->max_keys == 0 || a->max_keys > a->cache.n_ctx || a->max_count > a->max_keys)
-            return host_fail(HS_BAD_ARGUMENT, "max_keys must be max_count to n_ctx");
-        if (a->mask_words > 1024 || (uint64_t)a->mask_words * 32 < a->max_count)
-            return host_fail(HS_BAD_ARGUMENT, "the mask has too few words for max_count nodes");
-        if (a->n_seq > (1u << 20) || a->n_rows > (1u << 27)) return host_fail(HS_UNSUPPORTED, "too many trees or rows");
-        const uint64_t tiles = ((uint64_t)a->max_count * (a->n_head / a->n_kv_head) + 15) / 16;
-        if (a->n_seq * (uint64_t)a->n_kv_head * tiles > (1u << 30))
-            return host_fail(HS_UNSUPPORTED, "too many trees times heads");
-        const uint64_t width = (uint64_t)a->n_head * a->cache.head_dim;
-        t.q_stride = a->q_stride ? a->q_stride : width;
-        t.out_stride = a->out_stride ? a->out_stride : width;
-        if (t.q_stride < width || t.out_stride < width)
-            return host_fail(HS_BAD_ARGUMENT, "q_stride or out_stride is less than a row");
-        t.rule = rule->view;
-        t.q = a->q;
-        t.out = a->out;
-        t.seqs = reinterpret_cast<const TreeSeq*>(a->seqs);
-        t.mask = a->mask;
-        t.plane0 = a->plane0;
-        t.n_rows = a->n_rows;
-        t.n_seq = a->n_seq;
-        t.n_head = (int)a->n_head;
-        t.n_kv = (int)a->n_kv_head;
-        t.max_count = (int)a->max_count;
-        t.max_keys = (int)a->max_keys;
-        t.mask_words = (int)a->mask_words;
-        return launch(o, stream, "the tree attention", [&](cudaStream_t st) {
+        const int rc = tree_args(rule, a, &t);
+        if (rc || t.n_seq == 0) return rc;
+        return launch(rule->dev.ordinal, stream, "the tree attention", [&](cudaStream_t st) {
             return launch_tree_attention(t, rule->dev.num_sms, rule->dev.op_err, st);
         });
     });
@@ -303,85 +391,55 @@ void hs_weight_rule_free(hs_weight_rule* rule) {
     delete rule;
 }
 
+int hs_op_beam_select_check(const hs_weight_rule* rule, const hs_beam_select* a) {
+    if (!rule || !a) return host_fail(HS_BAD_ARGUMENT, "null argument");
+    BeamArgs b{};
+    return guarded([&]() -> int { return beam_args(rule, a, &b); });
+}
+
 int hs_op_beam_select(hs_weight_rule* rule, const hs_beam_select* a, void* stream) {
     if (!rule || !a) return host_fail(HS_BAD_ARGUMENT, "null argument");
     return guarded([&]() -> int {
-        const int o = rule->dev.ordinal;
-        if (a->groups == 0 || a->keep == 0) return HS_OK;
-        int rc;
-        if ((rc = need_array(a->dist, o, "dist")) || (rc = need_array(a->tops, o, "tops")) ||
-            (rc = need_array(a->base, o, "base")) || (rc = need_array(a->parent, o, "parent")) ||
-            (rc = need_array(a->token, o, "token")) || (rc = need_array(a->cost, o, "cost")) ||
-            (a->finished && (rc = need_array(a->finished, o, "finished"))))
-            return rc;
-        if (a->tile_shift != 6 && a->tile_shift != 7) return host_fail(HS_UNSUPPORTED, "tile_shift must be 6 or 7");
-        if (a->vocab < 2 || a->vocab > (uint32_t)MAX_CODER_VOCAB)
-            return host_fail(HS_UNSUPPORTED, "the vocabulary needs 2 to 65536 symbols");
-        if (a->beams == 0 || a->beams > HS_MAX_BEAMS) return host_fail(HS_UNSUPPORTED, "a group has 1 to 32 beams");
-        if (a->keep > HS_MAX_KEEP) return host_fail(HS_UNSUPPORTED, "keep is more than 64");
-        if (a->groups > (1u << 24)) return host_fail(HS_UNSUPPORTED, "too many groups");
-        if (rule->first > UINT64_MAX / a->vocab)
-            return host_fail(HS_UNSUPPORTED, "vocab times the largest weight does not fit in 64 bits");
-        const uint64_t tiles = (a->vocab + (1u << a->tile_shift) - 1) >> a->tile_shift;
         BeamArgs b{};
-        b.dist_stride = a->dist_stride ? a->dist_stride : a->vocab;
-        b.tops_stride = a->tops_stride ? a->tops_stride : tiles;
-        if (b.dist_stride < a->vocab || b.tops_stride < tiles)
-            return host_fail(HS_BAD_ARGUMENT, "dist_stride or tops_stride is less than a row");
-        b.dist = a->dist;
-        b.tops = a->tops;
-        b.base = a->base;
-        b.finished = a->finished;
-        b.parent = a->parent;
-        b.token = a->token;
-        b.cost = a->cost;
-        b.table = rule->table;
-        b.high = rule->high;
-        b.tlen = rule->len;
-        b.last_weight = rule->last_weight;
-        b.cut_bits = weight_cut_bits(rule->first);
-        b.first = rule->first;
-        b.tsh = (int)a->tile_shift;
-        b.vocab = (int)a->vocab;
-        b.groups = (int)a->groups;
-        b.beams = (int)a->beams;
-        b.keep = (int)a->keep;
-        return launch(o, stream, "the beam selection",
+        const int rc = beam_args(rule, a, &b);
+        if (rc || b.groups == 0) return rc;
+        return launch(rule->dev.ordinal, stream, "the beam selection",
                       [&](cudaStream_t st) { return launch_beam_select(b, rule->dev.num_sms, st); });
     });
+}
+
+int hs_op_cache_reorder_check(hs_dev* dev, const hs_cache_reorder* a) {
+    if (!dev || !a) return host_fail(HS_BAD_ARGUMENT, "null argument");
+    CacheView c{};
+    return guarded([&]() -> int { return reorder_args(dev_info(dev), a, &c); });
 }
 
 int hs_op_cache_reorder(hs_dev* dev, const hs_cache_reorder* a, void* stream) {
     if (!dev || !a) return host_fail(HS_BAD_ARGUMENT, "null argument");
     return guarded([&]() -> int {
         const DevInfo d = dev_info(dev);
-        if (a->groups == 0 || a->beams == 0) return HS_OK;
-        CacheView c;
-        int rc;
-        if ((rc = cache_view(a->cache, d.ordinal, &c)) || (rc = need_array(a->parents, d.ordinal, "parents")) ||
-            (rc = need_array(a->rows, d.ordinal, "rows")) ||
-            (a->slots && (rc = need_array(a->slots, d.ordinal, "slots"))))
-            return rc;
-        if (a->beams > HS_MAX_BEAMS) return host_fail(HS_UNSUPPORTED, "a group has 1 to 32 beams");
-        if ((uint64_t)a->groups * a->beams > a->cache.slots)
-            return host_fail(HS_BAD_ARGUMENT, "more beams than the cache has slots");
+        CacheView c{};
+        const int rc = reorder_args(d, a, &c);
+        if (rc || !c.k) return rc;
         return launch(d.ordinal, stream, "the cache reorder", [&](cudaStream_t st) {
             return launch_cache_reorder(c, a->slots, a->parents, a->rows, a->groups, a->beams, d.num_sms, d.op_err, st);
         });
     });
 }
 
+int hs_op_cache_commit_check(hs_dev* dev, const hs_cache_commit* a) {
+    if (!dev || !a) return host_fail(HS_BAD_ARGUMENT, "null argument");
+    CacheView c{};
+    return guarded([&]() -> int { return commit_args(dev_info(dev), a, &c); });
+}
+
 int hs_op_cache_commit(hs_dev* dev, const hs_cache_commit* a, void* stream) {
     if (!dev || !a) return host_fail(HS_BAD_ARGUMENT, "null argument");
     return guarded([&]() -> int {
         const DevInfo d = dev_info(dev);
-        if (a->n_seq == 0) return HS_OK;
-        CacheView c;
-        int rc;
-        if ((rc = cache_view(a->cache, d.ordinal, &c)) || (rc = need_array(a->seqs, d.ordinal, "seqs")) ||
-            (rc = need_array(a->path, d.ordinal, "path")) || (rc = need_array(a->lengths, d.ordinal, "lengths")))
-            return rc;
-        if (a->n_seq > a->cache.slots) return host_fail(HS_BAD_ARGUMENT, "more trees than the cache has slots");
+        CacheView c{};
+        const int rc = commit_args(d, a, &c);
+        if (rc || !c.k) return rc;
         return launch(d.ordinal, stream, "the cache commit", [&](cudaStream_t st) {
             return launch_cache_commit(c, reinterpret_cast<const TreeSeq*>(a->seqs), a->path, a->lengths, a->n_seq,
                                        a->path_stride, d.op_err, st);

@@ -164,3 +164,160 @@ def test_a_reorder_of_one_beam_is_checked_by_its_kernel(fake):
     """Groups of one beam have nothing to move, but a parent out of range is reported: the launch is made, as it is
     counted."""
     there(fake, reorders_of_one_beam)
+
+
+# ---- the tensors of the device-resident operators ----
+
+
+class Ops:
+    """Calls with good tensors on the stand-in device; a test changes one of them."""
+
+    def __init__(self):
+        self.rt = rt = fake_cuda.Runtime()
+        self.dev = B.CudaDevice(0)
+        t = self.t = lambda shape, dtype, strides=None: fake_cuda.Tensor(rt, shape, dtype, strides)
+        self.attn = B.AttnRule(self.dev, 1, 1, 1, 1, 30, [3, 2, 1])
+        self.weights = B.WeightRule(self.dev, [3, 2, 1])
+        # 3 slots of 4 planes of 32 rows of 16; 2 trees of up to 5 nodes; 2 groups of 3 beams over 300 symbols.
+        self.cache = dict(k=t((3, 4, 32, 16), "int8"), v=t((3, 4, 16, 32), "int8"), slots=3, planes=4, n_ctx=32, head_dim=16)
+        self.tree = dict(heads=8, kv_heads=4, q=t((10, 8, 16), "int8"), out=t((10, 8, 16), "int8"), rows=10,
+                         seqs=t((2, 4), "int32"), n_seq=2, max_count=5, max_keys=30, mask=t((10, 1), "int32"), mask_words=1)
+        self.beam = dict(dist=t((6, 512), "int16"), tops=t((6, 3), "int64"), vocab=300, groups=2, beams=3, keep=4,
+                         base=t((6,), "int64"), parent=t((2, 4), "int32"), token=t((2, 4), "int32"),
+                         cost=t((2, 4), "int64"), finished=t((6,), "uint8"))
+        self.reorder = dict(groups=1, beams=3, parent=t((1, 3), "int32"), rows=t((1, 3), "int32"), slots=t((1, 3), "int32"))
+        self.commit = dict(seqs=t((2, 4), "int32"), n_seq=2, path=t((2, 5), "int32"), path_ld=5, length=t((2,), "int32"))
+
+    def run(self, op, cache=None, **kw):
+        """The launches of a call."""
+        self.rt.clear()
+        c = B.KvCache(**{**self.cache, **(cache or {})})
+        if op == "tree":
+            call = B.TreeAttention(self.attn, c, **{**self.tree, **kw})
+        elif op == "beam":
+            call = B.BeamSelect(self.weights, **{**self.beam, **kw})
+        elif op == "reorder":
+            call = B.CacheReorder(self.dev, c, **{**self.reorder, **kw})
+        else:
+            call = B.CacheCommit(self.dev, c, **{**self.commit, **kw})
+        for _ in range(2):
+            call.run()
+        return len(self.rt.launches())
+
+    def refused(self, op, cache=None, code=B.HS_BAD_ARGUMENT, **kw):
+        with pytest.raises(B.HardShellError) as e:
+            self.run(op, cache, **kw)
+        assert e.value.code == code, str(e.value)
+        assert not self.rt.launches(), kw
+
+
+def tensors_that_do_not_fit():
+    o = Ops()
+    t = o.t
+    for op in ("tree", "beam", "reorder", "commit"):
+        assert o.run(op) == 2
+        for name, x in {**o.cache, **getattr(o, op)}.items() if op != "beam" else o.beam.items():
+            if not hasattr(x, "shape"):
+                continue
+            inside = name in ("k", "v")
+            wrong = {"int8": ("uint8", "int16", "float16"), "int32": ("int64", "float32", "int16"),
+                     "int16": ("int32", "bfloat16"), "int64": ("int32", "float64"), "uint8": ("int32", "float32")}
+            bad = [t(x.shape, d) for d in wrong[x.dtype.rsplit(".")[-1]]]           # another type
+            if name != "dist":  # (whose rows are longer than the vocabulary)
+                bad.append(t(x.shape[:-1] + (x.shape[-1] - 1,), x.dtype[6:]))           # too short
+            bad.append(t((0,) + x.shape[1:], x.dtype[6:]))                              # empty
+            if len(x.shape) > 1:
+                if x.shape[0] > 1:
+                    bad.append(t((x.shape[0] - 1,) + x.shape[1:], x.dtype[6:]))
+                    if name not in ("dist", "tops"):  # (whose strides are the tensors' own)
+                        bad.append(t(x.shape, x.dtype[6:], (x.strides[0] + 16,) + x.strides[1:]))  # a view with gaps
+                    bad.append(t(x.shape, x.dtype[6:], (0,) + x.strides[1:]))                 # one row, expanded
+                if x.shape[0] > 1 and x.shape[-1] > 1:
+                    turned = list(x.strides)
+                    turned[0], turned[-1] = 1, x.shape[0] * 700
+                    bad.append(t(x.shape, x.dtype[6:], turned))                               # transposed
+            else:
+                bad.append(t(x.shape, x.dtype[6:], (2,)))                                     # every other element
+            for y in bad:
+                if inside:
+                    o.refused(op, {name: y})
+                else:
+                    o.refused(op, **{name: y})
+
+
+def test_tensors_that_do_not_hold_what_a_call_reads_are_refused(fake):
+    """Another type, too few elements, gaps, expanded and transposed views of each tensor of each operator: an error,
+    and nothing is launched."""
+    there(fake, tensors_that_do_not_fit)
+
+
+def caches_that_do_not_fit():
+    o = Ops()
+    t = o.t
+    for op in ("tree", "reorder", "commit"):
+        o.refused(op, dict(v=t((3, 4, 32, 16), "int8")))               # values that are not transposed
+        o.refused(op, dict(k=t((3, 4, 16, 32), "int8")))
+        o.refused(op, dict(k=t((3, 4, 32, 16), "int8", (2048, 512, 1, 32))))   # a transposed view
+        o.refused(op, dict(slots=4))
+        o.refused(op, dict(slot_stride=2064))
+        # A batch's planes of a larger cache: its slots are slot_stride apart.
+        part = {n: t(o.cache[n].shape, "int8", (5 * 512, 512) + o.cache[n].strides[2:]) for n in ("k", "v")}
+        o.refused(op, part)
+        assert o.run(op, dict(part, slot_stride=5 * 512)) == 2
+        flat = {n: t((3 * 2048,), "int8") for n in ("k", "v")}
+        assert o.run(op, flat) == 2
+        assert o.run(op, {n: o.cache[n].data_ptr() for n in ("k", "v")}) == 2  # addresses are taken as they are
+
+
+def test_caches_that_do_not_fit_are_refused(fake):
+    there(fake, caches_that_do_not_fit)
+
+
+def views_that_fit():
+    o = Ops()
+    t = o.t
+    # q of a row of q, k and v; outputs with room behind each row.
+    assert o.run("tree", q=t((10, 8, 16), "int8", (384, 16, 1)), q_stride=384) == 2
+    o.refused("tree", q=t((10, 8, 16), "int8", (384, 16, 1)))
+    o.refused("tree", q=t((10, 8, 16), "int8", (384, 16, 1)), q_stride=256)
+    assert o.run("tree", out=t((10, 128), "int8", (144, 1)), out_stride=144) == 2
+    assert o.run("tree", q=t((40, 128), "int8"), q_stride=512) == 2
+    o.refused("tree", q=t((36, 128), "int8"), q_stride=512)
+    assert o.run("tree", seqs=t((9, 4), "int32"), mask=t((640,), "uint32")) == 2
+    # Logits by group and beam, parts of longer rows, and one row as a vector.
+    assert o.run("beam", dist=t((2, 3, 512), "uint16"), tops=t((2, 3, 3), "int64")) == 2
+    assert o.run("beam", dist=t((6, 300), "int16", (1000, 1)), tops=t((2, 3, 3), "int64", (12, 4, 1))) == 2
+    o.refused("beam", dist=t((2, 3, 300), "int16", (4000, 1000, 1)))   # the groups are not 3 rows apart
+    o.refused("beam", dist=t((2, 2, 512), "int16"))
+    o.refused("beam", dist=t((6, 512), "int16"), dist_stride=600)
+    assert o.run("beam", dist=t((300,), "int16"), tops=t((3,), "int64"), groups=1, beams=1) == 2
+    assert o.run("beam", finished=t((2, 3), "bool")) == 2
+    assert o.run("beam", finished=None) == 2
+    # Nothing to do: nothing is looked at.
+    assert o.run("tree", n_seq=0, q=t((1,), "int64")) == 0
+    assert o.run("beam", keep=0, dist=None) == 0
+    assert o.run("reorder", groups=0, parent=None) == 0
+    assert o.run("commit", n_seq=0, path=None) == 0
+
+
+def test_views_that_hold_what_a_call_reads_are_taken(fake):
+    there(fake, views_that_fit)
+
+
+def refusals_of_the_library_first():
+    o = Ops()
+    # What the library refuses keeps its code, whatever the tensors are.
+    small = o.t((1,), "float32")
+    o.refused("tree", code=B.HS_UNSUPPORTED, heads=7, q=small)
+    o.refused("tree", dict(n_ctx=8193, k=small), code=B.HS_UNSUPPORTED)
+    o.refused("beam", code=B.HS_UNSUPPORTED, keep=65)
+    o.refused("beam", code=B.HS_UNSUPPORTED, vocab=65537)
+    o.refused("reorder", code=B.HS_UNSUPPORTED, beams=33)
+    o.refused("reorder", groups=2)
+    o.refused("commit", n_seq=4)
+    for name in ("q", "out", "seqs", "mask"):
+        o.refused("tree", **{name: None})
+
+
+def test_the_library_refuses_first(fake):
+    there(fake, refusals_of_the_library_first)
