@@ -911,7 +911,7 @@ int run(hs_batch* b, const uint32_t* slots, const uint32_t* tokens, const uint32
         if ((rc = dalloc(&b->weights, (size_t)b->Rcap * c.V, b->owned))) return rc;
         b->bytes += (uint64_t)b->Rcap * c.V * 8;
     }
-    b->tree.clear();
+    if (n) b->tree.clear();
     Planner plan(b, slots, tokens, n, b->hist_work);
     auto& passes = plan.passes;
     // Coder answers: pass k uses half k & 1 of the host buffers, and the host prepares pass k + 1
@@ -1346,7 +1346,7 @@ int truncate_slot(hs_batch* b, uint32_t slot, uint64_t len) {
     const uint64_t drop = ss.len - len;
     const uint64_t here = pos > ss.first ? pos - ss.first : 0;
     if (drop <= here) {
-        b->tree.clear();
+        b->tree.trees.clear();  // (no rows run: the tables stay for hs_batch_tree_query)
         b->streams[slot].len = (uint32_t)len;
         b->pos[slot] = (int)(pos - drop);
         return HS_OK;
@@ -1657,7 +1657,8 @@ int beam_step(hs_batch* b, uint32_t groups, uint32_t beams, uint32_t* slots, uin
             return rc;
         b->bytes += 37 * Rc;
     }
-    b->tree.clear();
+    if (R) b->tree.clear();
+    else b->tree.trees.clear();
     uint32_t *d_row_of = b->d_beam_u32, *d_slots = d_row_of + Rc, *d_parent = d_slots + Rc, *d_token = d_parent + Rc,
              *d_held = d_token + Rc;
     if (R) {

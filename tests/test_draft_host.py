@@ -145,6 +145,51 @@ def test_a_tree_commit_that_fails_changes_nothing(fake):
     there(fake, tree_commits_that_fail)
 
 
+# ---- the end of trees and tables ----
+
+
+def tables_after_calls_that_run_no_rows():
+    batch = B.CudaBatch(B.CudaModel(B.CudaDevice(0), tiny_bytes()), 4, 64)
+
+    def trees():
+        for s in range(4):
+            batch.reset(s)
+        batch.run_coded([0] * 5, [1] * 5, [0] * 5, [1] * 5)
+        batch.run_tree([0, 0], [1, 2], [-1, 0])
+
+    def gone(f):
+        with pytest.raises(B.HardShellError) as e:
+            f()
+        assert e.value.code == B.HS_BAD_ARGUMENT
+
+    query = lambda: batch.tree_query([0, 1], [0, 0], [1, 2])  # noqa: E731
+    for call, trees_end in ((lambda: batch.truncate(0, 3), True), (lambda: batch.truncate(0, 5), True),
+                            (lambda: batch.tree_commit([0]), True), (lambda: batch.reset(3), False),
+                            (lambda: batch.run_coded([], [], [], []), False), (lambda: batch.run_weights([], []), False),
+                            (lambda: batch.decode_blocks([], [], []), False),
+                            (lambda: batch.beam_step(1, 2, [1, 2], [0, 0], [5, -1], [1, 0]), True)):
+        trees()
+        call()
+        query()
+        if trees_end:
+            gone(lambda: batch.tree_commit([0]))
+        else:
+            batch.tree_commit([0])
+    for call in (lambda: batch.run_coded([3], [1], [0], [1]), lambda: batch.run_weights([3], [1]),
+                 lambda: batch.decode_blocks([3], [b"\0" * 16], [1]),
+                 lambda: batch.beam_step(1, 2, [1, 2], [0, 0], [5, -1])):
+        trees()
+        call()
+        gone(query)
+        gone(lambda: batch.tree_commit([0]))
+
+
+def test_the_tables_of_a_tree_pass_stay_until_rows_run(fake):
+    """A truncation inside the context, a commit, a reset, a call without rows and a step without living beams run
+    nothing: the tables can still be asked."""
+    there(fake, tables_after_calls_that_run_no_rows)
+
+
 # ---- launches of the device-resident operators ----
 
 

@@ -9,6 +9,7 @@ import pytest
 
 import tests.draft_ref as R
 from taco_b200 import backend as B
+from taco_b200 import synth
 from tests.test_gpu_draft_ops import beam_case, dev, gpu, tree_case, tree_op, want_tree  # noqa: F401  (dev: the fixture)
 
 pytestmark = pytest.mark.gpu
@@ -176,3 +177,20 @@ def test_reorder_of_lone_beams(dev, parents, fault):
             dev.check()
     dev.check()
     assert np.array_equal(dk.cpu().numpy(), k) and np.array_equal(dv.cpu().numpy(), v)
+
+
+# ---- a batch ----
+
+
+def test_tables_after_a_truncation(dev):
+    """The tables of a tree pass answer as before once its slot went back inside its context."""
+    model = B.CudaModel(dev, synth.gpt2_hsm(7, shape=synth.MINI))
+    batch = B.CudaBatch(model, 2, 64)
+    batch.run_coded([0] * 9, range(1, 10), [0] * 9, range(1, 10))
+    asks = ([0, 1, 2, 3, 3], [0, 1, 0, 0, 1], [5, 1 << 31, 9, 2, 77])
+    want = batch.run_tree([0] * 4, [11, 12, 13, 14], [-1, 0, 0, 2], *asks)
+    batch.truncate(0, 6)
+    assert np.array_equal(batch.tree_query(*asks), want)
+    batch.run_weights([], [])
+    assert np.array_equal(batch.tree_query(*asks), want)
+    model.close()
