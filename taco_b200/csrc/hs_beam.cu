@@ -359,12 +359,12 @@ __global__ void __launch_bounds__(BT, BEAM_BLOCKS) k_beam_select(const __grid_co
         int N = 0;
         bool border = false;
         if (state == 1) {
-            // The weights without their low bits, from shared memory, give a lower bound of N; entries of
-            // the whole table from there on are tried one at a time.
+            // The weights without their low bits, from shared memory, give a lower bound of N. It is N unless the
+            // whole entry there passes at the upper end of the sum. The entries there are about table[0]^2 / W, at
+            // least table[0] / 2^16, and the bits left out below table[0] / 2^31, so that is rare. Entries of one
+            // value pass together, and may be thousands: none is tried one by one, the row takes the exact way below.
             const uint64_t W = sum_of(b), out = (uint64_t)a.vocab * low, up = W + out < W ? UINT64_MAX : W + out;
             N = norm_of(W, [&](int j) { return (uint64_t)sT[j] << sh.cut_bits; });
-            while (N < a.tlen && (u128)a.table[N] * W > one) N++;
-            // The upper end gives more if the first entry that does not pass would.
             border = N < a.tlen && (u128)a.table[N] * up > one;
         }
         if (lane == 0) {

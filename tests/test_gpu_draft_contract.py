@@ -10,7 +10,7 @@ import pytest
 import tests.draft_ref as R
 from taco_b200 import backend as B
 from taco_b200 import synth
-from tests.test_gpu_draft_ops import beam_case, dev, gpu, tree_case, tree_op, want_tree  # noqa: F401  (dev: the fixture)
+from tests.test_gpu_draft_ops import beam_case, dev, gpu, run_beam, tree_case, tree_op, want_tree  # noqa: F401  (dev: the fixture)
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -131,6 +131,53 @@ def test_the_logits_of_dead_and_finished_beams_need_not_be_there(dev, ended, voc
     for got, x in zip((parent, token, cost), want):
         assert np.array_equal(got.cpu().numpy(), x)
     rule.close()
+
+
+@pytest.mark.parametrize("low", [1, 2, 300, 511])
+@pytest.mark.parametrize("length", [1, 31, 33, 1025, 16000])
+def test_beam_entries_of_one_value(dev, length, low):
+    """Many equal entries that only the low bits of their value let pass."""
+    vocab, top = 1000, 1 << 40
+    c = beam_case(75, 3, 2, vocab)
+    c["dist"][:, :vocab] = 0
+    c["tops"][...] = 0
+    border = top // vocab  # (entries above it pass, as every weight of the rows is the first)
+    for value in (border, border + 1, (border >> 9 << 9) + low):
+        c["table"] = np.array([top] + [value] * length + [3, 2, 1, 0])
+        want = R.norm_of([int(x) for x in c["table"]], vocab * top)
+        assert want == (1 + length if value > border else 1)
+        got = run_beam(dev, c, 2)[2].reshape(3, 2)
+        assert np.array_equal(got, np.sort((c["base"][:, None] + want + np.zeros(2, np.int64)).reshape(3, 4), 1)[:, :2])
+
+
+def test_beam_time_of_entries_of_one_value(dev):
+    """A table with a long run of one value costs what any other of its length does (the run was walked entry by
+    entry, a read from global memory each: thousands of them against a few)."""
+    vocab, top, n = 1000, 1 << 40, 16000
+    c = beam_case(76, 1, 4, vocab)
+    c["dist"][:, :vocab] = 0
+    c["tops"][...] = 0
+    times = []
+    for step in (1000, 0):
+        c["table"] = np.concatenate([[top], top // vocab + 1 - step * np.arange(n)])
+        assert c["table"][-1] > 0
+        rule = B.WeightRule(dev, c["table"])
+        out = [torch.zeros((1, 4), dtype=t, device="cuda") for t in (torch.int32, torch.int32, torch.int64)]
+        op = B.BeamSelect(rule, gpu(c["dist"]), gpu(c["tops"]), vocab, 1, 4, 4, gpu(c["base"]), *out)
+        st = torch.cuda.current_stream()
+        best = []
+        for _ in range(7):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(10):
+                op.run(st.cuda_stream)
+            b.record()
+            b.synchronize()
+            best.append(a.elapsed_time(b))
+        times.append(min(best))
+        dev.check()
+        rule.close()
+    assert times[1] < 5 * times[0], times
 
 
 # ---- moves of cache rows ----
