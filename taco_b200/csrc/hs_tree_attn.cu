@@ -255,9 +255,11 @@ __device__ __forceinline__ uint64_t add_wide(uint64_t sum, uint32_t e) {
 
 // The dots become weights e = table[min(M - score, last)] (0 for keys not seen), summed over the quad's keys.
 // ext: the extremes of the whole rows (lane l has row l % 16). The narrow rules take the distance in one
-// multiply-add: M - floor((dot m + h) / 2^ss) = floor((M 2^ss + 2^ss - 1 - h - dot m) / 2^ss), all below 2^54
-// (M 2^ss is within 2^ss of some dot m); a distance is never negative for a key that is seen, and the unsigned
-// minimum keeps the index inside the table for the others.
+// multiply-add: M - floor((dot m + h) / 2^ss) = floor((M 2^ss + 2^ss - 1 - h - dot m) / 2^ss). With M the score of
+// the dot x and h = 2^(ss - 1), M 2^ss + 2^ss - 1 - h lies in x m .. x m + 2^ss - 1, and |x m|, |dot m| are below 2^52
+// (heads of at most 128): the sum is below 2^53 + 2^ss < 2^63 in magnitude for the shifts up to 62 of these rules. A
+// distance is never negative for a key that is seen, and the unsigned minimum keeps the index inside the table for
+// the others.
 template <int NT, bool NARROW, bool SSHI>
 __device__ __forceinline__ void tree_weigh(int32_t (&c)[NT][4], bool whole, const uint32_t (&seen)[2], int32_t ext,
                                            int32_t m, int ss, const int32_t* table, int last, uint64_t (&sum)[2]) {

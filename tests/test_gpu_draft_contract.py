@@ -10,7 +10,8 @@ import pytest
 import tests.draft_ref as R
 from taco_b200 import backend as B
 from taco_b200 import synth
-from tests.test_gpu_draft_ops import beam_case, dev, gpu, run_beam, tree_case, tree_op, want_tree  # noqa: F401  (dev: the fixture)
+from tests.test_gpu_draft_ops import (RULE, beam_case, check_tree, dev, gpu, run_beam, tree_case, tree_op,  # noqa: F401
+                                      want_tree)
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -73,6 +74,19 @@ def test_bad_records_among_more_trees_than_blocks(dev, n, most, n_ctx, heads):
         dev.check()
     dev.check()
     h.close()
+
+
+@pytest.mark.parametrize("counts,prefixes,n_ctx,hd", [([20], [300], 512, 64), ([20], [1100], 2048, 64), ([9], [600], 1024, 128),
+                                                     ([9], [400], 512, 128), ([9], [90], 256, 64)])
+@pytest.mark.parametrize("score_m", [2**31 - 1, -2**31 + 1])
+@pytest.mark.parametrize("score_s", [31, 32, 48, 51, 52, 53, 54, 61, 62, 63])
+def test_tree_scores_of_large_shifts(dev, counts, prefixes, n_ctx, hd, score_m, score_s):
+    """The distance in one multiply-add, up to the largest shift, with dots at their extremes."""
+    c = tree_case(77, counts, prefixes, n_ctx, hd=hd)
+    r = np.random.default_rng(78)
+    for name in ("q", "k"):
+        c[name][...] = np.where(r.random(c[name].shape[:-1] + (1,)) < 0.5, -128, 127)
+    check_tree(dev, c, dict(RULE, score_m=score_m, score_s=score_s, table=np.arange(200, 0, -1)))
 
 
 # ---- beam selection ----
