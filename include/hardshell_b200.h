@@ -203,8 +203,8 @@ int hs_batch_tree_query(hs_batch* batch, uint32_t n, const uint32_t* nodes, cons
 
 /* The nodes become inputs of their slots, as if hs_batch_run_coded had run their tokens: for each
  * slot a path from its context, each node the parent of the next, the nodes of a slot together.
- * Slots without a node stay as they were before the trees. All trees end. The cache rows move on
- * the GPU without a wait. Nothing changes on an error. */
+ * Slots without a node stay as they were before the trees. All trees end. The call does not wait for
+ * the cache rows that move on the GPU. Nothing changes on an error. */
 int hs_batch_tree_commit(hs_batch* batch, uint32_t n, const uint32_t* nodes);
 
 /* One step of a beam search with the model (a drafter): beam j of group g, i = g * beams + j, runs
@@ -513,7 +513,9 @@ typedef struct hs_tree_seq {
  * plane plane0 + h / (n_head / n_kv_head). q and out are int8 rows of n_head * head_dim, q_stride
  * and out_stride bytes apart (0: dense); rows of no tree stay as they were. count <= max_count <=
  * HS_MAX_TREE and prefix + count <= max_keys <= n_ctx for every tree, 32 * mask_words >= max_count.
- * Trees must not share rows. */
+ * Trees must not share rows. The launch is sized by max_count and max_keys: loose bounds change no
+ * result, but cost time (64 trees of 16 nodes at 200 keys, 12 heads of 64: 27 us with max_keys = 200,
+ * 41 us with 1,024, 272 us with 8,192). */
 typedef struct hs_tree_attention {
     hs_kv_cache cache;
     const int8_t* q;

@@ -14,13 +14,15 @@
 // one are read again (from L2), and each candidate finds its place by counting. The lists and sums go to
 // the first block's shared memory, which adds the normalisers and merges the lists.
 //
-// The sums are one table look-up per symbol, in shared memory at random banks: this bounds the kernel. The
-// look-ups take 32 bits, floor(table[j] / 2^s), so the sum is known to lie in [L 2^s, L 2^s + vocab (2^s -
-// 1)]. N does not decrease with W, so where both ends give one N it is exact; where they differ (W next to
-// a border) the low bits are summed as well.
+// The sums are one table look-up per symbol, in shared memory at random banks (about 5,500 cycles a row: 39 us of
+// the 256 groups below; the rest is the barriers and phases of a row). The look-ups take 32 bits, floor(table[j] /
+// 2^s), so the sum is known to lie in [L 2^s, L 2^s + vocab (2^s - 1)]. N does not decrease with W, so where both
+// ends give one N it is exact; where they differ (W next to a border) the low bits are summed as well.
 //
-// Measured (vocabulary 50257): 256 groups of 8 beams 99 us, a third of HBM's rate (212 MB of distances); 64
-// groups 31 us from L2, 39 us cold; one group of 4 beams 12 to 15 us, the latency of its six phases.
+// Measured (vocabulary 50257, repeated calls): 256 groups of 8 beams 108 us, 30 % of HBM's rate (206 MB of
+// distances); 64 groups 30 us from L2; one group of 4 beams 12 us, the latency of its six phases. With L2 flushed
+// before each call 123 and 33 us. A group that holds a row next to a border ends 15 us later (64 groups with one
+// such row 49 us): its first block alone reads that row again.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -69,13 +71,6 @@ struct BeamSmem {
 struct BeamShape {
     int segs, seg_vecs, batches, cut_bits;
 };
-
-// sum + e by the multiply-add pipe: the integer adds of the distances keep the other one.
-__device__ __forceinline__ uint64_t add_wide(uint64_t sum, uint32_t e) {
-    uint64_t r;
-    asm("mad.wide.u32 %0, %1, 1, %2;" : "=l"(r) : "r"(e), "l"(sum));
-    return r;
-}
 
 __device__ __forceinline__ int64_t warp_max8(int64_t v) {  // over lanes 0..7 (and their copies)
     for (int o = 4; o > 0; o >>= 1) {
@@ -204,7 +199,7 @@ __global__ void __launch_bounds__(BT, BEAM_BLOCKS) k_beam_select(const __grid_co
                 e[2 * j + 1] = sT[x[j] >> 16];
             }
 #pragma unroll
-            for (int j = 0; j < 8; j++) sum = add_wide(sum, e[j]);
+            for (int j = 0; j < 8; j++) sum = add_wide(sum, e[j]);  // (the adds of the distances keep the other pipe)
             return __vminu2(__vminu2(x[0], x[1]), __vminu2(x[2], x[3]));
         };
         auto far_of = [&](int s) -> uint32_t {
@@ -471,9 +466,10 @@ cudaError_t launch_beam_select(const BeamArgs& a, int num_sms, cudaStream_t st) 
     if (a.groups == 0) return cudaSuccess;
     // The split: `segs` segments a row and clusters of C blocks, by the time of the segments of the busiest
     // block (a fixed part each, and one that grows with their symbols and with the blocks that share an SM)
-    // and of the end of a group. Measured: 256 groups of 8, one segment, C = 1, 2, 4, 8: 118, 99, 101, 101 us (two
+    // and of the end of a group. Measured by repeated calls: 256 groups of 8, one segment, C = 1, 2, 4, 8: 118, 99, 101, 101 us (two
     // segments 134 at best); 64 groups of 8: 81, 46, 33, 31 us (42); one group of 4: 43, 25, 17, 17 us, two
-    // segments and C = 8 15 us, four 19 us; one lone beam 17 us whole, 11 us in eight segments. The rule takes the best of each, or one within 1 %.
+    // segments and C = 8 15 us, four 19 us; one lone beam 17 us whole, 11 us in eight segments. The rule takes the
+    // best of each, or one within 1 %.
     int C = 1;
     BeamShape sh = beam_shape(a, 1);
     double best = 1e300;

@@ -1,7 +1,8 @@
 // The moves of KV-cache rows: the reordering of the beams' states after a selection and the commit of
 // an accepted path of a draft tree. Both are in place: a thread owns the same bytes of every slot (or
 // row) that takes part, reads all of them before it writes any, so no order of threads matters.
-// Bytes in and out are the only cost (times: B200, 144 planes of 1,024 rows of 64).
+// Bytes in and out are the only cost (times: B200, 144 planes of 1,024 rows of 64, calls repeated on the same
+// caches; in a reorder every beam takes another one's rows, so all of them are read and written).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -45,10 +46,12 @@ __device__ __forceinline__ void put_head(int8_t* to, uint4 v, uint32_t n) {
 // T: the unit of a move (16 bytes where n_ctx and head_dim are multiples of 16, else a byte). B: the
 // most beams of a group. blockIdx.y is the group, blockIdx.x a plane's keys (rows * hd bytes from row 0)
 // or values (the first `rows` bytes of each channel's row): a unit of values may pass the last row, and
-// then goes by parts (byte by byte one group of 8 beams of 300 rows took 30 us, by parts 20).
+// then goes by parts (byte by byte one group of 8 beams of 300 rows took 30 us cold, by parts 20). Caches whose
+// sizes or addresses are no multiples of 16 go by bytes: 32 groups of 4 of 700 rows, n_ctx 1,000, half of the beams
+// living on, 1.64 ms, a group of 8 of 300 rows 55 us.
 //
-// Bound by HBM: 32 groups of 4 beams of 700 rows take 0.56 ms (5.9 TB/s in and out, 90 % of a copy's rate), 16 of
-// 8 0.57, 8 of 16 0.59. The loads of beams that a group does not have cost: the kernel for 32 takes 1.2 ms with
+// Bound by HBM: 32 groups of 4 beams of 700 rows take 0.56 ms (5.9 TB/s in and out, 90 % of a copy's rate; 0.37 to
+// 0.40 where about half of the beams live on), 16 of 8 0.57, 8 of 16 0.61. The loads of beams that a group does not have cost: the kernel for 32 takes 1.2 ms with
 // groups of 4, so there is one for 4, 8, 16 and 32.
 template <typename T, int B>
 __global__ void __launch_bounds__(move_threads(B)) k_cache_reorder(const CacheView c, const uint32_t* slots,
@@ -123,8 +126,9 @@ __global__ void __launch_bounds__(move_threads(B)) k_cache_reorder(const CacheVi
 // path is strictly increasing, so path[j] >= j: taken in ascending runs, all of a run's rows read before
 // any is written, no row is written before it is read. The bytes of a path lie in a few 32-byte sectors of
 // each channel's row of values: that traffic is the cost. A lane takes a path's byte of COMMIT_DEEP channels,
-// all in flight: 64 trees with a path of 8 take 28 us with 32 channels and three blocks an SM, 32 with 16
-// channels and 36 with 64 (paths of 24 of 128 nodes 54, 58, 55 us); the sectors alone would be about 15 us. A
+// all in flight: 64 trees with a path of 8, their sectors in L2, take 28 us with 32 channels and three blocks an
+// SM, 32 with 16 channels and 36 with 64 (paths of 24 of 128 nodes 54, 58, 55 us); from HBM 39 (and 50) us, where the
+// sectors alone would be 17 (25). A byte a lane is what is left: with a path of 8 a quarter of the lanes have one. A
 // warp shared by several channels of short paths is no faster (35 us).
 constexpr int COMMIT_DEEP = 32, COMMIT_WARPS = 8, COMMIT_BLOCKS = 3;
 

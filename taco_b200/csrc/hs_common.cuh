@@ -165,6 +165,13 @@ __device__ __forceinline__ uint64_t isqrt_u128_fast(u128 x) {
 
 // ---- sm_100a PTX wrappers ----
 
+// sum + e by the multiply-add pipe, where the other integer pipe bounds a kernel.
+__device__ __forceinline__ uint64_t add_wide(uint64_t sum, uint32_t e) {
+    uint64_t r;
+    asm("mad.wide.u32 %0, %1, 1, %2;" : "=l"(r) : "r"(e), "l"(sum));
+    return r;
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return (uint32_t)__cvta_generic_to_shared(p);
 }

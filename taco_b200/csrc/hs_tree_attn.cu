@@ -41,7 +41,8 @@ constexpr int ANY_THREADS = 128;
 // The kernel of every head width and alignment: one block per (row, head). Thread j takes the keys
 // j, j + 128, ... for the dots and the weights (kept in shared memory), then a warp takes a channel at
 // a time for the sum over the keys (V^T rows are contiguous). Each row reads its keys again (from L2) and
-// multiplies byte by byte: it is bounded by that, not by HBM.
+// multiplies byte by byte: it is bounded by that, not by HBM (64 trees of 16 nodes at 1,024 keys, 12 heads of 80:
+// 610 us, where 64-wide heads take 51).
 __global__ void __launch_bounds__(ANY_THREADS) k_tree_attention_any(const TreeArgs a, int* err) {
     extern __shared__ __align__(16) uint32_t s_any[];  // [max_keys] dots, then e, then p; then q
     __shared__ int64_t red[ANY_THREADS / 32];
@@ -128,11 +129,12 @@ __global__ void __launch_bounds__(ANY_THREADS) k_tree_attention_any(const TreeAr
 //   (u8 x s8) for each byte plane, the planes joined in 64 bits, O summed over warps and blocks.
 // Whole-number sums in any order: the split changes nothing. O is summed over a block's warps by additions in
 // shared memory (one word a lane and bank; parts of each warp, added up behind two more barriers, took 466 us
-// where this takes 405), and over a cluster's blocks when it is written, while the next item is under way.
+// where this took 405), and over a cluster's blocks when it is written, while the next item is under way.
 //
-// Bound: not HBM (23 % of it at 64 trees of 16 nodes and 1,024 keys, 51 us) but the integer work of a score (about
-// 25 instructions from the product to the probability's planes, one of them a table look-up in shared memory at
-// random banks) and the three latencies of an item that its warps meet at. 16 warps an SM are what 64 scores a
+// Bound: not HBM (23 % of it at 64 trees of 16 nodes and 1,024 keys, 51 us), nor the issue of the integer work of a
+// score (about 25 instructions from the product to the probability's planes, one of them a table look-up in shared
+// memory at random banks; two thirds of the issue slots are empty) but the latencies of an item, which its warps meet
+// at three times and two items an SM do not hide. 16 warps an SM are what 64 scores a
 // thread leave room for; 32 warps of 64 registers took 785 us where 16 of 128 took 560.
 //
 // Operands come straight from global memory in the layout of the fragments. The order of the channels in
@@ -244,13 +246,6 @@ __device__ __forceinline__ void tree_extremes(const int32_t (&c)[NT][4], bool wh
     };
     if (m >= 0) scan([](int32_t x, int32_t y) { return max(x, y); }, INT32_MIN);
     else scan([](int32_t x, int32_t y) { return min(x, y); }, INT32_MAX);
-}
-
-// sum + e on the multiply-add pipe (the other integer pipe bounds these kernels).
-__device__ __forceinline__ uint64_t add_wide(uint64_t sum, uint32_t e) {
-    uint64_t r;
-    asm("mad.wide.u32 %0, %1, 1, %2;" : "=l"(r) : "r"(e), "l"(sum));
-    return r;
 }
 
 // The dots become weights e = table[min(M - score, last)] (0 for keys not seen), summed over the quad's keys.
@@ -758,9 +753,9 @@ struct TreeShape {
 // last warp that has made its scores of a head asks for the next head's keys, the last that has multiplied
 // asks for its values; no warp waits to copy. One block per SM, 16 warps in two groups of 8 that take the
 // 16-row tiles of the head in turn, 128 keys a warp. The groups meet only within themselves, so one multiplies
-// while the other weighs. At 256 trees of 64 nodes and 1,024 keys, 12 heads, 405 us: an SM issues 1.35
-// instructions a cycle (33 %), the tensor pipe is busy 19 %, the integer pipes 21 and 25 %; the warps wait for
-// one another's rows (22 %), for the next instruction's operands (20 %) and for first rows and masks (16 %).
+// while the other weighs. At 256 trees of 64 nodes and 1,024 keys, 12 heads, 415 us: an SM issues 1.35
+// instructions a cycle (34 %), the tensor pipe is busy 20 %, the integer pipes 21 and 25 %; the warps wait for
+// one another's rows (25 %), for the next instruction's operands (20 %) and for first rows and masks (16 %).
 // The exponent table is held up to its last change (table_reach).
 
 constexpr int BK = 1024;                 // keys of a block
@@ -1052,7 +1047,7 @@ cudaError_t configure_bulk() {
     return cudaSuccess;
 }
 
-// Head width, warps, key tiles of a warp. A warp that holds few keys leaves a short context to more warps: 256 keys a
+// Head width, warps, key tiles of a warp (times by repeated calls, 12 heads). A warp that holds few keys leaves a short context to more warps: 256 keys a
 // block of 64-wide heads take 9.4 us (one tree of 8 at 200 keys, 12 heads) and 22.9 us (64 trees of 16 at 256),
 // 1,024 a block 12.9 and 31.2 us. Above that the longer slices win: 64 trees of 16 at 1,024 keys 50 us, 89 us in
 // clusters of four short blocks. Heads of 128, 512 or 1,024 keys a block: one tree of 8 at 512 keys 14.4 and 15.7
