@@ -830,7 +830,7 @@ __global__ void __launch_bounds__(BTHREADS, 1) k_tree_attention_bulk(const __gri
 
     // The copies of the keys (values) of the first work from `work` on that has rows, by one warp.
     auto copy = [&](int work, bool values) {
-        if (*(volatile uint32_t*)&sm.gave_up) return;
+        if (__shfl_sync(0xffffffffu, *(volatile uint32_t*)&sm.gave_up, 0)) return;  // (one answer for the warp)
         for (; work < works; work += stride) {
             const TreeSeq s = a.seqs[work / a.n_kv];
             if (!tree_seq_ok(s, a.n_rows, a.cache.slots, a.max_count, a.max_keys) || s.count == 0) continue;
