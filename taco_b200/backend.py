@@ -1013,18 +1013,19 @@ class _DeviceOp:
         self._check_fn, self._looks = getattr(lib(), name + "_check"), looks
         self._ref = ctypes.byref(args)
 
-    def _first(self):
+    def _first(self, looks):
         """The library's checks, then the tensors'."""
         _check(self._check_fn(self._handle.h, self._ref))
-        for look in self._looks:
+        for look in looks:
             _look(*look)
         self._looks = None
 
     def run(self, stream: int = 0):
         if not self._handle.h:
             raise HardShellError(HS_BAD_ARGUMENT, "the handle is closed")
-        if self._looks is not None:
-            self._first()
+        looks = self._looks  # (another thread's first run may end meanwhile)
+        if looks is not None:
+            self._first(looks)
         rc = self._fn(self._handle.h, self._ref, stream)
         if rc:
             _check(rc)

@@ -349,6 +349,28 @@ def test_views_that_hold_what_a_call_reads_are_taken(fake):
     there(fake, views_that_fit)
 
 
+def two_first_runs():
+    o = Ops()
+    o.rt.clear()
+    call = B.CacheReorder(o.dev, B.KvCache(**o.cache), **o.reorder)
+    check, other = call._check_fn, []
+
+    def checked(handle, args):
+        if not other:  # another thread's first run comes between, and ends first
+            other.append(1)
+            call.run()
+        return check(handle, args)
+
+    call._check_fn = checked
+    call.run()
+    assert len(o.rt.launches()) == 2
+
+
+def test_two_first_runs_of_one_call(fake):
+    """Two threads run an operator for the first time at once: both look it over, both launch."""
+    there(fake, two_first_runs)
+
+
 def refusals_of_the_library_first():
     o = Ops()
     # What the library refuses keeps its code, whatever the tensors are.
