@@ -240,6 +240,84 @@ def test_reorder_of_lone_beams(dev, parents, fault):
     assert np.array_equal(dk.cpu().numpy(), k) and np.array_equal(dv.cpu().numpy(), v)
 
 
+# ---- offsets past 32 bits ----
+
+FAR = 3 << 30  # bytes from a slot to the next
+
+
+@pytest.fixture(scope="module")
+def far_bytes():
+    """Three slots FAR apart; a test's values lie 2^30 bytes behind its keys."""
+    x = torch.empty(2 * FAR + (1 << 30) + (64 << 20), dtype=torch.int8, device="cuda")
+    yield x
+    del x
+    torch.cuda.empty_cache()
+
+
+def far_cache(x, k, v):
+    """The caches k, v in x, slots FAR apart, and a function that reads them back."""
+    slots, planes, n_ctx, hd = k.shape
+    size = planes * n_ctx * hd
+    parts = [[x[at + FAR * s:][:size] for s in range(slots)] for at in (0, 1 << 30)]
+    for part, y in zip(parts, (k, v)):
+        for s in range(slots):
+            part[s].copy_(gpu(y[s].reshape(-1)))
+    cache = B.KvCache(x, x[1 << 30:], slots, planes, n_ctx, hd, FAR)
+    return cache, lambda: [np.stack([p.cpu().numpy() for p in part]).reshape(y.shape) for part, y in zip(parts, (k, v))]
+
+
+@pytest.mark.parametrize("counts,prefixes,n_ctx,hd", [([20, 9], [300, 80], 512, 64), ([9, 3], [90, 200], 256, 64),
+                                                     ([9, 16], [1500, 30], 2048, 128), ([5, 7], [30, 20], 50, 20)])
+def test_trees_of_far_slots(dev, far_bytes, counts, prefixes, n_ctx, hd):
+    c = tree_case(79, counts, prefixes, n_ctx, hd=hd, slots=3)
+    c["seqs"][:, 2] = [2, 1]
+    cache, _ = far_cache(far_bytes, c["k"], c["v"])
+    out = torch.full(c["q"].shape, 99, dtype=torch.int8, device="cuda")
+    h = B.AttnRule(dev, *(RULE[n] for n in ("score_m", "score_s", "out_m", "out_s", "P", "table")))
+    B.TreeAttention(h, cache, 2, 2, gpu(c["q"]), out, out.shape[0], gpu(c["seqs"]), 2, c["max_count"], c["max_keys"],
+                    gpu(c["mask"]), c["mask"].shape[1]).run()
+    dev.check()
+    assert np.array_equal(out.cpu().numpy(), want_tree(c))
+    h.close()
+
+
+@pytest.mark.parametrize("n_ctx,hd", [(64, 16), (50, 20)])
+def test_moves_of_far_slots(dev, far_bytes, n_ctx, hd):
+    r = np.random.default_rng(80)
+    k = r.integers(-128, 128, (3, 3, n_ctx, hd)).astype(np.int8)
+    v = r.integers(-128, 128, (3, 3, hd, n_ctx)).astype(np.int8)
+    parents, rows = np.array([[2, 0, 1]]), np.array([40, 33, 50])
+    cache, back = far_cache(far_bytes, k, v)
+    B.CacheReorder(dev, cache, 1, 3, gpu(parents, np.int32), gpu(rows, np.int32)).run()
+    dev.check()
+    k, v = R.reorder(k, v, np.arange(3), parents, rows, 3)
+    for got, want in zip(back(), (k, v)):
+        assert np.array_equal(got, want)
+    seqs, path, lengths = np.array([[0, 30, 2, 15], [30, 9, 1, 0]]), np.array([[3, 8, 21, 29], [1, 2, 0, 0]]), np.array([4, 2])
+    B.CacheCommit(dev, cache, gpu(seqs, np.int32), 2, gpu(path, np.int32), 4, gpu(lengths, np.int32)).run()
+    dev.check()
+    for got, want in zip(back(), R.commit(k, v, seqs, path, lengths)):
+        assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("odd", [0, 1])
+def test_beams_of_far_rows(dev, far_bytes, odd):
+    """Rows of distances 3 GB apart, by vectors and by symbols."""
+    c = beam_case(81, 1, 3, 1000)
+    stride = FAR // 2 + odd
+    x = far_bytes.view(torch.int16)
+    for i in range(3):
+        x[i * stride:][:1000].copy_(gpu(c["dist"][i, :1000]))
+    rule = B.WeightRule(dev, c["table"])
+    out = [torch.zeros((1, 5), dtype=t, device="cuda") for t in (torch.int32, torch.int32, torch.int64)]
+    B.BeamSelect(rule, x, gpu(c["tops"]), 1000, 1, 3, 5, gpu(c["base"]), *out, dist_stride=stride).run()
+    dev.check()
+    want = R.beam_select(c["dist"], c["tops"], 7, 1000, 3, 5, c["base"], None, c["table"])
+    for got, y in zip(out, want):
+        assert np.array_equal(got.cpu().numpy(), y)
+    rule.close()
+
+
 # ---- a batch ----
 
 
@@ -254,4 +332,19 @@ def test_tables_after_a_truncation(dev):
     assert np.array_equal(batch.tree_query(*asks), want)
     batch.run_weights([], [])
     assert np.array_equal(batch.tree_query(*asks), want)
+    model.close()
+
+
+def test_more_queries_than_rows(dev):
+    """Queries in several chunks of the batch's rows, over and over on the same nodes: each as if asked alone."""
+    model = B.CudaModel(dev, synth.gpt2_hsm(7, shape=synth.MINI))
+    batch = B.CudaBatch(model, 1, 16)
+    r = np.random.default_rng(82)
+    n = 700
+    nodes, kinds = r.integers(0, 9, n), r.integers(0, 2, n)
+    values = np.where(kinds == 0, r.integers(0, model.vocab_size(), n),
+                      r.integers(0, 1 << 32, n))
+    got = batch.run_tree([0] * 9, range(20, 29), [-1, 0, 0, 1, 2, 2, -1, 6, 7], nodes, kinds, values)
+    for i in r.integers(0, n, 40).tolist() + [127, 128, 255, 256, n - 1]:
+        assert batch.tree_query(nodes[i:i + 1], kinds[i:i + 1], values[i:i + 1])[0] == got[i], i
     model.close()
